@@ -92,6 +92,7 @@ class Nf4sBlobEntry(ctypes.Structure):
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
+_F32 = ctypes.c_float
 _TP = ctypes.POINTER(Nf4sTensor)
 SIGNATURES = {
     "nf4s_abi_version": (_I32, []),
@@ -125,6 +126,18 @@ SIGNATURES = {
     "nf4s_gemm_wgrad": (_I32, [_P, _P, _I64, _I64, _I64, _P, _I32, _P]),
     "nf4s_gemm_wgrad_grouped": (_I32, [_P, _P, _P, _I32, _P, _I64, _I64, _I32, _P]),
     "nf4s_rmsnorm_fwd": (_I32, [_P, _P, _I64, _I64, ctypes.c_float, _P, _P, _P]),
+    "nf4s_block_norm_fwd": (_I32, [_P, _P, _P, _P, _P, _F32, _I64, _I64, _F32, _P, _P, _P, _P,
+                                   _P]),
+    "nf4s_block_norm_bwd": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _F32, _I64, _I64,
+                                   _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "nf4s_block_norm_bwd_workspace_size": (_I32, [_I64, _I64, ctypes.POINTER(_I64)]),
+    "nf4s_ckpt8_encode": (_I32, [_P, _I32, _I64, _I64, _P, _P, _P]),
+    "nf4s_ckpt8_decode": (_I32, [_P, _P, _I64, _I64, _P, _I32, _P]),
+    "nf4s_ckpt8_decode_norm": (_I32, [_P, _P, _P, _I64, _I64, _F32, _P, _P, _P, _P]),
+    "nf4s_linear_ce_fwd": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
+    "nf4s_linear_ce_bwd": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I32, _I32,
+                                  _P, _I64, _P]),
+    "nf4s_linear_ce_workspace_size": (_I32, [_I64, _I64, _I64, _I32, ctypes.POINTER(_I64)]),
     "nf4s_host_alloc": (_I32, [_I64, ctypes.POINTER(_P)]),
     "nf4s_host_free": (_I32, [_P]),
     "nf4s_dbuf_create": (_I32, [_I64, ctypes.POINTER(_P)]),

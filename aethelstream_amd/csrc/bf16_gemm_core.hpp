@@ -1,0 +1,377 @@
+// bf16_gemm_core.hpp - the tile product of the loss head's three bf16 GEMMs on
+// gfx950 (MI355X): out[l, r] = sum_k L[l, k] R[r, k], each operand stored
+// either along the reduction (rows of k) or across it (rows of l or r).
+//
+//   logits  X . W^T   both along
+//   dX      P . W     L along, R across
+//   dW      P^T . X   both across
+//
+// Workgroup = 4 waves in 2 x 2, tile = 64 kMT rows (l) x 64 kNT columns (r);
+// each wave owns 32 kMT x 32 kNT in kMT x kNT accumulators of
+// v_mfma_f32_32x32x16_bf16, R as the instruction's first operand: a lane holds
+// one row l of the output and groups of four adjacent columns.
+// Per 64-long step both operands' tiles move into LDS with direct-to-LDS loads,
+// into the stage that step t - 1 used, while step t computes from the other:
+// 2 x 64 KB for 256 x 256.  An operand along the reduction is read with
+// ds_read_b128, 8 consecutive k of one row a lane; one across it with the
+// transposing reads of tr_tile.hpp.
+#pragma once
+
+#include "abi_common.hpp"
+#include "gemm_common.hpp"
+#include "nf4_device.hpp"
+#include "tr_tile.hpp"
+
+namespace nf4s {
+
+constexpr int kGcThreads = 256;
+constexpr int kGcStep = 64;
+
+// One operand of a tile product, `ld` elements a row, from `p`: the tile's first
+// row (along), or the first k row at the tile's first column (across).  `left`
+// bytes from p may be read, a multiple of 16 from each row's start; what lies
+// past them reads as zero.
+struct GcOperand {
+  const uint16_t *p;
+  int64_t ld, left;
+};
+// Along: `rows` rows of k elements (a multiple of 8).  Across: k rows, `cols`
+// elements of each from p on.
+__device__ __forceinline__ GcOperand gc_along(const uint16_t *p, int64_t ld, int64_t rows,
+                                              int64_t k) {
+  return GcOperand{p, ld, rows > 0 ? ((rows - 1) * ld + k) * 2 : 0};
+}
+__device__ __forceinline__ GcOperand gc_across(const uint16_t *p, int64_t ld, int64_t cols,
+                                               int64_t k) {
+  return GcOperand{p, ld, k > 0 ? ((k - 1) * ld + cols) * 2 : 0};
+}
+
+// LDS tile of an operand along the reduction: rows of 128 bytes, 8 units of 16.
+// Unit u of row r lives at physical unit u ^ gc_swz(r): any 8 rows from a
+// multiple of 8 then spread one logical unit over all 32 banks, any 16 from a
+// multiple of 16 over all 64.
+__device__ __forceinline__ int gc_swz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+
+template <int kTiles, bool kAcross>
+struct GcSide {
+  static constexpr int kBytes = 8192 * kTiles;   // of one stage
+  static constexpr int kUnits = 8 * kTiles;      // across: units of a k row
+  static constexpr int kDmas = 2 * kTiles;       // per wave and step
+  static constexpr int kAddrs = kAcross ? kTiles : 4;
+
+  // Lane addresses of the fragment reads: across one per fragment, along one per
+  // sub-step of 16 (fragments are 32 rows = 4096 bytes apart).
+  static __device__ __forceinline__ void read_addrs(uint32_t (&a)[kAddrs], int lane, int half) {
+    if constexpr (kAcross) {
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) a[j] = wg_read_off<kUnits>(lane, half, j);
+    } else {
+      const int row = 32 * kTiles * half + (lane & 31);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        a[s] = (uint32_t)(128 * row + 16 * ((2 * s + (lane >> 5)) ^ gc_swz(row)));
+    }
+  }
+  static __device__ __forceinline__ u32x4 frag(const char *base, const uint32_t (&a)[kAddrs],
+                                               int s, int j) {
+    if constexpr (kAcross)
+      return wg_frag<kUnits>(base, a[j], s);
+    else
+      return *reinterpret_cast<const u32x4 *>(base + a[s] + 4096 * j);
+  }
+
+  // Byte offsets of this wave's DMAs from the operand's place at a step.
+  static __device__ __forceinline__ void dma_offsets(uint32_t (&v)[kDmas], int64_t ld, int lane,
+                                                     int wave) {
+#pragma unroll
+    for (int q = 0; q < kDmas; ++q) {
+      if constexpr (kAcross) {
+        constexpr int kRows = 64 / kUnits;  // k rows per instruction
+        const int r = 16 * wave + kRows * q + lane / kUnits;
+        v[q] = (uint32_t)(r * ld * 2 + 16 * wg_unit(r, lane % kUnits));
+      } else {
+        const int r = 8 * (kDmas * wave + q) + (lane >> 3);
+        v[q] = (uint32_t)(r * ld * 2 + 16 * ((lane & 7) ^ gc_swz(r)));
+      }
+    }
+  }
+  // Along, last step of a reduction that ends inside it: units past the end are
+  // moved out of range, where loads give zero.
+  static __device__ __forceinline__ void mask_tail(uint32_t (&v)[kDmas], int tail, int lane,
+                                                   int wave) {
+    if constexpr (!kAcross) {
+#pragma unroll
+      for (int q = 0; q < kDmas; ++q) {
+        const int r = 8 * (kDmas * wave + q) + (lane >> 3);
+        if (8 * ((lane & 7) ^ gc_swz(r)) >= tail) v[q] = 0x80000000u;
+      }
+    }
+  }
+  // LDS offset of this wave's DMA q.
+  static __device__ __forceinline__ int dma_lds(int q, int wave) {
+    return 1024 * (kDmas * wave + q);
+  }
+};
+
+// The place of an operand at a step: base pointer and bytes from it to the end
+// of what may be read.
+struct GcPlace {
+  const char *p;
+  int64_t left;
+  int64_t step;  // bytes from one step to the next
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
+    const int64_t n = left < 0 ? 0 : (left > 0x7fffffff ? 0x7fffffff : left);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)n, kBufferFlags);
+  }
+  __device__ __forceinline__ void advance() {
+    p += step;
+    left -= step;
+  }
+};
+
+template <int kMT, int kNT, bool kLAcross, bool kRAcross>
+struct GcCore {
+  using LSide = GcSide<kMT, kLAcross>;
+  using RSide = GcSide<kNT, kRAcross>;
+  static constexpr int kTileL = 64 * kMT, kTileR = 64 * kNT;
+  static constexpr int kStageBytes = LSide::kBytes + RSide::kBytes;
+  static constexpr int kLdsBytes = 2 * kStageBytes;
+  static constexpr int kSub = kMT * kNT;       // MFMAs per sub-step
+  static constexpr int kPost = kSub / 2;       // those that open the next step
+  static constexpr int kFront = 4 * kSub - kPost;
+  static constexpr int kReads = kMT + kNT;
+  static constexpr int kDmas = LSide::kDmas + RSide::kDmas;
+  static constexpr int kGap = (kFront - 1) / kDmas >= 2 ? 2 : 1;
+  static_assert(kDmas <= kFront, "one DMA per MFMA slot at most");
+
+  floatx16 acc[kMT][kNT];
+  u32x4 fl[2][kMT], fr[2][kNT];
+  uint32_t al[LSide::kAddrs], ar[RSide::kAddrs];
+  uint32_t vl[LSide::kDmas], vr[RSide::kDmas];
+  GcPlace pl, pr;
+
+  // Fragment read q of a sub-step, in the order its MFMAs use them: l0, r0, r1,
+  // .., l1, ..
+  __device__ __forceinline__ void read(const char *tl, const char *tr, int s, int b, int q) {
+    if (q == 0 || q > kNT) {
+      const int j = q == 0 ? 0 : q - kNT;
+      fl[b][j] = LSide::frag(tl, al, s, j);
+    } else {
+      fr[b][q - 1] = RSide::frag(tr, ar, s, q - 1);
+    }
+  }
+  template <int kI>
+  __device__ __forceinline__ void mfma(int b) {
+    constexpr int mt = kI / kNT, nt = kI % kNT;
+    acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(bf16x8, fr[b][nt]), __builtin_bit_cast(bf16x8, fl[b][mt]), acc[mt][nt],
+        0, 0, 0);
+  }
+  template <int kD>
+  __device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t rl, __amdgpu_buffer_rsrc_t rr,
+                                      char *nl, char *nr, int wave) {
+    if constexpr (kD < LSide::kDmas)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rl, (lds_void_t *)(nl + LSide::dma_lds(kD, wave)), 16, (int)vl[kD], 0, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rr, (lds_void_t *)(nr + RSide::dma_lds(kD - LSide::kDmas, wave)), 16,
+          (int)vr[kD - LSide::kDmas], 0, 0, 0);
+  }
+
+  // One step from stage `cl`/`cr`: the previous step's last kPost MFMAs with
+  // the reads of sub-step 0 between them, then 4 sub-steps of kSub, the
+  // fragments of sub-step s + 1 read during sub-step s, the DMAs of step t + 1
+  // (if `more`) into the other stage between the first MFMAs.  That stage was
+  // last read in step t - 1, whose reads ended before the barrier that closed
+  // it.  The __restrict__ stages tell the compiler that DMAs into one never
+  // alias reads of the other, so that it waits for them at the barriers only.
+  __device__ __forceinline__ void step(const char *__restrict__ cl, const char *__restrict__ cr,
+                                       char *__restrict__ nl, char *__restrict__ nr, bool more,
+                                       int wave) {
+    const __amdgpu_buffer_rsrc_t rl = pl.rsrc(), rr = pr.rsrc();
+    static_for<0, kPost>([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      mfma<kSub - kPost + i>(1);
+      static_for<0, kReads>([&](auto Q) {
+        constexpr int q = decltype(Q)::value;
+        if constexpr (q * kPost / kReads == i) read(cl, cr, 0, 0, q);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    static_for<0, kFront>([&](auto N) {
+      constexpr int n = decltype(N)::value;
+      constexpr int s = n / kSub, i = n % kSub;
+      mfma<i>(s & 1);
+      if constexpr (s < 3) {
+        static_for<0, kReads>([&](auto Q) {
+          constexpr int q = decltype(Q)::value;
+          if constexpr ((q < kSub ? q : kSub - 1) == i) read(cl, cr, s + 1, (s + 1) & 1, q);
+        });
+      }
+      if constexpr (n % kGap == 0 && n / kGap < kDmas) {
+        if (more) dma<n / kGap>(rl, rr, nl, nr, wave);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+
+  // The whole product into acc: k elements of the reduction, lds of kLdsBytes.
+  // With k no multiple of 8, an operand along the reduction holds zeros (and may
+  // be read) up to the next one.
+  __device__ __forceinline__ void run(const GcOperand &l, const GcOperand &r, int64_t k, char *lds,
+                                      int lane, int wave) {
+    char *sl[2] = {lds, lds + kStageBytes};
+    char *sr[2] = {lds + LSide::kBytes, lds + kStageBytes + LSide::kBytes};
+    LSide::read_addrs(al, lane, wave >> 1);
+    RSide::read_addrs(ar, lane, wave & 1);
+    LSide::dma_offsets(vl, l.ld, lane, wave);
+    RSide::dma_offsets(vr, r.ld, lane, wave);
+    pl = place<kLAcross>(l);
+    pr = place<kRAcross>(r);
+    const int nsteps = (int)((k + kGcStep - 1) / kGcStep);
+    const int tail = (int)(k % kGcStep);
+    auto before_last = [&](int t) {  // the next DMAs are the last step's
+      if (tail != 0 && t + 1 == nsteps - 1) {
+        LSide::mask_tail(vl, tail, lane, wave);
+        RSide::mask_tail(vr, tail, lane, wave);
+      }
+    };
+    before_last(-1);
+    if (nsteps > 0) {
+      const __amdgpu_buffer_rsrc_t rl = pl.rsrc(), rr = pr.rsrc();
+      static_for<0, kDmas>(
+          [&](auto D) { dma<decltype(D)::value>(rl, rr, sl[0], sr[0], wave); });
+    }
+    pl.advance();
+    pr.advance();
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[mt][nt][v] = 0.0f;
+    // The first step's opening MFMAs multiply zeros.
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) fl[1][i] = (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) fr[1][i] = (u32x4){0u, 0u, 0u, 0u};
+    step_barrier<0>();
+    int t = 0;
+#pragma unroll 1
+    for (; t + 2 <= nsteps; t += 2) {
+      before_last(t);
+      step(sl[0], sr[0], sl[1], sr[1], true, wave);
+      pl.advance();
+      pr.advance();
+      step_barrier<0>();
+      before_last(t + 1);
+      step(sl[1], sr[1], sl[0], sr[0], t + 2 < nsteps, wave);
+      pl.advance();
+      pr.advance();
+      step_barrier<0>();
+    }
+    if (t < nsteps) {
+      step(sl[0], sr[0], sl[1], sr[1], false, wave);
+      step_barrier<0>();
+    }
+    static_for<0, kPost>([&](auto I) { mfma<kSub - kPost + decltype(I)::value>(1); });
+  }
+
+  template <bool kAcross>
+  static __device__ __forceinline__ GcPlace place(const GcOperand &o) {
+    return GcPlace{reinterpret_cast<const char *>(o.p), o.left,
+                   kAcross ? kGcStep * o.ld * 2 : (int64_t)kGcStep * 2};
+  }
+};
+
+// Tile b of a one-dimensional grid of tiles_l x tiles_r: numbered row by row
+// within strips of `strip` tile columns, each XCD (workgroups b % 8) a
+// contiguous range, so that an XCD's resident workgroups form a patch that
+// shares its operands in that XCD's L2.
+__device__ __forceinline__ void gc_tile(int b, int tiles_l, int tiles_r, int strip, int &tl,
+                                        int &tr) {
+  const int T = tiles_l * tiles_r;
+  const int x = b & 7, base = T >> 3, rem = T & 7;
+  const int n = x * base + (x < rem ? x : rem) + (b >> 3);
+  const int per = tiles_l * strip;
+  const int s = n / per, i = n - s * per;
+  const int left = tiles_r - s * strip;
+  const int w = left < strip ? left : strip;
+  tl = i / w;
+  tr = s * strip + i - tl * w;
+}
+
+// Orders a wave's own LDS writes before its reads of other lanes' values, and
+// those reads before its next writes.
+__device__ __forceinline__ void gc_wave_sync() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+  asm volatile("" ::: "memory");
+}
+
+// Stores 32 rows x 32 kNT columns of a wave as bf16 through its 32 * 64 * kNT
+// bytes of LDS, whole rows of 64 kNT bytes: value(nt, v) is the lane's register
+// v of column tile nt, already final.  `out` points at row 0, column 0 of the
+// block; `rows` and `cols` (a multiple of 8) bound it.
+template <int kNT, class F>
+__device__ __forceinline__ void gc_store_bf16(F &&value, char *lds, uint16_t *out, int64_t ld,
+                                              int64_t rows, int64_t cols, int lane) {
+  constexpr int kChunks = 4 * kNT;  // 16-byte chunks of a row
+  const int row = lane & 31, grp = lane >> 5;
+#pragma unroll
+  for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const u32x2 w = {pack_bf16x2(value(nt, 4 * j), value(nt, 4 * j + 1)),
+                       pack_bf16x2(value(nt, 4 * j + 2), value(nt, 4 * j + 3))};
+      const int c = (4 * nt + j) ^ (row & (kChunks - 1));
+      *reinterpret_cast<u32x2 *>(lds + 16 * kChunks * row + 16 * c + 8 * grp) = w;
+    }
+  gc_wave_sync();
+  constexpr int kRows = 64 / kChunks;  // rows per store instruction
+  const int r0 = lane / kChunks, c = lane % kChunks;
+#pragma unroll
+  for (int i = 0; i < 32 / kRows; ++i) {
+    const int r = kRows * i + r0;
+    const u32x4 w = *reinterpret_cast<const u32x4 *>(lds + 16 * kChunks * r +
+                                                     16 * (c ^ (r & (kChunks - 1))));
+    if (r < rows && 8 * c < cols) *reinterpret_cast<u32x4 *>(out + r * ld + 8 * c) = w;
+  }
+  gc_wave_sync();
+}
+
+// The same for fp32 values, through 32 * 128 * kNT bytes; kAdd: added to what is
+// there.
+template <int kNT, bool kAdd, class F>
+__device__ __forceinline__ void gc_store_f32(F &&value, char *lds, float *out, int64_t ld,
+                                             int64_t rows, int64_t cols, int lane) {
+  constexpr int kChunks = 8 * kNT;
+  const int row = lane & 31, grp = lane >> 5;
+#pragma unroll
+  for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = (8 * nt + 2 * j + grp) ^ (row & (kChunks - 1));
+      *reinterpret_cast<floatx4 *>(lds + 16 * kChunks * row + 16 * c) =
+          (floatx4){value(nt, 4 * j), value(nt, 4 * j + 1), value(nt, 4 * j + 2),
+                    value(nt, 4 * j + 3)};
+    }
+  gc_wave_sync();
+  constexpr int kRows = 64 / kChunks;
+  const int r0 = lane / kChunks, c = lane % kChunks;
+#pragma unroll
+  for (int i = 0; i < 32 / kRows; ++i) {
+    const int r = kRows * i + r0;
+    floatx4 w = *reinterpret_cast<const floatx4 *>(lds + 16 * kChunks * r +
+                                                   16 * (c ^ (r & (kChunks - 1))));
+    if (r < rows && 4 * c < cols) {
+      floatx4 *p = reinterpret_cast<floatx4 *>(out + r * ld + 4 * c);
+      if constexpr (kAdd) w += *p;
+      *p = w;
+    }
+  }
+  gc_wave_sync();
+}
+
+}  // namespace nf4s

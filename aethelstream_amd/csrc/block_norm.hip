@@ -1,0 +1,440 @@
+// block_norm.hip - the norms around a block with its gate and residual scale,
+// forward and backward, for gfx950 (MI355X).
+//
+// Between two blocks of a decoder layer the reference adds the block's output
+// to the residual and norms the sum for the next block
+// (doublepass/src/forward.rs:246-249; rms_norm_fwd and rms_norm_bwd,
+// doublepass/src/math.rs:28-88).  Here that boundary is one kernel, with an
+// optional norm of the block's output, an optional gate per channel and a
+// residual scale:
+//   h^ = h / rms(h),  u = w_post h^          (or h^ = u = h without w_post)
+//   r' = r + alpha gate u                    (gate 1 without one)
+//   y  = w_pre r' / rms(r'),  rms(v) = sqrt(mean(v^2) + eps)
+// The forward reads h (bf16) and r (fp32) and writes r' (fp32) and y (bf16):
+// 12 bytes an element.
+//
+// Backward, from dy (bf16) and the gradient dr' (fp32) that reached r' by the
+// residual path.  With r^ = r' / rms_pre, e = w_pre dy, k = alpha gate w_post:
+//   g  = dr' + (e - r^ mean(e r^)) / rms_pre         = dr
+//   dh = (k g - h^ mean(k g h^)) / rms_post          (k g without w_post)
+//   dw_pre = sum_rows dy r^,  S = sum_rows g h^,
+//   dgate = alpha w_post S,   dw_post = alpha gate S.
+// The gate and the norm's weight share one column sum, as both scale h^.  The
+// second row mean needs g and so the first; it is taken from three sums of one
+// pass, A = sum e r^, B = sum k h^ (dr' + e / rms_pre), C = sum k h^ r^:
+//   sum k g h^ = B - (A / d) C / rms_pre,
+// which costs one barrier a row instead of two.  18 bytes an element, 15.03
+// where r' comes from its 8-bit checkpoint.  Both directions are bound by
+// memory.
+//
+// A thread holds up to 4 (8) chunks of four elements, a workgroup of up to 1024
+// threads a row.  Backward workgroups are persistent: workgroup b takes rows b,
+// b + G, ... and keeps its two column sums in registers, writes them once, and
+// a second kernel adds the G of them in order.
+#include "row_common.hpp"
+
+namespace nf4s {
+
+struct BlockNormFwd {
+  const uint16_t *h;
+  const float *res;
+  const float *w_pre, *w_post, *gate;  // w_post, gate: NULL if absent
+  float alpha, eps;
+  int32_t chunks;  // d / 4
+  float *res_out;  // may be res
+  uint16_t *y;
+  float *rms_pre, *rms_post;
+};
+
+template <int kMaxThreads, int kChunks>
+__global__ void __launch_bounds__(kMaxThreads) block_norm_fwd_kernel(const BlockNormFwd a) {
+  __shared__ float part[2][16];
+  const int64_t base = (int64_t)blockIdx.x * a.chunks;
+  const int threads = (int)blockDim.x;
+  const u32x2 *h = reinterpret_cast<const u32x2 *>(a.h) + base;
+  const floatx4 *res = reinterpret_cast<const floatx4 *>(a.res) + base;
+  const float inv_d = 1.0f / (float)(4 * a.chunks);
+  u32x2 hv[kChunks];
+  floatx4 r[kChunks];
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = (int)threadIdx.x + i * threads;
+    hv[i] = (u32x2){0u, 0u};
+    r[i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < a.chunks) {
+      hv[i] = __builtin_nontemporal_load(h + c);
+      r[i] = __builtin_nontemporal_load(res + c);
+    }
+  }
+  float scale = a.alpha;
+  if (a.w_post != nullptr) {
+    float sum[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const floatx4 v = bf16x4_values(hv[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[0] += v[j] * v[j];
+    }
+    row_block_sum(sum, part[0]);
+    const float rms = __builtin_sqrtf(sum[0] * inv_d + a.eps);
+    if (threadIdx.x == 0) a.rms_post[blockIdx.x] = rms;
+    scale /= rms;
+  }
+  float sum[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = (int)threadIdx.x + i * threads;
+    if (c < a.chunks) {
+      floatx4 u = bf16x4_values(hv[i]) * scale;
+      if (a.w_post != nullptr) u *= reinterpret_cast<const floatx4 *>(a.w_post)[c];
+      if (a.gate != nullptr) u *= reinterpret_cast<const floatx4 *>(a.gate)[c];
+      r[i] += u;
+      __builtin_nontemporal_store(r[i], reinterpret_cast<floatx4 *>(a.res_out) + base + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[0] += r[i][j] * r[i][j];
+    }
+  }
+  row_block_sum(sum, part[1]);
+  const float rms = __builtin_sqrtf(sum[0] * inv_d + a.eps);
+  if (threadIdx.x == 0) a.rms_pre[blockIdx.x] = rms;
+  const float inv = 1.0f / rms;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = (int)threadIdx.x + i * threads;
+    if (c < a.chunks) {
+      const floatx4 o = r[i] * inv * reinterpret_cast<const floatx4 *>(a.w_pre)[c];
+      __builtin_nontemporal_store(bf16x4_pack(o), reinterpret_cast<u32x2 *>(a.y) + base + c);
+    }
+  }
+}
+
+struct BlockNormBwd {
+  const uint16_t *dy;
+  const float *dres;  // NULL: zero
+  const float *res;   // r', or NULL with its checkpoint in codes and scales
+  const uint32_t *codes;
+  const float *scales;
+  const float *rms_pre, *w_pre;
+  const uint16_t *h;  // NULL: no block, y = norm(r') alone
+  const float *rms_post, *w_post, *gate;
+  float alpha;
+  int64_t m;
+  int32_t chunks, blocks;  // d / 4, checkpoint blocks a row
+  float *dres_out;         // may be dres
+  uint16_t *dh;
+  float *part;  // [G][2][d] column sums: dy r^, g h^
+};
+
+// kKeep: the row's operands and the weights stay in registers between the sums
+// and the outputs.  Rows past 16384 elements read them again instead.
+template <int kMaxThreads, int kChunks, bool kH, bool kKeep>
+__global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(const BlockNormBwd a) {
+  __shared__ float part[2][48];
+  const int threads = (int)blockDim.x;
+  const bool post = kH && a.w_post != nullptr;
+  const float inv_d = 1.0f / (float)(4 * a.chunks);
+  const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto weight_pre = [&](int c) { return reinterpret_cast<const floatx4 *>(a.w_pre)[c]; };
+  auto weight_k = [&](int c) {
+    floatx4 k = {a.alpha, a.alpha, a.alpha, a.alpha};
+    if (a.gate != nullptr) k *= reinterpret_cast<const floatx4 *>(a.gate)[c];
+    if (a.w_post != nullptr) k *= reinterpret_cast<const floatx4 *>(a.w_post)[c];
+    return k;
+  };
+  floatx4 wp[kChunks], wk[kChunks], sum_pre[kChunks], sum_h[kChunks];
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = (int)threadIdx.x + i * threads;
+    sum_pre[i] = sum_h[i] = zero;
+    wp[i] = wk[i] = zero;
+    if (kKeep && c < a.chunks) {
+      wp[i] = weight_pre(c);
+      if (kH) wk[i] = weight_k(c);
+    }
+  }
+
+  int turn = 0;
+#pragma unroll 1
+  for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
+    const int64_t base = row * a.chunks;
+    const float inv_pre = 1.0f / a.rms_pre[row];
+    const float inv_post = post ? 1.0f / a.rms_post[row] : 1.0f;
+    floatx4 r[kChunks], g[kChunks];
+    u32x2 dy[kChunks], h[kChunks];
+    auto load = [&](int i, int c) {
+      r[i] = g[i] = zero;
+      dy[i] = h[i] = (u32x2){0u, 0u};
+      if (c < a.chunks) {
+        if (a.res != nullptr)
+          r[i] = reinterpret_cast<const floatx4 *>(a.res)[base + c];
+        else
+          r[i] = ckpt_values(a.codes[base + c], a.scales[row * a.blocks + (c >> kCkptBlockShift)]);
+        if (a.dres != nullptr) g[i] = reinterpret_cast<const floatx4 *>(a.dres)[base + c];
+        dy[i] = reinterpret_cast<const u32x2 *>(a.dy)[base + c];
+        if (kH) h[i] = reinterpret_cast<const u32x2 *>(a.h)[base + c];
+      }
+    };
+    if constexpr (kKeep) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) load(i, (int)threadIdx.x + i * threads);
+    }
+    float s[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int c = (int)threadIdx.x + i * threads;
+      floatx4 p = wp[i], k = wk[i];
+      if constexpr (!kKeep) {
+        load(i, c);
+        p = c < a.chunks ? weight_pre(c) : zero;
+        if (kH) k = c < a.chunks ? weight_k(c) : zero;
+      }
+      const floatx4 rh = r[i] * inv_pre, e = bf16x4_values(dy[i]) * p;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[0] += e[j] * rh[j];
+      if (post) {
+        const floatx4 kh = bf16x4_values(h[i]) * inv_post * k;
+        const floatx4 b = g[i] + e * inv_pre;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[1] += kh[j] * b[j];
+          s[2] += kh[j] * rh[j];
+        }
+      }
+    }
+    row_block_sum(s, part[turn]);
+    turn ^= 1;
+    const float mean_pre = s[0] * inv_d;
+    const float mean_post = (s[1] - mean_pre * s[2] * inv_pre) * inv_d;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int c = (int)threadIdx.x + i * threads;
+      floatx4 p = wp[i], k = wk[i];
+      if constexpr (!kKeep) {
+        load(i, c);
+        p = c < a.chunks ? weight_pre(c) : zero;
+        if (kH) k = c < a.chunks ? weight_k(c) : zero;
+      }
+      if (c >= a.chunks) continue;
+      const floatx4 rh = r[i] * inv_pre, v = bf16x4_values(dy[i]);
+      const floatx4 t = g[i] + (v * p - rh * mean_pre) * inv_pre;
+      sum_pre[i] += v * rh;
+      __builtin_nontemporal_store(t, reinterpret_cast<floatx4 *>(a.dres_out) + base + c);
+      if constexpr (kH) {
+        const floatx4 hh = bf16x4_values(h[i]) * inv_post;
+        sum_h[i] += t * hh;
+        floatx4 o = t * k;
+        if (post) o = (o - hh * mean_post) * inv_post;
+        __builtin_nontemporal_store(bf16x4_pack(o), reinterpret_cast<u32x2 *>(a.dh) + base + c);
+      }
+    }
+  }
+  floatx4 *out = reinterpret_cast<floatx4 *>(a.part) + (int64_t)blockIdx.x * 2 * a.chunks;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = (int)threadIdx.x + i * threads;
+    if (c < a.chunks) {
+      out[c] = sum_pre[i];
+      if (kH) out[a.chunks + c] = sum_h[i];
+    }
+  }
+}
+
+// Adds the workgroups' column sums in order: a workgroup takes 16 chunks of
+// columns, its 16 row groups each every 16th partial, joined through LDS.
+__global__ void __launch_bounds__(256) block_norm_columns_kernel(
+    const float *part, int32_t parts, int32_t chunks, const float *w_post, const float *gate,
+    float alpha, float *dw_pre, float *dw_post, float *dgate) {
+  __shared__ floatx4 lds[16][16];
+  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const int per = (chunks + 15) / 16;
+  const int which = (int)blockIdx.x / per;  // 0: dy r^, 1: g h^
+  const int c = ((int)blockIdx.x - which * per) * 16 + lane;
+  floatx4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < chunks) {
+    const floatx4 *p = reinterpret_cast<const floatx4 *>(part) + (int64_t)which * chunks + c;
+    for (int i = group; i < parts; i += 16) s += p[(int64_t)i * 2 * chunks];
+  }
+  lds[group][lane] = s;
+  __syncthreads();
+  if (group != 0 || c >= chunks) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += lds[i][lane];
+  if (which == 0) {
+    reinterpret_cast<floatx4 *>(dw_pre)[c] = s;
+    return;
+  }
+  s *= alpha;
+  if (dw_post != nullptr) {
+    floatx4 v = s;
+    if (gate != nullptr) v *= reinterpret_cast<const floatx4 *>(gate)[c];
+    reinterpret_cast<floatx4 *>(dw_post)[c] = v;
+  }
+  if (dgate != nullptr) {
+    floatx4 v = s;
+    if (w_post != nullptr) v *= reinterpret_cast<const floatx4 *>(w_post)[c];
+    reinterpret_cast<floatx4 *>(dgate)[c] = v;
+  }
+}
+
+// Threads of a row of `chunks` chunks: four chunks a thread up to 1024 threads,
+// then eight.
+static int row_chunks_per_thread(int64_t chunks) { return chunks <= 4096 ? 4 : 8; }
+static int row_threads(int64_t chunks) {
+  const int64_t per = row_chunks_per_thread(chunks);
+  return (int)(((chunks + per - 1) / per + 63) / 64 * 64);
+}
+
+// Workgroups of the backward: 16 waves a CU, and at least 4 rows each, as every
+// one writes two rows of column sums.
+static int64_t bwd_groups(int64_t m, int64_t d) {
+  const int64_t waves = row_threads(d / 4) / 64;
+  const int64_t most = (int64_t)cu_slots() * (waves >= 16 ? 1 : 16 / waves);
+  const int64_t rows = (m + 3) / 4;
+  return rows < most ? rows : most;
+}
+
+static int32_t row_shape(int64_t m, int64_t d) {
+  if (m < 0 || d <= 0)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "bad block norm shape m=%lld d=%lld", (long long)m,
+                (long long)d);
+  if (d % 4 != 0)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "block norm needs d %% 4 == 0, got %lld",
+                (long long)d);
+  if (d > kMaxRow)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "block norm row of %lld elements is too long",
+                (long long)d);
+  if (m > kMaxThreadsPerLaunch / 1024)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many rows");
+  return NF4S_OK;
+}
+
+}  // namespace nf4s
+
+using namespace nf4s;
+
+extern "C" {
+
+int32_t nf4s_block_norm_fwd(const uint16_t *h, const float *res, const float *w_pre,
+                            const float *w_post, const float *gate, float alpha, int64_t m,
+                            int64_t d, float eps, float *res_out, uint16_t *y, float *rms_pre,
+                            float *rms_post, void *stream) {
+  clear_error();
+  const int32_t rc = row_shape(m, d);
+  if (rc != NF4S_OK || m == 0) return rc;
+  if (h == nullptr || res == nullptr || w_pre == nullptr || res_out == nullptr || y == nullptr ||
+      rms_pre == nullptr || (w_post != nullptr && rms_post == nullptr))
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "NULL buffer");
+  if (!aligned(res, 16) || !aligned(w_pre, 16) || !aligned(w_post, 16) || !aligned(gate, 16) ||
+      !aligned(res_out, 16) || !aligned(h, 8) || !aligned(y, 8) || !aligned(rms_pre, 4) ||
+      !aligned(rms_post, 4))
+    return fail(NF4S_ERR_MISALIGNED,
+                "block norm: fp32 rows and weights must be 16-byte aligned, h and y 8-byte");
+  const BlockNormFwd a{h,   res, w_pre,   w_post, gate,    alpha,
+                       eps, (int32_t)(d / 4), res_out, y,      rms_pre, rms_post};
+  const int threads = row_threads(d / 4);
+  auto *kernel = row_chunks_per_thread(d / 4) == 8 ? block_norm_fwd_kernel<1024, 8>
+                 : threads <= 512                  ? block_norm_fwd_kernel<512, 4>
+                                                   : block_norm_fwd_kernel<1024, 4>;
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)m), dim3(threads), 0, as_stream(stream), a);
+  return check_launch("block_norm_fwd_kernel");
+}
+
+int32_t nf4s_block_norm_bwd_workspace_size(int64_t m, int64_t d, int64_t *bytes) {
+  clear_error();
+  if (bytes == nullptr) return fail(NF4S_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  *bytes = 0;
+  const int32_t rc = row_shape(m, d);
+  if (rc != NF4S_OK) return rc;
+  *bytes = bwd_groups(m, d) * 2 * d * 4;
+  return NF4S_OK;
+}
+
+int32_t nf4s_block_norm_bwd(const uint16_t *dy, const float *dres, const float *res,
+                            const uint8_t *res_codes, const float *res_scales, const float *rms_pre,
+                            const float *w_pre, const uint16_t *h, const float *rms_post,
+                            const float *w_post, const float *gate, float alpha, int64_t m,
+                            int64_t d, float *dres_out, uint16_t *dh, float *dw_pre,
+                            float *dw_post, float *dgate, void *workspace,
+                            int64_t workspace_bytes, void *stream) {
+  clear_error();
+  const int32_t rc = row_shape(m, d);
+  if (rc != NF4S_OK) return rc;
+  if (w_pre == nullptr || dw_pre == nullptr)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "w_pre or dw_pre is NULL");
+  if ((w_post != nullptr) != (dw_post != nullptr) || (gate != nullptr) != (dgate != nullptr))
+    return fail(NF4S_ERR_INVALID_ARGUMENT,
+                "dw_post goes with w_post, and dgate with gate: both or neither");
+  if (!aligned(w_pre, 16) || !aligned(w_post, 16) || !aligned(gate, 16) || !aligned(dw_pre, 16) ||
+      !aligned(dw_post, 16) || !aligned(dgate, 16))
+    return fail(NF4S_ERR_MISALIGNED, "block norm: weights and their gradients must be 16-byte "
+                                     "aligned");
+  const int64_t groups = bwd_groups(m, d);
+  if (m > 0) {
+    const bool coded = res_codes != nullptr;
+    if (dy == nullptr || rms_pre == nullptr || dres_out == nullptr)
+      return fail(NF4S_ERR_INVALID_ARGUMENT, "NULL buffer");
+    if (coded == (res != nullptr) || coded != (res_scales != nullptr))
+      return fail(NF4S_ERR_INVALID_ARGUMENT,
+                  "exactly one of res and res_codes with res_scales must be set");
+    if ((h != nullptr) != (dh != nullptr))
+      return fail(NF4S_ERR_INVALID_ARGUMENT, "dh goes with h: both or neither");
+    if (h == nullptr && (w_post != nullptr || gate != nullptr))
+      return fail(NF4S_ERR_INVALID_ARGUMENT, "w_post and gate need h");
+    if (w_post != nullptr && rms_post == nullptr)
+      return fail(NF4S_ERR_INVALID_ARGUMENT, "w_post needs rms_post");
+    if (!aligned(dres, 16) || !aligned(res, 16) || !aligned(dres_out, 16) || !aligned(dy, 8) ||
+        !aligned(h, 8) || !aligned(dh, 8) || !aligned(res_codes, 4) || !aligned(res_scales, 4) ||
+        !aligned(rms_pre, 4) || !aligned(rms_post, 4))
+      return fail(NF4S_ERR_MISALIGNED,
+                  "block norm: fp32 rows must be 16-byte aligned, dy, h and dh 8-byte");
+    if (workspace == nullptr || workspace_bytes < groups * 2 * d * 4)
+      return fail(NF4S_ERR_INVALID_ARGUMENT, "block norm backward needs %lld workspace bytes",
+                  (long long)(groups * 2 * d * 4));
+    if (!aligned(workspace, 16))
+      return fail(NF4S_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+  }
+  const hipStream_t s = as_stream(stream);
+  const int32_t chunks = (int32_t)(d / 4);
+  if (m > 0) {
+    const BlockNormBwd a{dy,
+                         dres,
+                         res,
+                         reinterpret_cast<const uint32_t *>(res_codes),
+                         res_scales,
+                         rms_pre,
+                         w_pre,
+                         h,
+                         rms_post,
+                         w_post,
+                         gate,
+                         alpha,
+                         m,
+                         chunks,
+                         (int32_t)((d + kCkptBlock - 1) / kCkptBlock),
+                         dres_out,
+                         dh,
+                         static_cast<float *>(workspace)};
+    const int threads = row_threads(chunks);
+    const bool blk = h != nullptr;
+    auto *kernel = blk ? block_norm_bwd_kernel<512, 4, true, true>
+                       : block_norm_bwd_kernel<512, 4, false, true>;
+    if (row_chunks_per_thread(chunks) == 8)
+      kernel = blk ? block_norm_bwd_kernel<1024, 8, true, false>
+                   : block_norm_bwd_kernel<1024, 8, false, false>;
+    else if (threads > 512)
+      kernel = blk ? block_norm_bwd_kernel<1024, 4, true, true>
+                   : block_norm_bwd_kernel<1024, 4, false, true>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)groups), dim3(threads), 0, s, a);
+    const int32_t rc2 = check_launch("block_norm_bwd_kernel");
+    if (rc2 != NF4S_OK) return rc2;
+  }
+  // Over no rows the sums are zero.
+  const bool along = dw_post != nullptr || dgate != nullptr;
+  hipLaunchKernelGGL(block_norm_columns_kernel, dim3((chunks + 15) / 16 * (along ? 2 : 1)),
+                     dim3(256), 0, s, static_cast<const float *>(workspace), (int32_t)groups,
+                     chunks, w_post, gate, alpha, dw_pre, dw_post, dgate);
+  return check_launch("block_norm_columns_kernel");
+}
+
+}  // extern "C"

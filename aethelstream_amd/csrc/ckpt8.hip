@@ -1,0 +1,269 @@
+// ckpt8.hip - activation checkpoints in 8 bits for gfx950 (MI355X).
+//
+// What the first pass of a double-pass step keeps for the second (the
+// reference keeps per-channel int8 activations, doublepass/src/checkpoint.rs
+// :21-60 and ramflow/kernels/checkpoint_compress.cu:53-145).  Here a scale
+// belongs to 128 elements of one row, so one loud channel costs its own block
+// its precision and no other, and a row is coded in one read of it:
+//   s = max(absmax / 127, 2^-126),  q = rint(x * (1 / s)),  x^ = q * s
+// in fp32, q in [-127, 127].  The floor of s is the smallest normal number:
+// below it 1 / s would overflow, and a block of zeros needs no case of its
+// own.  A block that holds an infinity or a NaN has a NaN scale and so reads
+// back as NaN throughout: it is not hidden.
+//
+// All kernels are bound by memory.
+#include "row_common.hpp"
+
+namespace nf4s {
+
+constexpr int kCkptThreads = 256;
+
+// The larger of two non-negative values, NaN if either is one: as integers,
+// whose order is that of non-negative floats, with NaNs above infinity.
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
+  return umax(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, true));
+}
+// Largest over the 16 lanes of a row, then of two rows, in every lane of them.
+__device__ __forceinline__ uint32_t row16_umax(uint32_t v) {
+  v = dpp_umax<0x128>(v);
+  v = dpp_umax<0x124>(v);
+  v = dpp_umax<0x122>(v);
+  return dpp_umax<0x121>(v);
+}
+__device__ __forceinline__ uint32_t row32_umax(uint32_t v) {
+  v = row16_umax(v);
+  const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return umax((uint32_t)s[0], (uint32_t)s[1]);
+}
+
+// The largest scale of which 127 are finite: one step below the largest fp32
+// value / 127, which rounds up.
+constexpr float kCkptMaxScale = 0x1.020406p+121f;
+
+// Scale of a block from the bits of its largest magnitude.
+__device__ __forceinline__ float ckpt_scale(uint32_t top) {
+  if (top >= 0x7f800000u) return __builtin_nanf("");
+  return fminf(fmaxf(__builtin_bit_cast(float, top) / 127.0f, 0x1p-126f), kCkptMaxScale);
+}
+
+__device__ __forceinline__ uint32_t ckpt_code4(const floatx4 &v, float inv) {
+  uint32_t q = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // Finite blocks give |r| <= 127; the clamp gives a NaN's conversion a value.
+    const float r = fminf(fmaxf(__builtin_rintf(v[i] * inv), -127.0f), 127.0f);
+    q |= ((uint32_t)(int32_t)r & 0xffu) << (8 * i);
+  }
+  return q;
+}
+
+__device__ __forceinline__ uint32_t top_of(const floatx4 &v) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float f = v[i];  // a bit cast of the element itself reads element 0
+    t = umax(t, __builtin_bit_cast(uint32_t, f) & 0x7fffffffu);
+  }
+  return t;
+}
+
+// One chunk of four elements a lane, 32 lanes a block.  Workgroup b takes
+// chunks [256 (b % segs), ..) of row b / segs; where rows are whole blocks the
+// caller passes the tensor as one long row.
+template <bool kBf16>
+__global__ void __launch_bounds__(kCkptThreads) ckpt_encode_kernel(const void *__restrict__ x,
+                                                                  int64_t chunks, uint32_t segs,
+                                                                  int64_t blocks,
+                                                                  uint32_t *__restrict__ codes,
+                                                                  float *__restrict__ scales) {
+  const int64_t row = blockIdx.x / segs;
+  const int64_t c = (int64_t)(blockIdx.x % segs) * kCkptThreads + threadIdx.x;
+  floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < chunks) {
+    if constexpr (kBf16)
+      v = bf16x4_values(
+          __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(x) + row * chunks + c));
+    else
+      v = __builtin_nontemporal_load(reinterpret_cast<const floatx4 *>(x) + row * chunks + c);
+  }
+  const float s = ckpt_scale(row32_umax(top_of(v)));
+  if (c < chunks) {
+    codes[row * chunks + c] = ckpt_code4(v, 1.0f / s);
+    if ((threadIdx.x & 31) == 0) scales[row * blocks + (c >> kCkptBlockShift)] = s;
+  }
+}
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kCkptThreads) ckpt_decode_kernel(const uint32_t *codes,
+                                                                  const float *scales,
+                                                                  int64_t chunks, uint32_t segs,
+                                                                  int64_t blocks, void *y) {
+  const int64_t row = blockIdx.x / segs;
+  const int64_t c = (int64_t)(blockIdx.x % segs) * kCkptThreads + threadIdx.x;
+  if (c >= chunks) return;
+  const floatx4 v =
+      ckpt_values(codes[row * chunks + c], scales[row * blocks + (c >> kCkptBlockShift)]);
+  if constexpr (kBf16)
+    __builtin_nontemporal_store(bf16x4_pack((floatx4){fp32_rounded(v[0]), fp32_rounded(v[1]),
+                                                      fp32_rounded(v[2]), fp32_rounded(v[3])}),
+                                reinterpret_cast<u32x2 *>(y) + row * chunks + c);
+  else
+    __builtin_nontemporal_store(v, reinterpret_cast<floatx4 *>(y) + row * chunks + c);
+}
+
+// Decode and RMSNorm of a row in one pass: the recompute's first step, whose
+// residual (fp32, if asked for) and GEMM operand (bf16) it writes.  The row
+// stays in registers between the sum of squares and the outputs.
+template <int kMaxThreads, int kChunks>
+__global__ void __launch_bounds__(kMaxThreads) ckpt_norm_kernel(const uint32_t *codes,
+                                                                const float *scales,
+                                                                const float *w, int32_t chunks,
+                                                                int32_t blocks, float eps,
+                                                                float *x, uint16_t *y,
+                                                                float *rms) {
+  __shared__ float part[16];
+  const int64_t row = blockIdx.x;
+  const int threads = (int)blockDim.x;
+  floatx4 v[kChunks];
+  float sum[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = (int)threadIdx.x + i * threads;
+    v[i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < chunks)
+      v[i] = ckpt_values(codes[row * chunks + c], scales[row * blocks + (c >> kCkptBlockShift)]);
+  }
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[0] += v[i][j] * v[i][j];
+  row_block_sum(sum, part);
+  const float r = __builtin_sqrtf(sum[0] / (float)(4 * chunks) + eps);
+  const float inv = 1.0f / r;
+  if (threadIdx.x == 0) rms[row] = r;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = (int)threadIdx.x + i * threads;
+    if (c < chunks) {
+      if (x != nullptr)
+        __builtin_nontemporal_store(v[i], reinterpret_cast<floatx4 *>(x) + row * chunks + c);
+      const floatx4 g = reinterpret_cast<const floatx4 *>(w)[c];
+      floatx4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = fp32_rounded(v[i][j] * inv * g[j]);
+      __builtin_nontemporal_store(bf16x4_pack(o), reinterpret_cast<u32x2 *>(y) + row * chunks + c);
+    }
+  }
+}
+
+// Checks of a checkpoint's sizes; *chunks, *segs and the grid of the encode
+// and decode kernels.
+static int32_t ckpt_plan(int64_t m, int64_t d, int64_t &chunks, uint32_t &segs, int64_t &blocks,
+                         uint32_t &grid) {
+  if (m < 0 || d <= 0)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "bad checkpoint shape m=%lld d=%lld", (long long)m,
+                (long long)d);
+  if (d % 4 != 0)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "checkpoint needs d %% 4 == 0, got %lld",
+                (long long)d);
+  if (d > ((int64_t)1 << 32) || (m > 0 && d > ((int64_t)1 << 39) / m))
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "checkpoint of %lld x %lld elements is too large",
+                (long long)m, (long long)d);
+  chunks = d / 4;
+  blocks = (d + kCkptBlock - 1) / kCkptBlock;
+  int64_t rows = m;
+  if (d % kCkptBlock == 0) {  // no block ends early: one long row
+    chunks *= m;
+    blocks *= m;
+    rows = m > 0 ? 1 : 0;
+  }
+  const int64_t s = (chunks + kCkptThreads - 1) / kCkptThreads;
+  if (rows > 0 && s > kMaxThreadsPerLaunch / kCkptThreads / rows)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "checkpoint of %lld x %lld elements is too large",
+                (long long)m, (long long)d);
+  segs = (uint32_t)s;
+  grid = (uint32_t)(s * rows);
+  return NF4S_OK;
+}
+
+}  // namespace nf4s
+
+using namespace nf4s;
+
+extern "C" {
+
+int32_t nf4s_ckpt8_encode(const void *x, int32_t x_is_bf16, int64_t m, int64_t d, uint8_t *codes,
+                          float *scales, void *stream) {
+  clear_error();
+  int64_t chunks, blocks;
+  uint32_t segs, grid;
+  const int32_t rc = ckpt_plan(m, d, chunks, segs, blocks, grid);
+  if (rc != NF4S_OK || m == 0) return rc;
+  if (x == nullptr || codes == nullptr || scales == nullptr)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "NULL buffer");
+  if (!aligned(x, x_is_bf16 ? 8 : 16) || !aligned(codes, 4) || !aligned(scales, 4))
+    return fail(NF4S_ERR_MISALIGNED,
+                "checkpoint: fp32 x must be 16-byte aligned, bf16 x 8-byte, codes and scales "
+                "4-byte");
+  auto *kernel = x_is_bf16 ? ckpt_encode_kernel<true> : ckpt_encode_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kCkptThreads), 0, as_stream(stream), x, chunks, segs,
+                     blocks, reinterpret_cast<uint32_t *>(codes), scales);
+  return check_launch("ckpt_encode_kernel");
+}
+
+int32_t nf4s_ckpt8_decode(const uint8_t *codes, const float *scales, int64_t m, int64_t d, void *x,
+                          int32_t x_is_bf16, void *stream) {
+  clear_error();
+  int64_t chunks, blocks;
+  uint32_t segs, grid;
+  const int32_t rc = ckpt_plan(m, d, chunks, segs, blocks, grid);
+  if (rc != NF4S_OK || m == 0) return rc;
+  if (x == nullptr || codes == nullptr || scales == nullptr)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "NULL buffer");
+  if (!aligned(x, x_is_bf16 ? 8 : 16) || !aligned(codes, 4) || !aligned(scales, 4))
+    return fail(NF4S_ERR_MISALIGNED,
+                "checkpoint: fp32 x must be 16-byte aligned, bf16 x 8-byte, codes and scales "
+                "4-byte");
+  auto *kernel = x_is_bf16 ? ckpt_decode_kernel<true> : ckpt_decode_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kCkptThreads), 0, as_stream(stream),
+                     reinterpret_cast<const uint32_t *>(codes), scales, chunks, segs, blocks, x);
+  return check_launch("ckpt_decode_kernel");
+}
+
+int32_t nf4s_ckpt8_decode_norm(const uint8_t *codes, const float *scales, const float *w, int64_t m,
+                               int64_t d, float eps, float *x, uint16_t *y, float *rms,
+                               void *stream) {
+  clear_error();
+  int64_t chunks, blocks;
+  uint32_t segs, grid;
+  const int32_t rc = ckpt_plan(m, d, chunks, segs, blocks, grid);
+  if (rc != NF4S_OK) return rc;
+  if (d > kMaxRow)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "norm row of %lld elements is too long",
+                (long long)d);
+  if (m > kMaxThreadsPerLaunch / 1024)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many rows");
+  if (m == 0) return NF4S_OK;
+  if (codes == nullptr || scales == nullptr || w == nullptr || y == nullptr || rms == nullptr)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "NULL buffer");
+  if (!aligned(codes, 4) || !aligned(scales, 4) || !aligned(w, 16) || !aligned(x, 16) ||
+      !aligned(y, 8) || !aligned(rms, 4))
+    return fail(NF4S_ERR_MISALIGNED,
+                "x and w must be 16-byte aligned, y 8-byte, codes, scales and rms 4-byte");
+  const int32_t row_chunks = (int32_t)(d / 4);
+  const int32_t row_blocks = (int32_t)((d + kCkptBlock - 1) / kCkptBlock);
+  // Four chunks a thread up to 1024 threads, then eight.
+  const int per = d <= 16384 ? 4 : 8;
+  const int threads = ((row_chunks + per - 1) / per + 63) / 64 * 64;
+  auto *kernel = per == 8 ? ckpt_norm_kernel<1024, 8>
+                          : (threads <= 512 ? ckpt_norm_kernel<512, 4> : ckpt_norm_kernel<1024, 4>);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)m), dim3(threads), 0, as_stream(stream),
+                     reinterpret_cast<const uint32_t *>(codes), scales, w, row_chunks, row_blocks,
+                     eps, x, y, rms);
+  return check_launch("ckpt_norm_kernel");
+}
+
+}  // extern "C"

@@ -1,0 +1,501 @@
+// linear_ce.hip - cross entropy of a linear head over a large vocabulary, with
+// its gradients, without keeping the logits, for gfx950 (MI355X).
+//
+// x [M, d] and w [V, d] bf16, one target a token (the reference streams the
+// vocabulary in tiles with an online softmax, doublepass/src/loss.rs and
+// doublepass/kernels/fused_ce.cu:71-173):
+//   z = x . w^T,  lse_m = log sum_c exp z_mc,  loss_m = lse_m - z_m,t(m)
+//   G_mc = (exp(z_mc - lse_m) - [c = t(m)]) dloss_m
+//   dx = G . w,   dw = G^T . x
+// An ignored target gives loss 0 and a row of G that is 0; one outside [0, V)
+// that is not the ignored value gives NaN.  Products accumulate in fp32;
+// maxima, sums, lse and loss are fp32.
+//
+// Forward: a tile of logits (tokens x vocabulary) stays in its accumulators; a
+// lane holds one token's columns, so the tile's maximum and sum of exponentials
+// are sums over registers and one exchange.  They leave as 8 bytes per token
+// and 32 kNT columns, and a second kernel joins them: M V / 16 bytes written at
+// 256 x 256 tiles, where the logits would be 2 M V.
+// Backward: the vocabulary in pieces whose G (bf16, the operand of both
+// products: one rounding of each value, as of every dY of the weight gradients)
+// fits kCePieceBytes.  Per piece: logits again, turned into G in the epilogue;
+// dx += G . w in fp32; the piece's rows of dw.  The four products of a training
+// step are matrix-rate bound, the forward of few tokens reads w at memory rate.
+#include "bf16_gemm_core.hpp"
+
+namespace nf4s {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// G of a piece: what the Infinity Cache (256 MB) holds between the kernel that
+// writes it and the two that read it.
+constexpr int64_t kCePieceBytes = (int64_t)256 << 20;
+// Tokens of one forward launch, which bounds its partial sums.
+constexpr int64_t kCeTokens = 16384;
+// A launch counts its threads in 32 bits.
+constexpr int64_t kMaxTiles = 0xffffffffll / kGcThreads;
+
+struct CeLogits {
+  const uint16_t *x, *w;  // w at the piece's first row
+  const int64_t *targets;
+  int64_t M, d;
+  int64_t v0;        // first column of the piece
+  int32_t vn;        // its columns
+  int64_t V, ignore;
+  int32_t tiles_l, tiles_r, strip;
+  // forward
+  float2 *part;      // [2 tiles_r][M]: maximum, sum of exponentials
+  float *zt;         // [M] logit of the target
+  // backward
+  const float *lse, *dloss;
+  uint16_t *g;       // [M, ldg]
+  int64_t ldg;
+};
+
+__device__ __forceinline__ float other_half(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  // s[0]: lanes 0-31's value in both halves, s[1]: lanes 32-63's.
+  return __builtin_bit_cast(float, (uint32_t)((threadIdx.x & 32) ? s[0] : s[1]));
+}
+
+__device__ __forceinline__ float exp_of(float x) {
+  return __builtin_amdgcn_exp2f(x * kLog2e);
+}
+
+// Column of the wave's block (0 .. 32 kNT - 1) of the lane's register v of
+// column tile nt is 32 nt + 8 (v / 4) + 4 (lane / 32) + v % 4.
+template <int kMT, int kNT, bool kGrad>
+__global__ void __launch_bounds__(kGcThreads, kMT == 4 ? 1 : 2) ce_logits_kernel(const CeLogits a) {
+  using Core = GcCore<kMT, kNT, false, false>;
+  __shared__ __attribute__((aligned(16))) char lds[Core::kLdsBytes];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int lane = threadIdx.x & 63;
+  int tl, tr;
+  gc_tile(blockIdx.x, a.tiles_l, a.tiles_r, a.strip, tl, tr);
+  const int64_t l0 = (int64_t)tl * Core::kTileL;
+  const int r0 = tr * Core::kTileR;
+  const int64_t lrows = a.M - l0 < Core::kTileL ? a.M - l0 : Core::kTileL;
+  const int rrows = a.vn - r0 < Core::kTileR ? a.vn - r0 : Core::kTileR;
+  Core core;
+  core.run(gc_along(a.x + l0 * a.d, a.d, lrows, a.d),
+           gc_along(a.w + (int64_t)r0 * a.d, a.d, rrows, a.d), a.d, lds, lane, wave);
+
+  const int64_t row0 = l0 + 32 * kMT * (wave >> 1);  // the wave's first token
+  const int c0 = 32 * kNT * (wave & 1);              // and its first column in the tile
+  const int cols = rrows - c0;                       // its columns that exist (may be <= 0)
+#pragma unroll
+  for (int mt = 0; mt < kMT; ++mt) {
+    // One 32-token block at a time: interleaved, the blocks spill.
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "+v"(lane));
+    floatx16 (&z)[kNT] = core.acc[mt];
+    if (cols < 32 * kNT) {  // columns past the vocabulary
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (32 * nt + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3) >= cols)
+            z[nt][v] = -__builtin_inff();
+    }
+    const int grp = lane >> 5;
+    const int64_t row = row0 + 32 * mt + (lane & 31);
+    const bool here = row < a.M;
+    const int64_t t = here ? a.targets[row] : a.ignore;
+    // The target's register among this lane's, or -1.
+    const int64_t rel = t - (a.v0 + r0 + c0);
+    const bool mine = t != a.ignore && rel >= 0 && rel < 32 * kNT && rel < cols &&
+                      (((int)rel >> 2) & 1) == grp;
+    const int at = mine ? 16 * ((int)rel >> 5) + 4 * (((int)rel >> 3) & 3) + ((int)rel & 3) : -1;
+    if constexpr (!kGrad) {
+      if (__ballot(mine) != 0) {
+        float zt = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) zt = at == 16 * nt + v ? z[nt][v] : zt;
+        if (mine) a.zt[row] = zt;
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) top = fmaxf(top, z[nt][v]);
+      top = fmaxf(top, other_half(top));
+      // Nothing but -inf: any finite reference gives a sum of 0.
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sum += exp_of(z[nt][v] - ref);
+      sum += other_half(sum);
+      if (here && grp == 0)
+        a.part[(int64_t)(2 * tr + (wave & 1)) * a.M + row] = make_float2(top, sum);
+    } else {
+      const float lse = here ? a.lse[row] : 0.0f;
+      const bool skip = t == a.ignore;
+      float dl = here && !skip ? a.dloss[row] : 0.0f;
+      if (!skip && (t < 0 || t >= a.V)) dl = __builtin_nanf("");
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) z[nt][v] = exp_of(z[nt][v] - lse);
+      if (__ballot(mine) != 0) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) z[nt][v] -= at == 16 * nt + v ? 1.0f : 0.0f;
+      }
+      // Columns of the piece's last, partial 64 hold zeros: G is read in steps of 64.
+      gc_store_bf16<kNT>(
+          [&](int nt, int v) { return skip ? 0.0f : fp32_rounded(z[nt][v] * dl); },
+          lds + 32 * 64 * kNT * wave, a.g + (row0 + 32 * mt) * a.ldg + r0 + c0, a.ldg,
+          a.M - (row0 + 32 * mt), a.ldg - (r0 + c0), lane);
+    }
+  }
+}
+
+// Joins a token's partial sums: 32 threads a token take every 32nd slice, then
+// meet in a fixed order.
+__global__ void __launch_bounds__(256) ce_join_kernel(const float2 *part, const float *zt,
+                                                      const int64_t *targets, int64_t M,
+                                                      int32_t slices, int64_t V, int64_t ignore,
+                                                      float *loss, float *lse) {
+  __shared__ float2 lds[32][8];
+  const int tok = threadIdx.x & 7, grp = threadIdx.x >> 3;
+  const int64_t row = (int64_t)blockIdx.x * 8 + tok;
+  auto join = [](float2 a, float2 b) {
+    const float top = fmaxf(a.x, b.x);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    return make_float2(top, a.y * exp_of(a.x - ref) + b.y * exp_of(b.x - ref));
+  };
+  float2 s = make_float2(-__builtin_inff(), 0.0f);
+  if (row < M)
+    for (int i = grp; i < slices; i += 32) s = join(s, part[(int64_t)i * M + row]);
+  lds[grp][tok] = s;
+  __syncthreads();
+  if (grp != 0 || row >= M) return;
+  for (int i = 1; i < 32; ++i) s = join(s, lds[i][tok]);
+  const float l = s.x + __builtin_amdgcn_logf(s.y) * kLn2;
+  lse[row] = l;
+  const int64_t t = targets[row];
+  float v = 0.0f;
+  if (t != ignore)
+    v = t < 0 || t >= V ? __builtin_nanf("")
+                        : (s.x - zt[row]) + __builtin_amdgcn_logf(s.y) * kLn2;
+  loss[row] = v;
+}
+
+struct CeProduct {
+  const uint16_t *l, *r;
+  int64_t ldl, ldr;
+  int64_t rows, cols;   // of the output
+  int64_t k;            // reduction
+  int64_t slice;        // reduction of one slice (a multiple of kGcStep)
+  int32_t tiles_l, tiles_r, strip;
+  void *out;            // leading dimension ld
+  int64_t ld, slice_stride;
+};
+
+// Output of a product: dx partials (fp32, stored or added) along the vocabulary,
+// dw (fp32 or bf16) along the tokens.
+enum { kOutF32, kOutF32Add, kOutBf16 };
+
+template <int kMT, bool kLAcross, int kOut>
+__global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_product_kernel(
+    const CeProduct a) {
+  using Core = GcCore<kMT, 4, kLAcross, true>;
+  __shared__ __attribute__((aligned(16))) char lds[Core::kLdsBytes];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int T = a.tiles_l * a.tiles_r;
+  const int slice = (int)blockIdx.x / T;
+  int tl, tr;
+  gc_tile((int)blockIdx.x - slice * T, a.tiles_l, a.tiles_r, a.strip, tl, tr);
+  const int64_t l0 = (int64_t)tl * Core::kTileL, r0 = (int64_t)tr * Core::kTileR;
+  const int64_t k0 = slice * a.slice;
+  const int64_t k = a.k - k0 < a.slice ? a.k - k0 : a.slice;
+  const GcOperand r = gc_across(a.r + k0 * a.ldr + r0, a.ldr, a.cols - r0, k);
+  Core core;
+  if constexpr (kLAcross) {
+    // G's rows are ldl long: the zeros past the piece's columns are there too.
+    core.run(gc_across(a.l + k0 * a.ldl + l0, a.ldl, a.ldl - l0, k), r, k, lds, lane, wave);
+  } else {
+    const int64_t rows = a.rows - l0 < Core::kTileL ? a.rows - l0 : Core::kTileL;
+    core.run(gc_along(a.l + l0 * a.ldl + k0, a.ldl, rows, (k + 7) & ~(int64_t)7), r, k, lds, lane,
+             wave);
+  }
+  const int64_t row0 = 32 * kMT * (wave >> 1), c0 = r0 + 128 * (wave & 1);
+#pragma unroll
+  for (int mt = 0; mt < kMT; ++mt) {
+    auto value = [&](int nt, int v) { return core.acc[mt][nt][v]; };
+    const int64_t row = l0 + row0 + 32 * mt;
+    const int64_t at = slice * a.slice_stride + row * a.ld + c0;
+    if constexpr (kOut == kOutBf16)
+      gc_store_bf16<4>(value, lds + 8192 * wave, static_cast<uint16_t *>(a.out) + at, a.ld,
+                       a.rows - row, a.cols - c0, lane);
+    else
+      gc_store_f32<4, kOut == kOutF32Add>(value, lds + 16384 * wave,
+                                          static_cast<float *>(a.out) + at, a.ld, a.rows - row,
+                                          a.cols - c0, lane);
+  }
+}
+
+// dx = the sum of its slices' fp32 sums, rounded once.
+__global__ void __launch_bounds__(256) ce_dx_kernel(const floatx4 *part, int32_t slices,
+                                                    int64_t chunks, u32x2 *dx) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks;
+       i += (int64_t)gridDim.x * 256) {
+    floatx4 s = part[i];
+    for (int p = 1; p < slices; ++p) s += part[p * chunks + i];
+    dx[i] = (u32x2){pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
+  }
+}
+
+template <typename T>
+__global__ void ce_zero_kernel(T *p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * blockDim.x)
+    p[i] = T(0);
+}
+
+static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// Tile heights (64 kMT tokens) of the logits and of dx.
+static int ce_mt(int64_t m) { return m <= 64 ? 1 : (m <= 128 ? 2 : 4); }
+
+struct CePlan {
+  int mt, nt;            // logits tile
+  int64_t tokens;        // forward: tokens of one launch
+  int64_t piece, ldg;    // backward: columns of a piece, row length of G
+  int64_t slices, slice; // of dx's reduction over a piece
+  int64_t fwd_bytes, g_bytes, bwd_bytes;
+};
+
+static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
+  if (m < 0 || v <= 0 || d <= 0)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "bad cross-entropy shape m=%lld v=%lld d=%lld",
+                (long long)m, (long long)v, (long long)d);
+  if (d % 8 != 0)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "cross entropy needs d %% 8 == 0, got %lld",
+                (long long)d);
+  // Offsets within a tile's step and tile counts are 32-bit.
+  if (d > ((int64_t)1 << 20) || v > ((int64_t)1 << 28) || m > ((int64_t)1 << 24))
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE,
+                "cross entropy of m=%lld v=%lld d=%lld beyond m 2^24, v 2^28, d 2^20",
+                (long long)m, (long long)v, (long long)d);
+  p.mt = ce_mt(m);
+  p.nt = p.mt == 4 ? 4 : 2;
+  p.tokens = m < kCeTokens ? m : kCeTokens;
+  const int64_t slices = 2 * ((v + 64 * p.nt - 1) / (64 * p.nt));
+  p.fwd_bytes = up(slices * p.tokens * 8, 256) + p.tokens * 4;
+  int64_t most = m > 0 ? kCePieceBytes / (2 * m) / 256 * 256 : v;
+  most = most < 256 ? 256 : (most > (1 << 20) ? (1 << 20) : most);
+  const int64_t pieces = (v + most - 1) / most;
+  p.piece = up((v + pieces - 1) / pieces, 256);
+  if (p.piece > v) p.piece = v;
+  p.ldg = up(p.piece, 64);
+  // Slices of dx's reduction: as many as fill the chip, of at least 8 steps.
+  const int64_t tiles = ((m + 64 * p.mt - 1) / (64 * p.mt)) * ((d + 255) / 256);
+  const int64_t slots = (int64_t)cu_slots() * (p.mt == 1 ? 2 : 1);
+  int64_t s = tiles > 0 ? slots / tiles : 1;
+  const int64_t least = (p.ldg + 8 * kGcStep - 1) / (8 * kGcStep);
+  s = s < 1 ? 1 : (s > least ? least : s);
+  p.slice = up((p.ldg + s - 1) / s, kGcStep);
+  p.slices = (p.ldg + p.slice - 1) / p.slice;
+  p.g_bytes = up(m * p.ldg * 2, 256);
+  p.bwd_bytes = p.g_bytes + p.slices * m * d * 4;
+  const int64_t tokens64 = (m + 63) / 64;
+  if (tokens64 * ((v + 127) / 128) > kMaxTiles || ((v + 127) / 128) * ((d + 255) / 256) > kMaxTiles)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many tiles");
+  return NF4S_OK;
+}
+
+template <bool kGrad>
+static int32_t ce_logits(const CePlan &p, CeLogits a, hipStream_t s) {
+  a.tiles_l = (int32_t)((a.M + 64 * p.mt - 1) / (64 * p.mt));
+  a.tiles_r = (int32_t)((a.vn + 64 * p.nt - 1) / (64 * p.nt));
+  a.strip = 8;
+  auto *kernel = p.mt == 4   ? ce_logits_kernel<4, 4, kGrad>
+                 : p.mt == 2 ? ce_logits_kernel<2, 2, kGrad>
+                             : ce_logits_kernel<1, 2, kGrad>;
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)a.tiles_l * (uint32_t)a.tiles_r), dim3(kGcThreads), 0,
+                     s, a);
+  return check_launch("ce_logits_kernel");
+}
+
+template <int kMT, bool kLAcross, int kOut>
+static int32_t ce_product(CeProduct a, hipStream_t s) {
+  a.tiles_l = (int32_t)((a.rows + 64 * kMT - 1) / (64 * kMT));
+  a.tiles_r = (int32_t)((a.cols + 255) / 256);
+  a.strip = 8;
+  const int64_t slices = (a.k + a.slice - 1) / a.slice;
+  auto *kernel = ce_product_kernel<kMT, kLAcross, kOut>;
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)(slices * a.tiles_l * a.tiles_r)), dim3(kGcThreads), 0,
+                     s, a);
+  return check_launch("ce_product_kernel");
+}
+
+template <int kOut>
+static int32_t ce_dx_piece(const CePlan &p, const CeProduct &a, hipStream_t s) {
+  return p.mt == 4   ? ce_product<4, false, kOut>(a, s)
+         : p.mt == 2 ? ce_product<2, false, kOut>(a, s)
+                     : ce_product<1, false, kOut>(a, s);
+}
+
+static int32_t ce_operands(const uint16_t *x, const uint16_t *w, const int64_t *targets, int64_t m,
+                           void *workspace, int64_t workspace_bytes, int64_t need) {
+  if (w == nullptr || (m > 0 && (x == nullptr || targets == nullptr)))
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "NULL buffer");
+  if (!aligned(w, 16) || (m > 0 && (!aligned(x, 16) || !aligned(targets, 8))))
+    return fail(NF4S_ERR_MISALIGNED, "x and w must be 16-byte aligned, targets 8-byte");
+  if (m > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "cross entropy needs %lld workspace bytes",
+                (long long)need);
+  if (m > 0 && !aligned(workspace, 16))
+    return fail(NF4S_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+  return NF4S_OK;
+}
+
+}  // namespace nf4s
+
+using namespace nf4s;
+
+extern "C" {
+
+int32_t nf4s_linear_ce_workspace_size(int64_t m, int64_t v, int64_t d, int32_t backward,
+                                      int64_t *bytes) {
+  clear_error();
+  if (bytes == nullptr) return fail(NF4S_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  *bytes = 0;
+  CePlan p;
+  const int32_t rc = ce_plan(m, v, d, p);
+  if (rc == NF4S_OK && m > 0) *bytes = backward ? p.bwd_bytes : p.fwd_bytes;
+  return rc;
+}
+
+int32_t nf4s_linear_ce_fwd(const uint16_t *x, const uint16_t *w, const int64_t *targets, int64_t m,
+                           int64_t v, int64_t d, int64_t ignore_index, float *loss, float *lse,
+                           void *workspace, int64_t workspace_bytes, void *stream) {
+  clear_error();
+  CePlan p;
+  int32_t rc = ce_plan(m, v, d, p);
+  if (rc != NF4S_OK || m == 0) return rc;
+  rc = ce_operands(x, w, targets, m, workspace, workspace_bytes, p.fwd_bytes);
+  if (rc != NF4S_OK) return rc;
+  if (loss == nullptr || lse == nullptr)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "loss or lse is NULL");
+  if (!aligned(loss, 4) || !aligned(lse, 4))
+    return fail(NF4S_ERR_MISALIGNED, "loss and lse must be 4-byte aligned");
+  const hipStream_t s = as_stream(stream);
+  const int32_t slices = (int32_t)(2 * ((v + 64 * p.nt - 1) / (64 * p.nt)));
+  CeLogits a{};
+  a.w = w;
+  a.d = d;
+  a.vn = (int32_t)v;
+  a.V = v;
+  a.ignore = ignore_index;
+  a.part = static_cast<float2 *>(workspace);
+  a.zt = reinterpret_cast<float *>(static_cast<char *>(workspace) +
+                                   up((int64_t)slices * p.tokens * 8, 256));
+  for (int64_t m0 = 0; m0 < m; m0 += p.tokens) {
+    a.M = m - m0 < p.tokens ? m - m0 : p.tokens;
+    a.x = x + m0 * d;
+    a.targets = targets + m0;
+    rc = ce_logits<false>(p, a, s);
+    if (rc != NF4S_OK) return rc;
+    hipLaunchKernelGGL(ce_join_kernel, dim3((uint32_t)((a.M + 7) / 8)), dim3(256), 0, s, a.part,
+                       a.zt, a.targets, a.M, slices, v, ignore_index, loss + m0, lse + m0);
+    rc = check_launch("ce_join_kernel");
+    if (rc != NF4S_OK) return rc;
+  }
+  return NF4S_OK;
+}
+
+int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
+                           const float *lse, const float *dloss, int64_t m, int64_t v, int64_t d,
+                           int64_t ignore_index, uint16_t *dx, void *dw, int32_t dw_is_f32,
+                           int32_t accumulate, void *workspace, int64_t workspace_bytes,
+                           void *stream) {
+  clear_error();
+  CePlan p;
+  int32_t rc = ce_plan(m, v, d, p);
+  if (rc != NF4S_OK) return rc;
+  rc = ce_operands(x, w, targets, m, workspace, workspace_bytes, p.bwd_bytes);
+  if (rc != NF4S_OK) return rc;
+  if (accumulate && !dw_is_f32)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "dw accumulates in fp32 only");
+  if (dw == nullptr || (m > 0 && (lse == nullptr || dloss == nullptr || dx == nullptr)))
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "lse, dloss, dx or dw is NULL");
+  if (!aligned(dw, 16) || (m > 0 && (!aligned(dx, 16) || !aligned(lse, 4) || !aligned(dloss, 4))))
+    return fail(NF4S_ERR_MISALIGNED, "dx and dw must be 16-byte aligned, lse and dloss 4-byte");
+  const hipStream_t s = as_stream(stream);
+  if (m == 0) {
+    if (accumulate) return NF4S_OK;
+    const int64_t n = dw_is_f32 ? v * d : v * d / 2;  // 32-bit words
+    hipLaunchKernelGGL(ce_zero_kernel<uint32_t>, dim3(4096), dim3(256), 0, s,
+                       static_cast<uint32_t *>(dw), n);
+    return check_launch("ce_zero_kernel");
+  }
+  uint16_t *g = static_cast<uint16_t *>(workspace);
+  float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.g_bytes);
+  for (int64_t v0 = 0; v0 < v; v0 += p.piece) {
+    const int64_t vn = v - v0 < p.piece ? v - v0 : p.piece;
+    CeLogits a{};
+    a.x = x;
+    a.w = w + v0 * d;
+    a.targets = targets;
+    a.M = m;
+    a.d = d;
+    a.v0 = v0;
+    a.vn = (int32_t)vn;
+    a.V = v;
+    a.ignore = ignore_index;
+    a.lse = lse;
+    a.dloss = dloss;
+    a.g = g;
+    a.ldg = p.ldg;
+    rc = ce_logits<true>(p, a, s);
+    if (rc != NF4S_OK) return rc;
+    CeProduct b{};  // dx += G . w
+    b.l = g;
+    b.ldl = p.ldg;
+    b.r = w + v0 * d;
+    b.ldr = d;
+    b.rows = m;
+    b.cols = d;
+    b.k = vn;
+    b.slice = p.slice;
+    b.out = part;
+    b.ld = d;
+    b.slice_stride = m * d;
+    rc = v0 == 0 ? ce_dx_piece<kOutF32>(p, b, s) : ce_dx_piece<kOutF32Add>(p, b, s);
+    if (rc != NF4S_OK) return rc;
+    CeProduct c{};  // the piece's rows of dw = G^T . x
+    c.l = g;
+    c.ldl = p.ldg;
+    c.r = x;
+    c.ldr = d;
+    c.rows = vn;
+    c.cols = d;
+    c.k = m;
+    c.slice = up(m, kGcStep);
+    c.out = dw_is_f32 ? static_cast<void *>(static_cast<float *>(dw) + v0 * d)
+                      : static_cast<void *>(static_cast<uint16_t *>(dw) + v0 * d);
+    c.ld = d;
+    rc = accumulate  ? ce_product<4, true, kOutF32Add>(c, s)
+         : dw_is_f32 ? ce_product<4, true, kOutF32>(c, s)
+                     : ce_product<4, true, kOutBf16>(c, s);
+    if (rc != NF4S_OK) return rc;
+  }
+  const int64_t chunks = m * d / 4;
+  const int64_t blocks = (chunks + 255) / 256;
+  hipLaunchKernelGGL(ce_dx_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0,
+                     s, reinterpret_cast<const floatx4 *>(part), (int32_t)p.slices, chunks,
+                     reinterpret_cast<u32x2 *>(dx));
+  return check_launch("ce_dx_kernel");
+}
+
+}  // extern "C"

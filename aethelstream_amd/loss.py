@@ -1,0 +1,98 @@
+"""Cross entropy of a linear head without keeping the logits, and its gradients.
+
+``linear_cross_entropy``      loss and log-sum-exp of each token of x . W^T
+``linear_cross_entropy_bwd``  dX and dW for given gradients of the losses
+
+They take the place of the reference's two passes over vocabulary tiles
+(doublepass/src/loss.rs, doublepass/kernels/fused_ce.cu:71-207): the logits live
+in the accumulators of a tile, the gradients are computed in pieces of the
+vocabulary.  x is bf16 [M, d] (the final norm's output), W the bf16 head [V, d],
+targets int64 [M]; losses and log-sum-exp are fp32.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .gemm import _workspace_for
+from .nf4 import _require_cuda, _stream_ptr
+
+IGNORE_INDEX = -100
+
+
+def workspace_bytes(m: int, v: int, d: int, backward: bool) -> int:
+    """Workspace of the forward, or of the gradients, for M tokens and a [V, d] head."""
+    out = ctypes.c_int64(0)
+    _lib.check(_lib.load().nf4s_linear_ce_workspace_size(m, v, d, int(backward),
+                                                         ctypes.byref(out)))
+    return int(out.value)
+
+
+def _check_head(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor) -> None:
+    _require_cuda(x, w, targets)
+    if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+        raise ValueError("x and w must be bfloat16")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x [M, d] and w [V, d] must share d, got {list(x.shape)} and "
+                         f"{list(w.shape)}")
+    if targets.dtype != torch.int64 or list(targets.shape) != [x.shape[0]]:
+        raise ValueError(f"targets must be int64 [{x.shape[0]}]")
+    if w.device != x.device or targets.device != x.device:
+        raise ValueError("x, w and targets must be on one device")
+
+
+def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
+                         ignore_index: int = IGNORE_INDEX,
+                         workspace: Optional[torch.Tensor] = None
+                         ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(loss [M], lse [M]) in fp32.  A target equal to ``ignore_index`` has loss
+    0; any other outside [0, V) has loss NaN (it is only seen on the device).
+    ``workspace``: a buffer to use instead of one from torch's caching allocator,
+    if it holds :func:`workspace_bytes`."""
+    _check_head(x, w, targets)
+    m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
+    loss = torch.empty(m, dtype=torch.float32, device=x.device)
+    lse = torch.empty(m, dtype=torch.float32, device=x.device)
+    workspace = _workspace_for(workspace_bytes(m, v, d, False), workspace, x)
+    _lib.check(_lib.load().nf4s_linear_ce_fwd(
+        x.data_ptr(), w.data_ptr(), targets.data_ptr(), m, v, d, ignore_index, loss.data_ptr(),
+        lse.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        _stream_ptr(x)))
+    return loss, lse
+
+
+def linear_cross_entropy_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
+                             lse: torch.Tensor, dloss: torch.Tensor,
+                             ignore_index: int = IGNORE_INDEX, dw: Optional[torch.Tensor] = None,
+                             accumulate: bool = False,
+                             workspace: Optional[torch.Tensor] = None
+                             ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dx bf16 [M, d], dw [V, d]) for the gradient ``dloss`` fp32 [M] of each
+    token's loss.  dw is bf16 unless a float32 ``dw`` is given, which the
+    micro-batches of a step may ``accumulate`` into."""
+    _check_head(x, w, targets)
+    _require_cuda(lse, dloss, dw)
+    m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
+    for t, name in ((lse, "lse"), (dloss, "dloss")):
+        if t.dtype != torch.float32 or list(t.shape) != [m] or t.device != x.device:
+            raise ValueError(f"{name} must be float32 [{m}] on x's device")
+    if dw is None:
+        if accumulate:
+            raise ValueError("accumulate needs an existing float32 dw")
+        dw = torch.empty(v, d, dtype=torch.bfloat16, device=x.device)
+    if dw.dtype not in (torch.bfloat16, torch.float32) or list(dw.shape) != [v, d] \
+            or dw.device != x.device:
+        raise ValueError(f"dw must be bfloat16 or float32 [{v}, {d}] on x's device")
+    if accumulate and dw.dtype != torch.float32:
+        raise ValueError("accumulate needs a float32 dw")
+    dx = torch.empty(m, d, dtype=torch.bfloat16, device=x.device)
+    workspace = _workspace_for(workspace_bytes(m, v, d, True), workspace, x)
+    _lib.check(_lib.load().nf4s_linear_ce_bwd(
+        x.data_ptr(), w.data_ptr(), targets.data_ptr(), lse.data_ptr(), dloss.data_ptr(), m, v, d,
+        ignore_index, dx.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32),
+        int(accumulate), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        _stream_ptr(x)))
+    return dx, dw

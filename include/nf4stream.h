@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define NF4S_ABI_VERSION 3
+#define NF4S_ABI_VERSION 4
 
 enum nf4s_status {
     NF4S_OK = 0,
@@ -341,6 +341,102 @@ int32_t nf4s_gemm_wgrad_grouped(const void *const *dys, const int64_t *ns,
  */
 int32_t nf4s_rmsnorm_fwd(const float *x, const float *w, int64_t m, int64_t d, float eps,
                          uint16_t *y, float *rms, void *stream);
+
+/*
+ * The norms around a block with its gate and residual scale, forward, for rows
+ * of d elements:
+ *   u = w_post * h / rms_post   (u = h when w_post is NULL)
+ *   res_out = res + alpha * gate * u   (gate NULL: 1)
+ *   y = bf16(w_pre * res_out / rms_pre),  rms = sqrt(mean of squares + eps)
+ * h and y are bf16 [m, d], res and res_out fp32 [m, d], the weights and the
+ * gate fp32 [d], rms_pre and rms_post (set iff w_post is) fp32 [m].  res_out may
+ * be res.  Replaces the residual add and the next rms_norm_fwd of
+ * single_layer_forward (doublepass/src/forward.rs:246-249).
+ * Requires d % 4 == 0, d <= 32768, fp32 buffers of rows and weights 16-byte
+ * aligned, bf16 ones 8-byte.
+ */
+int32_t nf4s_block_norm_fwd(const uint16_t *h, const float *res, const float *w_pre,
+                            const float *w_post, const float *gate, float alpha, int64_t m,
+                            int64_t d, float eps, float *res_out, uint16_t *y, float *rms_pre,
+                            float *rms_post, void *stream);
+
+/*
+ * Its backward.  dy (bf16) is the gradient of y, dres (fp32, NULL: zero) the one
+ * that reaches res_out by the residual path.  res_out comes as fp32 (res) or as
+ * its 8-bit checkpoint (res_codes, res_scales: nf4s_ckpt8_encode), exactly one
+ * of them.  Writes dres_out = the gradient of res (fp32, may be dres), dh (bf16,
+ * set iff h is), and the column sums dw_pre, dw_post (set iff w_post is) and
+ * dgate (set iff gate is), all fp32 [d], zero when m = 0.  h = NULL is the plain
+ * RMSNorm backward (rms_norm_bwd, doublepass/src/math.rs:61-88), without w_post
+ * and gate.  The workspace holds the column sums of the launch's workgroups,
+ * which a second kernel adds in order: results do not depend on timing.
+ */
+int32_t nf4s_block_norm_bwd(const uint16_t *dy, const float *dres, const float *res,
+                            const uint8_t *res_codes, const float *res_scales,
+                            const float *rms_pre, const float *w_pre, const uint16_t *h,
+                            const float *rms_post, const float *w_post, const float *gate,
+                            float alpha, int64_t m, int64_t d, float *dres_out, uint16_t *dh,
+                            float *dw_pre, float *dw_post, float *dgate, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+/* Workspace bytes nf4s_block_norm_bwd needs.  Allocates nothing. */
+int32_t nf4s_block_norm_bwd_workspace_size(int64_t m, int64_t d, int64_t *bytes);
+
+/* ---------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits: [m, d] signed codes (two's complement) and
+ * fp32 scales [m, ceil(d / 128)], one for 128 elements along a row (the row's
+ * last block may be shorter).  Takes the place of the reference's per-channel
+ * int8 checkpoints (doublepass/src/checkpoint.rs:21-60,
+ * ramflow/kernels/checkpoint_compress.cu:53-145).
+ *   scale = max(absmax / 127, 2^-126), code = rint(x * (1 / scale))
+ * in fp32; a value reads back as code * scale.  A block with an infinity or a
+ * NaN has a NaN scale.  d % 4 == 0; fp32 activations 16-byte aligned, bf16 ones
+ * 8-byte, codes and scales 4-byte.
+ * ------------------------------------------------------------------------- */
+int32_t nf4s_ckpt8_encode(const void *x, int32_t x_is_bf16, int64_t m, int64_t d,
+                          uint8_t *codes, float *scales, void *stream);
+int32_t nf4s_ckpt8_decode(const uint8_t *codes, const float *scales, int64_t m, int64_t d,
+                          void *x, int32_t x_is_bf16, void *stream);
+/*
+ * The recompute's first step in one pass: x = the decoded checkpoint (fp32, NULL:
+ * not written), rms = sqrt(mean x^2 + eps) and y = bf16(w * x / rms) per row.
+ * d <= 32768.
+ */
+int32_t nf4s_ckpt8_decode_norm(const uint8_t *codes, const float *scales, const float *w,
+                               int64_t m, int64_t d, float eps, float *x, uint16_t *y,
+                               float *rms, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Cross entropy of a linear head, without keeping the logits z = x . w^T:
+ *   lse[i] = log sum_c exp z[i, c],  loss[i] = lse[i] - z[i, targets[i]]
+ * x [m, d] and w [v, d] bf16 row-major, targets int64 [m], loss and lse fp32
+ * [m].  A target equal to ignore_index gives loss 0 and no gradient, any other
+ * outside [0, v) gives NaN.  Takes the place of the reference's two passes over
+ * vocabulary tiles (doublepass/src/loss.rs,
+ * doublepass/kernels/fused_ce.cu:71-207).
+ * Requires d % 8 == 0, m <= 2^24, v <= 2^28, d <= 2^20; x, w, dx, dw and the
+ * workspace 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+int32_t nf4s_linear_ce_fwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
+                           int64_t m, int64_t v, int64_t d, int64_t ignore_index, float *loss,
+                           float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+/*
+ * Gradients for given dloss (fp32 [m], the gradient of each token's loss) and
+ * the forward's lse:
+ *   G[i, c] = (exp(z[i, c] - lse[i]) - [c = targets[i]]) * dloss[i]
+ *   dx = G . w (bf16 [m, d]),  dw = G^T . x (bf16 [v, d], or fp32 with
+ *   dw_is_f32; accumulate, fp32 only, adds to dw)
+ * G is computed in pieces of the vocabulary and rounded to bf16 as an operand
+ * of both products, which accumulate in fp32.
+ */
+int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
+                           const float *lse, const float *dloss, int64_t m, int64_t v, int64_t d,
+                           int64_t ignore_index, uint16_t *dx, void *dw, int32_t dw_is_f32,
+                           int32_t accumulate, void *workspace, int64_t workspace_bytes,
+                           void *stream);
+/* Workspace bytes the forward (backward = 0) or the gradients need.  Calls that
+ * share a workspace must not overlap. */
+int32_t nf4s_linear_ce_workspace_size(int64_t m, int64_t v, int64_t d, int32_t backward,
+                                      int64_t *bytes);
 
 /* ---------------------------------------------------------------------------
  * Streamed layer stack (one GPU).  Layers wait in pinned host memory and are

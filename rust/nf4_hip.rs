@@ -14,7 +14,7 @@
 
 use std::os::raw::{c_char, c_void};
 
-pub const NF4S_ABI_VERSION: i32 = 3;
+pub const NF4S_ABI_VERSION: i32 = 4;
 
 pub const NF4S_OK: i32 = 0;
 pub const NF4S_ERR_INVALID_ARGUMENT: i32 = 1;
@@ -176,6 +176,37 @@ extern "C" {
                                    k: i64, accumulate: i32, stream: *mut c_void) -> i32;
     pub fn nf4s_rmsnorm_fwd(x: *const f32, w: *const f32, m: i64, d: i64, eps: f32, y: *mut u16,
                             rms: *mut f32, stream: *mut c_void) -> i32;
+
+    pub fn nf4s_block_norm_fwd(h: *const u16, res: *const f32, w_pre: *const f32,
+                               w_post: *const f32, gate: *const f32, alpha: f32, m: i64, d: i64,
+                               eps: f32, res_out: *mut f32, y: *mut u16, rms_pre: *mut f32,
+                               rms_post: *mut f32, stream: *mut c_void) -> i32;
+    pub fn nf4s_block_norm_bwd(dy: *const u16, dres: *const f32, res: *const f32,
+                               res_codes: *const u8, res_scales: *const f32, rms_pre: *const f32,
+                               w_pre: *const f32, h: *const u16, rms_post: *const f32,
+                               w_post: *const f32, gate: *const f32, alpha: f32, m: i64, d: i64,
+                               dres_out: *mut f32, dh: *mut u16, dw_pre: *mut f32,
+                               dw_post: *mut f32, dgate: *mut f32, workspace: *mut c_void,
+                               workspace_bytes: i64, stream: *mut c_void) -> i32;
+    pub fn nf4s_block_norm_bwd_workspace_size(m: i64, d: i64, bytes: *mut i64) -> i32;
+    pub fn nf4s_ckpt8_encode(x: *const c_void, x_is_bf16: i32, m: i64, d: i64, codes: *mut u8,
+                             scales: *mut f32, stream: *mut c_void) -> i32;
+    pub fn nf4s_ckpt8_decode(codes: *const u8, scales: *const f32, m: i64, d: i64, x: *mut c_void,
+                             x_is_bf16: i32, stream: *mut c_void) -> i32;
+    pub fn nf4s_ckpt8_decode_norm(codes: *const u8, scales: *const f32, w: *const f32, m: i64,
+                                  d: i64, eps: f32, x: *mut f32, y: *mut u16, rms: *mut f32,
+                                  stream: *mut c_void) -> i32;
+    pub fn nf4s_linear_ce_fwd(x: *const u16, w: *const u16, targets: *const i64, m: i64, v: i64,
+                              d: i64, ignore_index: i64, loss: *mut f32, lse: *mut f32,
+                              workspace: *mut c_void, workspace_bytes: i64,
+                              stream: *mut c_void) -> i32;
+    pub fn nf4s_linear_ce_bwd(x: *const u16, w: *const u16, targets: *const i64, lse: *const f32,
+                              dloss: *const f32, m: i64, v: i64, d: i64, ignore_index: i64,
+                              dx: *mut u16, dw: *mut c_void, dw_is_f32: i32, accumulate: i32,
+                              workspace: *mut c_void, workspace_bytes: i64,
+                              stream: *mut c_void) -> i32;
+    pub fn nf4s_linear_ce_workspace_size(m: i64, v: i64, d: i64, backward: i32,
+                                         bytes: *mut i64) -> i32;
 
     pub fn nf4s_host_alloc(bytes: i64, out: *mut *mut c_void) -> i32;
     pub fn nf4s_host_free(p: *mut c_void) -> i32;
