@@ -5,7 +5,7 @@
 // :21-60 and ramflow/kernels/checkpoint_compress.cu:53-145).  Here a scale
 // belongs to 128 elements of one row, so one loud channel costs its own block
 // its precision and no other, and a row is coded in one read of it:
-//   s = max(absmax / 127, 2^-126),  q = rint(x * (1 / s)),  x^ = q * s
+//   s = max(absmax * (1 / 127), 2^-126),  q = rint(x * (1 / s)),  x^ = q * s
 // in fp32, q in [-127, 127].  The floor of s is the smallest normal number:
 // below it 1 / s would overflow, and a block of zeros needs no case of its
 // own.  A block that holds an infinity or a NaN has a NaN scale and so reads
@@ -42,11 +42,12 @@ __device__ __forceinline__ uint32_t row32_umax(uint32_t v) {
 // The largest scale of which 127 are finite: one step below the largest fp32
 // value / 127, which rounds up.
 constexpr float kCkptMaxScale = 0x1.020406p+121f;
+constexpr float kOver127 = 1.0f / 127.0f;
 
 // Scale of a block from the bits of its largest magnitude.
 __device__ __forceinline__ float ckpt_scale(uint32_t top) {
   if (top >= 0x7f800000u) return __builtin_nanf("");
-  return fminf(fmaxf(__builtin_bit_cast(float, top) / 127.0f, 0x1p-126f), kCkptMaxScale);
+  return fminf(fmaxf(__builtin_bit_cast(float, top) * kOver127, 0x1p-126f), kCkptMaxScale);
 }
 
 __device__ __forceinline__ uint32_t ckpt_code4(const floatx4 &v, float inv) {

@@ -5,8 +5,8 @@
 // vocabulary in tiles with an online softmax, doublepass/src/loss.rs and
 // doublepass/kernels/fused_ce.cu:71-173):
 //   z = x . w^T,  lse_m = log sum_c exp z_mc,  loss_m = lse_m - z_m,t(m)
-//   G_mc = (exp(z_mc - lse_m) - [c = t(m)]) dloss_m
-//   dx = G . w,   dw = G^T . x
+//   G_mc = (exp(z_mc - lse_m) - [c = t(m)]) dloss_m / c
+//   dx = c G . w,   dw = c G^T . x,   c = max |dloss|
 // An ignored target gives loss 0 and a row of G that is 0; one outside [0, V)
 // that is not the ignored value gives NaN.  Products accumulate in fp32;
 // maxima, sums, lse and loss are fp32.
@@ -18,7 +18,10 @@
 // 256 x 256 tiles, where the logits would be 2 M V.
 // Backward: the vocabulary in pieces whose G (bf16, the operand of both
 // products: one rounding of each value, as of every dY of the weight gradients)
-// fits kCePieceBytes.  Per piece: logits again, turned into G in the epilogue;
+// fits kCePieceBytes.  The common factor c stays out of G: the tokens of a mean
+// all have dloss = c, whose rounding error would be that of every target's
+// entry (up to 2^-8 at once); divided by c those entries are close to -1.  Per
+// piece: logits again, turned into G in the epilogue;
 // dx += G . w in fp32; the piece's rows of dw.  The four products of a training
 // step are matrix-rate bound, the forward of few tokens reads w at memory rate.
 #include "bf16_gemm_core.hpp"
@@ -49,6 +52,7 @@ struct CeLogits {
   float *zt;         // [M] logit of the target
   // backward
   const float *lse, *dloss;
+  const float *common;  // c
   uint16_t *g;       // [M, ldg]
   int64_t ldg;
 };
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 4 ? 1 : 2) ce_logits_kernel
     } else {
       const float lse = here ? a.lse[row] : 0.0f;
       const bool skip = t == a.ignore;
-      float dl = here && !skip ? a.dloss[row] : 0.0f;
+      float dl = here && !skip ? a.dloss[row] / *a.common : 0.0f;
       if (!skip && (t < 0 || t >= a.V)) dl = __builtin_nanf("");
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
@@ -197,6 +201,7 @@ struct CeProduct {
   int32_t tiles_l, tiles_r, strip;
   void *out;            // leading dimension ld
   int64_t ld, slice_stride;
+  const float *common;  // dw: the factor of the products
 };
 
 // Output of a product: dx partials (fp32, stored or added) along the vocabulary,
@@ -228,9 +233,12 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_product_kerne
              wave);
   }
   const int64_t row0 = 32 * kMT * (wave >> 1), c0 = r0 + 128 * (wave & 1);
+  const float common = kLAcross ? *a.common : 1.0f;
 #pragma unroll
   for (int mt = 0; mt < kMT; ++mt) {
-    auto value = [&](int nt, int v) { return core.acc[mt][nt][v]; };
+    auto value = [&](int nt, int v) {
+      return kLAcross ? fp32_rounded(core.acc[mt][nt][v] * common) : core.acc[mt][nt][v];
+    };
     const int64_t row = l0 + row0 + 32 * mt;
     const int64_t at = slice * a.slice_stride + row * a.ld + c0;
     if constexpr (kOut == kOutBf16)
@@ -243,15 +251,38 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_product_kerne
   }
 }
 
-// dx = the sum of its slices' fp32 sums, rounded once.
+// dx = c times the sum of its slices' fp32 sums, rounded once.
 __global__ void __launch_bounds__(256) ce_dx_kernel(const floatx4 *part, int32_t slices,
-                                                    int64_t chunks, u32x2 *dx) {
+                                                    int64_t chunks, const float *common,
+                                                    u32x2 *dx) {
+  const float c = *common;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks;
        i += (int64_t)gridDim.x * 256) {
     floatx4 s = part[i];
     for (int p = 1; p < slices; ++p) s += part[p * chunks + i];
-    dx[i] = (u32x2){pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
+    dx[i] = (u32x2){pack_bf16x2(fp32_rounded(s[0] * c), fp32_rounded(s[1] * c)),
+                    pack_bf16x2(fp32_rounded(s[2] * c), fp32_rounded(s[3] * c))};
   }
+}
+
+// c = max |dloss|, or 1 if that is zero or not finite.
+__global__ void __launch_bounds__(1024) ce_common_kernel(const float *dloss,
+                                                         const int64_t *targets, int64_t ignore,
+                                                         int64_t M, float *common) {
+  __shared__ float part[16];
+  float top = 0.0f;
+  for (int64_t i = threadIdx.x; i < M; i += 1024) {
+    // A NaN counts as infinite (fmaxf would drop it); an ignored token not at all.
+    const float v = fabsf(dloss[i]);
+    if (targets[i] != ignore) top = fmaxf(top, v < __builtin_inff() ? v : __builtin_inff());
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
+  *common = top == 0.0f || top == __builtin_inff() ? 1.0f : top;
 }
 
 template <typename T>
@@ -306,7 +337,7 @@ static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
   p.slice = up((p.ldg + s - 1) / s, kGcStep);
   p.slices = (p.ldg + p.slice - 1) / p.slice;
   p.g_bytes = up(m * p.ldg * 2, 256);
-  p.bwd_bytes = p.g_bytes + p.slices * m * d * 4;
+  p.bwd_bytes = p.g_bytes + p.slices * m * d * 4 + 16;  // G, dx's sums, c
   const int64_t tokens64 = (m + 63) / 64;
   if (tokens64 * ((v + 127) / 128) > kMaxTiles || ((v + 127) / 128) * ((d + 255) / 256) > kMaxTiles)
     return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many tiles");
@@ -441,6 +472,11 @@ int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *
   }
   uint16_t *g = static_cast<uint16_t *>(workspace);
   float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.g_bytes);
+  float *common = part + p.slices * m * d;
+  hipLaunchKernelGGL(ce_common_kernel, dim3(1), dim3(1024), 0, s, dloss, targets, ignore_index, m,
+                     common);
+  rc = check_launch("ce_common_kernel");
+  if (rc != NF4S_OK) return rc;
   for (int64_t v0 = 0; v0 < v; v0 += p.piece) {
     const int64_t vn = v - v0 < p.piece ? v - v0 : p.piece;
     CeLogits a{};
@@ -455,6 +491,7 @@ int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *
     a.ignore = ignore_index;
     a.lse = lse;
     a.dloss = dloss;
+    a.common = common;
     a.g = g;
     a.ldg = p.ldg;
     rc = ce_logits<true>(p, a, s);
@@ -485,6 +522,7 @@ int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *
     c.out = dw_is_f32 ? static_cast<void *>(static_cast<float *>(dw) + v0 * d)
                       : static_cast<void *>(static_cast<uint16_t *>(dw) + v0 * d);
     c.ld = d;
+    c.common = common;
     rc = accumulate  ? ce_product<4, true, kOutF32Add>(c, s)
          : dw_is_f32 ? ce_product<4, true, kOutF32>(c, s)
                      : ce_product<4, true, kOutBf16>(c, s);
@@ -494,7 +532,7 @@ int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *
   const int64_t blocks = (chunks + 255) / 256;
   hipLaunchKernelGGL(ce_dx_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0,
                      s, reinterpret_cast<const floatx4 *>(part), (int32_t)p.slices, chunks,
-                     reinterpret_cast<u32x2 *>(dx));
+                     common, reinterpret_cast<u32x2 *>(dx));
   return check_launch("ce_dx_kernel");
 }
 

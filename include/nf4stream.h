@@ -387,7 +387,7 @@ int32_t nf4s_block_norm_bwd_workspace_size(int64_t m, int64_t d, int64_t *bytes)
  * last block may be shorter).  Takes the place of the reference's per-channel
  * int8 checkpoints (doublepass/src/checkpoint.rs:21-60,
  * ramflow/kernels/checkpoint_compress.cu:53-145).
- *   scale = max(absmax / 127, 2^-126), code = rint(x * (1 / scale))
+ *   scale = max(absmax * (1 / 127), 2^-126), code = rint(x * (1 / scale))
  * in fp32; a value reads back as code * scale.  A block with an infinity or a
  * NaN has a NaN scale.  d % 4 == 0; fp32 activations 16-byte aligned, bf16 ones
  * 8-byte, codes and scales 4-byte.

@@ -24,7 +24,7 @@ def _reference(x):
     pad = np.zeros((m, blocks * 128), np.float32)
     pad[:, :d] = x
     pad = pad.reshape(m, blocks, 128)
-    scale = np.abs(pad).max(2) / np.float32(127)
+    scale = np.abs(pad).max(2) * (np.float32(1) / np.float32(127))
     # The largest scale: 127 of it are still finite.
     scale = np.clip(scale, np.float32(2.0 ** -126), np.float32(float.fromhex("0x1.020406p+121")))
     inv = np.float32(1) / scale

@@ -108,7 +108,7 @@ def test_workspace_queries():
     for m, v, d in ((4096, 128000, 8192), (65536, 32000, 4096)):
         assert q(m, v, d, 0, ctypes.byref(out)) == 0 and 0 < out.value < m * v // 8
     assert q(4096, 128000, 8192, 1, ctypes.byref(out)) == 0
-    assert out.value <= (256 << 20) + 4096 * 8192 * 4
+    assert out.value <= (256 << 20) + 4096 * 8192 * 4 + 16
     q = lib.nf4s_block_norm_bwd_workspace_size
     assert q(4, 64, None) == INVALID and q(4, 62, ctypes.byref(out)) == SHAPE
     assert q(0, 64, ctypes.byref(out)) == 0 and out.value == 0
