@@ -11,8 +11,8 @@
 // v_mfma_f32_32x32x16_bf16, R as the instruction's first operand: a lane holds
 // one row l of the output and groups of four adjacent columns.
 // Per 64-long step both operands' tiles move into LDS with direct-to-LDS loads,
-// into the stage that step t - 1 used, while step t computes from the other:
-// 2 x 64 KB for 256 x 256.  An operand along the reduction is read with
+// into rings of kNL and kNR stages: while step t computes, L of step t + kNL - 1
+// and R of step t + kNR - 1 are on their way.  An operand along the reduction is read with
 // ds_read_b128, 8 consecutive k of one row a lane; one across it with the
 // transposing reads of tr_tile.hpp.
 #pragma once
@@ -129,19 +129,36 @@ struct GcPlace {
   }
 };
 
+// Stages of the rings.  256 x 256 tiles: 3 of L and 2 of R are the 160 KB of a
+// CU.  128 x 128 and 64 x 256 tiles: 2 of each, and two workgroups a CU; 64 x
+// 128: 3 of each and two workgroups.
+template <int kMT, int kNT>
+constexpr int kGcStagesL = kMT * kNT == 4 ? 2 : 3;
+template <int kMT, int kNT>
+constexpr int kGcStagesR = kMT * kNT == 4 || kMT * kNT == 16 ? 2 : 3;
+
 template <int kMT, int kNT, bool kLAcross, bool kRAcross>
 struct GcCore {
   using LSide = GcSide<kMT, kLAcross>;
   using RSide = GcSide<kNT, kRAcross>;
   static constexpr int kTileL = 64 * kMT, kTileR = 64 * kNT;
-  static constexpr int kStageBytes = LSide::kBytes + RSide::kBytes;
-  static constexpr int kLdsBytes = 2 * kStageBytes;
+  static constexpr int kNL = kGcStagesL<kMT, kNT>, kNR = kGcStagesR<kMT, kNT>;
+  static_assert((kNL == 2 || kNL == 3) && kNR >= 2 && kNR <= kNL, "kInFlight below");
+  static constexpr int kPeriod = kNL == kNR ? kNL : 6;  // steps until both rings are back
+  // DMAs of step t + 2 that may be in flight when step t closes: all, L's, none.
+  static constexpr int kInFlight = kNR == 3 ? LSide::kDmas + RSide::kDmas
+                                            : (kNL == 3 ? LSide::kDmas : 0);
+  static constexpr int kLdsBytes = kNL * LSide::kBytes + kNR * RSide::kBytes;
   static constexpr int kSub = kMT * kNT;       // MFMAs per sub-step
   static constexpr int kPost = kSub / 2;       // those that open the next step
   static constexpr int kFront = 4 * kSub - kPost;
   static constexpr int kReads = kMT + kNT;
   static constexpr int kDmas = LSide::kDmas + RSide::kDmas;
-  static constexpr int kGap = (kFront - 1) / kDmas >= 2 ? 2 : 1;
+  // MFMAs from one DMA to the next.  Reads and DMAs together keep LDS busy for
+  // three quarters of a 256 x 256 step at the MFMA rate: spread over the step
+  // (3) they ran 4096 x 32000 x 8192 logits at 1294 TFLOP/s, every 2 MFMAs
+  // 1259, every one 1156.
+  static constexpr int kGap = (kFront - 1) / kDmas;
   static_assert(kDmas <= kFront, "one DMA per MFMA slot at most");
 
   floatx16 acc[kMT][kNT];
@@ -152,12 +169,12 @@ struct GcCore {
 
   // Fragment read q of a sub-step, in the order its MFMAs use them: l0, r0, r1,
   // .., l1, ..
-  __device__ __forceinline__ void read(const char *tl, const char *tr, int s, int b, int q) {
+  __device__ __forceinline__ void read(const char *lds, int s, int b, int q) {
     if (q == 0 || q > kNT) {
       const int j = q == 0 ? 0 : q - kNT;
-      fl[b][j] = LSide::frag(tl, al, s, j);
+      fl[b][j] = LSide::frag(lds, al, s, j);
     } else {
-      fr[b][q - 1] = RSide::frag(tr, ar, s, q - 1);
+      fr[b][q - 1] = RSide::frag(lds, ar, s, q - 1);
     }
   }
   template <int kI>
@@ -167,35 +184,39 @@ struct GcCore {
         __builtin_bit_cast(bf16x8, fr[b][nt]), __builtin_bit_cast(bf16x8, fl[b][mt]), acc[mt][nt],
         0, 0, 0);
   }
+  // DMA d of a step: R's, which are needed first, then L's.
   template <int kD>
   __device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t rl, __amdgpu_buffer_rsrc_t rr,
-                                      char *nl, char *nr, int wave) {
-    if constexpr (kD < LSide::kDmas)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rl, (lds_void_t *)(nl + LSide::dma_lds(kD, wave)), 16, (int)vl[kD], 0, 0, 0);
-    else
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rr, (lds_void_t *)(nr + RSide::dma_lds(kD - LSide::kDmas, wave)), 16,
-          (int)vr[kD - LSide::kDmas], 0, 0, 0);
+                                      char *nl, char *nr, bool more_l, bool more_r, int wave) {
+    if constexpr (kD < RSide::kDmas) {
+      if (more_r)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rr, (lds_void_t *)(nr + RSide::dma_lds(kD, wave)), 16, (int)vr[kD], 0, 0, 0);
+    } else {
+      constexpr int d = kD - RSide::kDmas;
+      if (more_l)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rl, (lds_void_t *)(nl + LSide::dma_lds(d, wave)), 16, (int)vl[d], 0, 0, 0);
+    }
   }
 
-  // One step from stage `cl`/`cr`: the previous step's last kPost MFMAs with
+  // One step from the stages that al and ar address: the previous step's last kPost MFMAs with
   // the reads of sub-step 0 between them, then 4 sub-steps of kSub, the
-  // fragments of sub-step s + 1 read during sub-step s, the DMAs of step t + 1
-  // (if `more`) into the other stage between the first MFMAs.  That stage was
-  // last read in step t - 1, whose reads ended before the barrier that closed
-  // it.  The __restrict__ stages tell the compiler that DMAs into one never
-  // alias reads of the other, so that it waits for them at the barriers only.
-  __device__ __forceinline__ void step(const char *__restrict__ cl, const char *__restrict__ cr,
-                                       char *__restrict__ nl, char *__restrict__ nr, bool more,
-                                       int wave) {
+  // fragments of sub-step s + 1 read during sub-step s, the DMAs of the steps
+  // ahead (if they exist) into stages `nl`/`nr` between the first MFMAs.  Those
+  // stages were last read in step t - 1, whose reads ended before the barrier
+  // that closed it.  The __restrict__ stages tell the compiler that DMAs into
+  // one never alias reads of the other, so that it waits for them at the
+  // barriers only.
+  __device__ __forceinline__ void step(const char *__restrict__ lds, char *__restrict__ nl,
+                                       char *__restrict__ nr, bool more_l, bool more_r, int wave) {
     const __amdgpu_buffer_rsrc_t rl = pl.rsrc(), rr = pr.rsrc();
     static_for<0, kPost>([&](auto I) {
       constexpr int i = decltype(I)::value;
       mfma<kSub - kPost + i>(1);
       static_for<0, kReads>([&](auto Q) {
         constexpr int q = decltype(Q)::value;
-        if constexpr (q * kPost / kReads == i) read(cl, cr, 0, 0, q);
+        if constexpr (q * kPost / kReads == i) read(lds, 0, 0, q);
       });
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -206,14 +227,35 @@ struct GcCore {
       if constexpr (s < 3) {
         static_for<0, kReads>([&](auto Q) {
           constexpr int q = decltype(Q)::value;
-          if constexpr ((q < kSub ? q : kSub - 1) == i) read(cl, cr, s + 1, (s + 1) & 1, q);
+          if constexpr ((q < kSub ? q : kSub - 1) == i) read(lds, s + 1, (s + 1) & 1, q);
         });
       }
       if constexpr (n % kGap == 0 && n / kGap < kDmas) {
-        if (more) dma<n / kGap>(rl, rr, nl, nr, wave);
+        dma<n / kGap>(rl, rr, nl, nr, more_l, more_r, wave);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
+  }
+
+  // Read addresses from stage kI % kN of a ring to the next.  Opaque, as the
+  // compiler would keep the addresses of every stage in registers.
+  template <int kBytes, int kN, int kI, int kA>
+  static __device__ __forceinline__ void move(uint32_t (&a)[kA]) {
+#pragma unroll
+    for (int i = 0; i < kA; ++i) {
+      a[i] += (kI % kN == kN - 1 ? 1 - kN : 1) * kBytes;
+      asm volatile("" : "+v"(a[i]));
+    }
+  }
+
+  // The barrier that closes step t: this wave's DMAs of step t + 1 have landed
+  // and its LDS reads of step t have ended.  Those of step t + 2 that are already
+  // issued may be in flight: they were issued after step t + 1's.
+  static __device__ __forceinline__ void close_step(int t, int nsteps) {
+    if (t + 2 < nsteps)
+      step_barrier<kInFlight>();
+    else
+      step_barrier<0>();
   }
 
   // The whole product into acc: k elements of the reduction, lds of kLdsBytes.
@@ -221,30 +263,39 @@ struct GcCore {
   // be read) up to the next one.
   __device__ __forceinline__ void run(const GcOperand &l, const GcOperand &r, int64_t k, char *lds,
                                       int lane, int wave) {
-    char *sl[2] = {lds, lds + kStageBytes};
-    char *sr[2] = {lds + LSide::kBytes, lds + kStageBytes + LSide::kBytes};
+    char *sl[kNL], *sr[kNR];
+#pragma unroll
+    for (int i = 0; i < kNL; ++i) sl[i] = lds + i * LSide::kBytes;
+#pragma unroll
+    for (int i = 0; i < kNR; ++i) sr[i] = lds + kNL * LSide::kBytes + i * RSide::kBytes;
     LSide::read_addrs(al, lane, wave >> 1);
     RSide::read_addrs(ar, lane, wave & 1);
+#pragma unroll
+    for (int i = 0; i < RSide::kAddrs; ++i) ar[i] += kNL * LSide::kBytes;
     LSide::dma_offsets(vl, l.ld, lane, wave);
     RSide::dma_offsets(vr, r.ld, lane, wave);
     pl = place<kLAcross>(l);
     pr = place<kRAcross>(r);
     const int nsteps = (int)((k + kGcStep - 1) / kGcStep);
     const int tail = (int)(k % kGcStep);
-    auto before_last = [&](int t) {  // the next DMAs are the last step's
-      if (tail != 0 && t + 1 == nsteps - 1) {
-        LSide::mask_tail(vl, tail, lane, wave);
-        RSide::mask_tail(vr, tail, lane, wave);
-      }
+    // Called with the step whose DMAs are next.
+    auto mask_l = [&](int t) {
+      if (tail != 0 && t == nsteps - 1) LSide::mask_tail(vl, tail, lane, wave);
     };
-    before_last(-1);
-    if (nsteps > 0) {
+    auto mask_r = [&](int t) {
+      if (tail != 0 && t == nsteps - 1) RSide::mask_tail(vr, tail, lane, wave);
+    };
+    static_for<0, kNL - 1>([&](auto P) {
+      constexpr int t = decltype(P)::value;
+      mask_l(t);
+      mask_r(t);
       const __amdgpu_buffer_rsrc_t rl = pl.rsrc(), rr = pr.rsrc();
-      static_for<0, kDmas>(
-          [&](auto D) { dma<decltype(D)::value>(rl, rr, sl[0], sr[0], wave); });
-    }
-    pl.advance();
-    pr.advance();
+      static_for<t < kNR - 1 ? 0 : RSide::kDmas, kDmas>([&](auto D) {
+        dma<decltype(D)::value>(rl, rr, sl[t], sr[t % kNR], t < nsteps, t < nsteps, wave);
+      });
+      pl.advance();
+      if (t < kNR - 1) pr.advance();
+    });
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
@@ -256,25 +307,26 @@ struct GcCore {
     for (int i = 0; i < kMT; ++i) fl[1][i] = (u32x4){0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < kNT; ++i) fr[1][i] = (u32x4){0u, 0u, 0u, 0u};
-    step_barrier<0>();
+    close_step(-1, nsteps);
     int t = 0;
+    auto one = [&](auto P) {
+      constexpr int i = decltype(P)::value;
+      mask_l(t + kNL - 1);
+      mask_r(t + kNR - 1);
+      step(lds, sl[(i + kNL - 1) % kNL], sr[(i + kNR - 1) % kNR], t + kNL - 1 < nsteps,
+           t + kNR - 1 < nsteps, wave);
+      pl.advance();
+      pr.advance();
+      move<LSide::kBytes, kNL, i>(al);
+      move<RSide::kBytes, kNR, i>(ar);
+      close_step(t, nsteps);
+      ++t;
+    };
 #pragma unroll 1
-    for (; t + 2 <= nsteps; t += 2) {
-      before_last(t);
-      step(sl[0], sr[0], sl[1], sr[1], true, wave);
-      pl.advance();
-      pr.advance();
-      step_barrier<0>();
-      before_last(t + 1);
-      step(sl[1], sr[1], sl[0], sr[0], t + 2 < nsteps, wave);
-      pl.advance();
-      pr.advance();
-      step_barrier<0>();
-    }
-    if (t < nsteps) {
-      step(sl[0], sr[0], sl[1], sr[1], false, wave);
-      step_barrier<0>();
-    }
+    while (t + kPeriod <= nsteps) static_for<0, kPeriod>(one);
+    static_for<0, kPeriod - 1>([&](auto P) {
+      if (t < nsteps) one(P);
+    });
     static_for<0, kPost>([&](auto I) { mfma<kSub - kPost + decltype(I)::value>(1); });
   }
 
