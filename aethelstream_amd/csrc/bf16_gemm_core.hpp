@@ -130,7 +130,7 @@ struct GcPlace {
 };
 
 // Stages of the rings.  256 x 256 tiles: 3 of L and 2 of R are the 160 KB of a
-// CU.  128 x 128 and 64 x 256 tiles: 2 of each, and two workgroups a CU; 64 x
+// CU.  64 x 256 and 128 x 128 tiles: 2 of each, and two workgroups a CU; 64 x
 // 128: 3 of each and two workgroups.
 template <int kMT, int kNT>
 constexpr int kGcStagesL = kMT * kNT == 4 ? 2 : 3;
@@ -366,7 +366,7 @@ __device__ __forceinline__ void gc_wave_sync() {
 // bytes of LDS, whole rows of 64 kNT bytes: value(nt, v) is the lane's register
 // v of column tile nt, already final.  `out` points at row 0, column 0 of the
 // block; `rows` and `cols` (a multiple of 8) bound it.
-template <int kNT, class F>
+template <int kNT, bool kNt, class F>
 __device__ __forceinline__ void gc_store_bf16(F &&value, char *lds, uint16_t *out, int64_t ld,
                                               int64_t rows, int64_t cols, int lane) {
   constexpr int kChunks = 4 * kNT;  // 16-byte chunks of a row
@@ -388,14 +388,20 @@ __device__ __forceinline__ void gc_store_bf16(F &&value, char *lds, uint16_t *ou
     const int r = kRows * i + r0;
     const u32x4 w = *reinterpret_cast<const u32x4 *>(lds + 16 * kChunks * r +
                                                      16 * (c ^ (r & (kChunks - 1))));
-    if (r < rows && 8 * c < cols) *reinterpret_cast<u32x4 *>(out + r * ld + 8 * c) = w;
+    if (r < rows && 8 * c < cols) {
+      u32x4 *p = reinterpret_cast<u32x4 *>(out + r * ld + 8 * c);
+      if constexpr (kNt)
+        __builtin_nontemporal_store(w, p);
+      else
+        *p = w;
+    }
   }
   gc_wave_sync();
 }
 
 // The same for fp32 values, through 32 * 128 * kNT bytes; kAdd: added to what is
 // there.
-template <int kNT, bool kAdd, class F>
+template <int kNT, bool kAdd, bool kNt, class F>
 __device__ __forceinline__ void gc_store_f32(F &&value, char *lds, float *out, int64_t ld,
                                              int64_t rows, int64_t cols, int lane) {
   constexpr int kChunks = 8 * kNT;
@@ -420,7 +426,10 @@ __device__ __forceinline__ void gc_store_f32(F &&value, char *lds, float *out, i
     if (r < rows && 4 * c < cols) {
       floatx4 *p = reinterpret_cast<floatx4 *>(out + r * ld + 4 * c);
       if constexpr (kAdd) w += *p;
-      *p = w;
+      if constexpr (kNt)
+        __builtin_nontemporal_store(w, p);
+      else
+        *p = w;
     }
   }
   gc_wave_sync();

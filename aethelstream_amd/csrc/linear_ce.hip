@@ -54,7 +54,7 @@ struct CeLogits {
   const float *lse, *dloss;
   const float *common;  // c
   uint16_t *g;       // [M, ldg]
-  int64_t ldg;
+  int64_t ldg, gcols;  // row length of G, columns of it from g on
 };
 
 __device__ __forceinline__ float other_half(float v) {
@@ -71,7 +71,7 @@ __device__ __forceinline__ float exp_of(float x) {
 // Column of the wave's block (0 .. 32 kNT - 1) of the lane's register v of
 // column tile nt is 32 nt + 8 (v / 4) + 4 (lane / 32) + v % 4.
 template <int kMT, int kNT, bool kGrad>
-__global__ void __launch_bounds__(kGcThreads, kMT == 4 ? 1 : 2) ce_logits_kernel(const CeLogits a) {
+__global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_logits_kernel(const CeLogits a) {
   using Core = GcCore<kMT, kNT, false, false>;
   __shared__ __attribute__((aligned(16))) char lds[Core::kLdsBytes];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -153,35 +153,50 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 4 ? 1 : 2) ce_logits_kernel
           for (int v = 0; v < 16; ++v) z[nt][v] -= at == 16 * nt + v ? 1.0f : 0.0f;
       }
       // Columns of the piece's last, partial 64 hold zeros: G is read in steps of 64.
-      gc_store_bf16<kNT>(
+      gc_store_bf16<kNT, false>(
           [&](int nt, int v) { return skip ? 0.0f : fp32_rounded(z[nt][v] * dl); },
           lds + 32 * 64 * kNT * wave, a.g + (row0 + 32 * mt) * a.ldg + r0 + c0, a.ldg,
-          a.M - (row0 + 32 * mt), a.ldg - (r0 + c0), lane);
+          a.M - (row0 + 32 * mt), a.gcols - (r0 + c0), lane);
     }
   }
 }
 
-// Joins a token's partial sums: 32 threads a token take every 32nd slice, then
-// meet in a fixed order.
+// Joins a token's partial sums: 256 / kTokens threads a token take every so many
+// slices, four loads ahead, then meet in a fixed order.
+template <int kTokens>
 __global__ void __launch_bounds__(256) ce_join_kernel(const float2 *part, const float *zt,
                                                       const int64_t *targets, int64_t M,
                                                       int32_t slices, int64_t V, int64_t ignore,
                                                       float *loss, float *lse) {
-  __shared__ float2 lds[32][8];
-  const int tok = threadIdx.x & 7, grp = threadIdx.x >> 3;
-  const int64_t row = (int64_t)blockIdx.x * 8 + tok;
+  constexpr int kGroups = 256 / kTokens;
+  __shared__ float2 lds[kGroups][kTokens];
+  const int tok = threadIdx.x % kTokens, grp = threadIdx.x / kTokens;
+  const int64_t row = (int64_t)blockIdx.x * kTokens + tok;
   auto join = [](float2 a, float2 b) {
     const float top = fmaxf(a.x, b.x);
     const float ref = top == -__builtin_inff() ? 0.0f : top;
     return make_float2(top, a.y * exp_of(a.x - ref) + b.y * exp_of(b.x - ref));
   };
-  float2 s = make_float2(-__builtin_inff(), 0.0f);
+  const float2 none = make_float2(-__builtin_inff(), 0.0f);
+  float2 s = none;
   if (row < M)
-    for (int i = grp; i < slices; i += 32) s = join(s, part[(int64_t)i * M + row]);
+    for (int i = grp; i < slices; i += 4 * kGroups) {
+      float2 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = i + j * kGroups;
+        v[j] = n < slices ? part[(int64_t)n * M + row] : none;
+      }
+      s = join(s, join(join(v[0], v[1]), join(v[2], v[3])));
+    }
   lds[grp][tok] = s;
-  __syncthreads();
+#pragma unroll
+  for (int half = kGroups / 2; half >= 1; half /= 2) {
+    __syncthreads();
+    if (grp < half) lds[grp][tok] = join(lds[grp][tok], lds[grp + half][tok]);
+  }
   if (grp != 0 || row >= M) return;
-  for (int i = 1; i < 32; ++i) s = join(s, lds[i][tok]);
+  s = lds[0][tok];
   const float l = s.x + __builtin_amdgcn_logf(s.y) * kLn2;
   lse[row] = l;
   const int64_t t = targets[row];
@@ -205,7 +220,8 @@ struct CeProduct {
 };
 
 // Output of a product: dx partials (fp32, stored or added) along the vocabulary,
-// dw (fp32 or bf16) along the tokens.
+// dw (fp32 or bf16) along the tokens.  dw is not read again and leaves by
+// non-temporal stores: 77 tokens, 32000 x 4096, gradients 228 -> 203 us.
 enum { kOutF32, kOutF32Add, kOutBf16 };
 
 template <int kMT, bool kLAcross, int kOut>
@@ -242,10 +258,10 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_product_kerne
     const int64_t row = l0 + row0 + 32 * mt;
     const int64_t at = slice * a.slice_stride + row * a.ld + c0;
     if constexpr (kOut == kOutBf16)
-      gc_store_bf16<4>(value, lds + 8192 * wave, static_cast<uint16_t *>(a.out) + at, a.ld,
+      gc_store_bf16<4, true>(value, lds + 8192 * wave, static_cast<uint16_t *>(a.out) + at, a.ld,
                        a.rows - row, a.cols - c0, lane);
     else
-      gc_store_f32<4, kOut == kOutF32Add>(value, lds + 16384 * wave,
+      gc_store_f32<4, kOut == kOutF32Add, kLAcross>(value, lds + 16384 * wave,
                                           static_cast<float *>(a.out) + at, a.ld, a.rows - row,
                                           a.cols - c0, lane);
   }
@@ -298,15 +314,98 @@ constexpr int kCeStrip = 4;
 
 static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
-// Tile heights (64 kMT tokens) of the logits and of dx.
-static int ce_mt(int64_t m) { return m <= 64 ? 1 : (m <= 128 ? 2 : 4); }
+// Tile heights (64 kMT tokens) of dx.
+static int ce_dx_mt(int64_t m) { return m <= 64 ? 1 : (m <= 128 ? 2 : 4); }
+
+// A logits launch: 64 mt x 64 nt tiles over the next `cols` columns.
+struct CeLaunch {
+  int mt, nt;
+  int64_t cols;
+};
+
+// The tiles of m > 0 tokens by v > 0 columns of length d, as one launch, or as whole
+// rounds of large tiles and the rest in smaller ones.  Cost of a launch in us:
+// each round takes, per step of 64, `lo` when few tiles run to `hi` when the
+// chip is full (less traffic and a higher clock when it is not); w is read at
+// `tbs`, again by part for each further row of tiles; 8 us beside.  Fitted to
+// forwards of 1 to 1500 tokens over 1000 to 128000 columns, d = 1024 to 8192
+// (times in us at d = 4096 with 64 x 128, 128 x 256 and 256 x 256 tiles):
+//   1 token, 32000 columns 45, 52, 81;  128 tokens 65, 62, 89;
+//   256 tokens 97, 70, 96;  512 tokens 163, 126, 114;
+//   1000 tokens, 50021 columns 556, 409, 398.
+// 128 x 128 and 128 x 64 tiles were within 3 % of the best of the three at
+// most, and are not built.
+struct CeTile {
+  int mt, nt, slots;  // slots: workgroups a CU
+  double lo, hi, tbs;
+};
+constexpr CeTile kCeTiles[3] = {{1, 2, 2, 0.30, 0.62, 5.4}, {2, 4, 1, 0.66, 0.92, 5.7},
+                                {4, 4, 1, 1.14, 1.62, 5.4}};
+
+static int64_t ceil_to(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static double ce_cost(const CeTile &c, int64_t m, int64_t v, int64_t d) {
+  const int64_t tl = ceil_to(m, 64 * c.mt), T = tl * ceil_to(v, 64 * c.nt);
+  const int64_t slots = (int64_t)cu_slots() * c.slots;
+  const double steps = (double)ceil_to(d, kGcStep);
+  const double part = (double)(T % slots) / (double)slots;
+  const double compute =
+      steps * ((double)(T / slots) * c.hi + (part > 0.0 ? c.lo + (c.hi - c.lo) * part : 0.0));
+  const double memory = 2e-6 * (double)v * (double)d / c.tbs * (0.75 + 0.25 * (double)tl);
+  return 8.0 + (compute > memory ? compute : memory);
+}
+
+static int ce_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&out)[2]) {
+  double best = 1e300;
+  int count = 0;
+  auto smallest = [&](int64_t cols, int upto, const CeTile *&c) {
+    double least = 1e300;
+    for (int i = 0; i < upto; ++i) {
+      const double t = ce_cost(kCeTiles[i], m, cols, d);
+      if (t < least) {
+        least = t;
+        c = &kCeTiles[i];
+      }
+    }
+    return least;
+  };
+  const CeTile *c = nullptr;
+  best = smallest(v, 3, c);
+  out[0] = CeLaunch{c->mt, c->nt, v};
+  count = 1;
+  for (int i = 1; i < 3; ++i) {
+    const CeTile &a = kCeTiles[i];
+    const int64_t tl = ceil_to(m, 64 * a.mt), T = tl * ceil_to(v, 64 * a.nt);
+    const int64_t rounds = T / cu_slots();
+    const int64_t cols = rounds * cu_slots() / tl * (64 * a.nt);
+    if (rounds == 0 || cols == 0 || cols >= v) continue;
+    const double t = ce_cost(a, m, cols, d) + smallest(v - cols, i, c);
+    if (t < best) {
+      best = t;
+      out[0] = CeLaunch{a.mt, a.nt, cols};
+      out[1] = CeLaunch{c->mt, c->nt, v - cols};
+      count = 2;
+    }
+  }
+  return count;
+}
+
+// Partial sums a token leaves: one for each half tile.
+static int64_t ce_slices(int64_t m, int64_t v, int64_t d) {
+  CeLaunch l[2];
+  const int n = ce_tiles(m, v, d, l);
+  int64_t s = 0;
+  for (int i = 0; i < n; ++i) s += 2 * ceil_to(l[i].cols, 64 * l[i].nt);
+  return s;
+}
 
 struct CePlan {
-  int mt, nt;            // logits tile
   int64_t tokens;        // forward: tokens of one launch
+  int64_t part_bytes, fwd_bytes;
   int64_t piece, ldg;    // backward: columns of a piece, row length of G
+  int dx_mt;
   int64_t slices, slice; // of dx's reduction over a piece
-  int64_t fwd_bytes, g_bytes, bwd_bytes;
+  int64_t g_bytes, bwd_bytes;
 };
 
 static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
@@ -321,11 +420,16 @@ static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
     return fail(NF4S_ERR_UNSUPPORTED_SHAPE,
                 "cross entropy of m=%lld v=%lld d=%lld beyond m 2^24, v 2^28, d 2^20",
                 (long long)m, (long long)v, (long long)d);
-  p.mt = ce_mt(m);
-  p.nt = p.mt == 4 ? 4 : 2;
+  if (ceil_to(m, 64) * ceil_to(v, 128) > kMaxTiles || ceil_to(v, 128) * ceil_to(d, 128) > kMaxTiles)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many tiles");
   p.tokens = m < kCeTokens ? m : kCeTokens;
-  const int64_t slices = 2 * ((v + 64 * p.nt - 1) / (64 * p.nt));
-  p.fwd_bytes = up(slices * p.tokens * 8, 256) + p.tokens * 4;
+  p.part_bytes = m > 0 ? ce_slices(p.tokens, v, d) * p.tokens : 0;
+  if (m > 0 && m % p.tokens != 0) {
+    const int64_t last = ce_slices(m % p.tokens, v, d) * (m % p.tokens);
+    if (last > p.part_bytes) p.part_bytes = last;
+  }
+  p.part_bytes = up(p.part_bytes * 8, 256);
+  p.fwd_bytes = p.part_bytes + p.tokens * 4;
   int64_t most = m > 0 ? kCePieceBytes / (2 * m) / 256 * 256 : v;
   most = most < 256 ? 256 : (most > (1 << 20) ? (1 << 20) : most);
   const int64_t pieces = (v + most - 1) / most;
@@ -333,32 +437,47 @@ static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
   if (p.piece > v) p.piece = v;
   p.ldg = up(p.piece, 64);
   // Slices of dx's reduction: as many as fill the chip, of at least 8 steps.
-  const int64_t tiles = ((m + 64 * p.mt - 1) / (64 * p.mt)) * ((d + 255) / 256);
-  const int64_t slots = (int64_t)cu_slots() * (p.mt == 1 ? 2 : 1);
+  p.dx_mt = ce_dx_mt(m);
+  const int64_t tiles = ceil_to(m, 64 * p.dx_mt) * ceil_to(d, 256);
+  const int64_t slots = (int64_t)cu_slots() * (p.dx_mt == 1 ? 2 : 1);
   int64_t s = tiles > 0 ? slots / tiles : 1;
-  const int64_t least = (p.ldg + 8 * kGcStep - 1) / (8 * kGcStep);
+  const int64_t least = ceil_to(p.ldg, 8 * kGcStep);
   s = s < 1 ? 1 : (s > least ? least : s);
-  p.slice = up((p.ldg + s - 1) / s, kGcStep);
-  p.slices = (p.ldg + p.slice - 1) / p.slice;
+  p.slice = up(ceil_to(p.ldg, s), kGcStep);
+  p.slices = ceil_to(p.ldg, p.slice);
   p.g_bytes = up(m * p.ldg * 2, 256);
   p.bwd_bytes = p.g_bytes + p.slices * m * d * 4 + 16;  // G, dx's sums, c
-  const int64_t tokens64 = (m + 63) / 64;
-  if (tokens64 * ((v + 127) / 128) > kMaxTiles || ((v + 127) / 128) * ((d + 255) / 256) > kMaxTiles)
-    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many tiles");
   return NF4S_OK;
 }
 
+// The logits of a.M tokens and a.vn columns, in one launch or two; *slices: the
+// partial sums of a token.
 template <bool kGrad>
-static int32_t ce_logits(const CePlan &p, CeLogits a, hipStream_t s) {
-  a.tiles_l = (int32_t)((a.M + 64 * p.mt - 1) / (64 * p.mt));
-  a.tiles_r = (int32_t)((a.vn + 64 * p.nt - 1) / (64 * p.nt));
-  a.strip = kCeStrip;
-  auto *kernel = p.mt == 4   ? ce_logits_kernel<4, 4, kGrad>
-                 : p.mt == 2 ? ce_logits_kernel<2, 2, kGrad>
-                             : ce_logits_kernel<1, 2, kGrad>;
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)a.tiles_l * (uint32_t)a.tiles_r), dim3(kGcThreads), 0,
-                     s, a);
-  return check_launch("ce_logits_kernel");
+static int32_t ce_logits(CeLogits a, int64_t *slices, hipStream_t s) {
+  CeLaunch l[2];
+  const int n = ce_tiles(a.M, a.vn, a.d, l);
+  int64_t done = 0;
+  for (int i = 0; i < n; ++i) {
+    a.vn = (int32_t)l[i].cols;
+    a.tiles_l = (int32_t)ceil_to(a.M, 64 * l[i].mt);
+    a.tiles_r = (int32_t)ceil_to(a.vn, 64 * l[i].nt);
+    a.strip = kCeStrip;
+    auto *kernel = l[i].mt == 4   ? ce_logits_kernel<4, 4, kGrad>
+                   : l[i].mt == 2 ? ce_logits_kernel<2, 4, kGrad>
+                                  : ce_logits_kernel<1, 2, kGrad>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)a.tiles_l * (uint32_t)a.tiles_r), dim3(kGcThreads),
+                       0, s, a);
+    const int32_t rc = check_launch("ce_logits_kernel");
+    if (rc != NF4S_OK) return rc;
+    a.w += a.vn * a.d;
+    a.v0 += a.vn;
+    if (kGrad) a.g += a.vn;
+    if (!kGrad) a.part += 2 * a.tiles_r * a.M;
+    a.gcols -= a.vn;
+    done += 2 * a.tiles_r;
+  }
+  if (slices != nullptr) *slices = done;
+  return NF4S_OK;
 }
 
 template <int kMT, bool kLAcross, int kOut>
@@ -375,9 +494,9 @@ static int32_t ce_product(CeProduct a, hipStream_t s) {
 
 template <int kOut>
 static int32_t ce_dx_piece(const CePlan &p, const CeProduct &a, hipStream_t s) {
-  return p.mt == 4   ? ce_product<4, false, kOut>(a, s)
-         : p.mt == 2 ? ce_product<2, false, kOut>(a, s)
-                     : ce_product<1, false, kOut>(a, s);
+  return p.dx_mt == 4   ? ce_product<4, false, kOut>(a, s)
+         : p.dx_mt == 2 ? ce_product<2, false, kOut>(a, s)
+                        : ce_product<1, false, kOut>(a, s);
 }
 
 static int32_t ce_operands(const uint16_t *x, const uint16_t *w, const int64_t *targets, int64_t m,
@@ -425,7 +544,6 @@ int32_t nf4s_linear_ce_fwd(const uint16_t *x, const uint16_t *w, const int64_t *
   if (!aligned(loss, 4) || !aligned(lse, 4))
     return fail(NF4S_ERR_MISALIGNED, "loss and lse must be 4-byte aligned");
   const hipStream_t s = as_stream(stream);
-  const int32_t slices = (int32_t)(2 * ((v + 64 * p.nt - 1) / (64 * p.nt)));
   CeLogits a{};
   a.w = w;
   a.d = d;
@@ -433,16 +551,18 @@ int32_t nf4s_linear_ce_fwd(const uint16_t *x, const uint16_t *w, const int64_t *
   a.V = v;
   a.ignore = ignore_index;
   a.part = static_cast<float2 *>(workspace);
-  a.zt = reinterpret_cast<float *>(static_cast<char *>(workspace) +
-                                   up((int64_t)slices * p.tokens * 8, 256));
+  a.zt = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.part_bytes);
   for (int64_t m0 = 0; m0 < m; m0 += p.tokens) {
     a.M = m - m0 < p.tokens ? m - m0 : p.tokens;
     a.x = x + m0 * d;
     a.targets = targets + m0;
-    rc = ce_logits<false>(p, a, s);
+    int64_t slices = 0;
+    rc = ce_logits<false>(a, &slices, s);
     if (rc != NF4S_OK) return rc;
-    hipLaunchKernelGGL(ce_join_kernel, dim3((uint32_t)((a.M + 7) / 8)), dim3(256), 0, s, a.part,
-                       a.zt, a.targets, a.M, slices, v, ignore_index, loss + m0, lse + m0);
+    const bool few = a.M < 512;
+    hipLaunchKernelGGL(few ? ce_join_kernel<1> : ce_join_kernel<8>,
+                       dim3((uint32_t)(few ? a.M : (a.M + 7) / 8)), dim3(256), 0, s, a.part, a.zt,
+                       a.targets, a.M, (int32_t)slices, v, ignore_index, loss + m0, lse + m0);
     rc = check_launch("ce_join_kernel");
     if (rc != NF4S_OK) return rc;
   }
@@ -497,8 +617,8 @@ int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *
     a.dloss = dloss;
     a.common = common;
     a.g = g;
-    a.ldg = p.ldg;
-    rc = ce_logits<true>(p, a, s);
+    a.ldg = a.gcols = p.ldg;
+    rc = ce_logits<true>(a, nullptr, s);
     if (rc != NF4S_OK) return rc;
     CeProduct b{};  // dx += G . w
     b.l = g;
