@@ -24,6 +24,8 @@
 // piece: logits again, turned into G in the epilogue;
 // dx += G . w in fp32; the piece's rows of dw.  The four products of a training
 // step are matrix-rate bound, the forward of few tokens reads w at memory rate.
+#include <cmath>
+
 #include "bf16_gemm_core.hpp"
 
 namespace nf4s {
@@ -224,10 +226,10 @@ struct CeProduct {
 // non-temporal stores: 77 tokens, 32000 x 4096, gradients 228 -> 203 us.
 enum { kOutF32, kOutF32Add, kOutBf16 };
 
-template <int kMT, bool kLAcross, int kOut>
-__global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_product_kernel(
+template <int kMT, int kNT, bool kLAcross, int kOut>
+__global__ void __launch_bounds__(kGcThreads, kMT * kNT == 4 ? 2 : 1) ce_product_kernel(
     const CeProduct a) {
-  using Core = GcCore<kMT, 4, kLAcross, true>;
+  using Core = GcCore<kMT, kNT, kLAcross, true>;
   __shared__ __attribute__((aligned(16))) char lds[Core::kLdsBytes];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_product_kerne
     core.run(gc_along(a.l + l0 * a.ldl + k0, a.ldl, rows, (k + 7) & ~(int64_t)7), r, k, lds, lane,
              wave);
   }
-  const int64_t row0 = 32 * kMT * (wave >> 1), c0 = r0 + 128 * (wave & 1);
+  const int64_t row0 = 32 * kMT * (wave >> 1), c0 = r0 + 32 * kNT * (wave & 1);
   const float common = kLAcross ? *a.common : 1.0f;
 #pragma unroll
   for (int mt = 0; mt < kMT; ++mt) {
@@ -258,10 +260,10 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_product_kerne
     const int64_t row = l0 + row0 + 32 * mt;
     const int64_t at = slice * a.slice_stride + row * a.ld + c0;
     if constexpr (kOut == kOutBf16)
-      gc_store_bf16<4, true>(value, lds + 8192 * wave, static_cast<uint16_t *>(a.out) + at, a.ld,
+      gc_store_bf16<kNT, true>(value, lds + 2048 * kNT * wave, static_cast<uint16_t *>(a.out) + at, a.ld,
                        a.rows - row, a.cols - c0, lane);
     else
-      gc_store_f32<4, kOut == kOutF32Add, kLAcross>(value, lds + 16384 * wave,
+      gc_store_f32<kNT, kOut == kOutF32Add, kLAcross>(value, lds + 4096 * kNT * wave,
                                           static_cast<float *>(a.out) + at, a.ld, a.rows - row,
                                           a.cols - c0, lane);
   }
@@ -308,14 +310,13 @@ __global__ void ce_zero_kernel(T *p, int64_t n) {
     p[i] = T(0);
 }
 
+constexpr int64_t kCeFewTokens = 128;
+
 // Tile columns of a strip (gc_tile): 4096 x 32000 x 8192 logits 1601 us with 4,
 // 1627 with 6, 1659 with 8, 2056 with 16 (that one before the third L stage).
 constexpr int kCeStrip = 4;
 
 static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-
-// Tile heights (64 kMT tokens) of dx.
-static int ce_dx_mt(int64_t m) { return m <= 64 ? 1 : (m <= 128 ? 2 : 4); }
 
 // A logits launch: 64 mt x 64 nt tiles over the next `cols` columns.
 struct CeLaunch {
@@ -327,8 +328,8 @@ struct CeLaunch {
 // rounds of large tiles and the rest in smaller ones.  Cost of a launch in us:
 // each round takes, per step of 64, `lo` when few tiles run to `hi` when the
 // chip is full (less traffic and a higher clock when it is not); w is read at
-// `tbs`, again by part for each further row of tiles; 8 us beside.  Fitted to
-// forwards of 1 to 1500 tokens over 1000 to 128000 columns, d = 1024 to 8192
+// `tbs`, again by part for each further row of tiles; 8 us beside, 14 for a
+// second launch.  Fitted to forwards of 1 to 1500 tokens over 1000 to 128000 columns, d = 1024 to 8192
 // (times in us at d = 4096 with 64 x 128, 128 x 256 and 256 x 256 tiles):
 //   1 token, 32000 columns 45, 52, 81;  128 tokens 65, 62, 89;
 //   256 tokens 97, 70, 96;  512 tokens 163, 126, 114;
@@ -339,7 +340,7 @@ struct CeTile {
   int mt, nt, slots;  // slots: workgroups a CU
   double lo, hi, tbs;
 };
-constexpr CeTile kCeTiles[3] = {{1, 2, 2, 0.30, 0.62, 5.4}, {2, 4, 1, 0.66, 0.92, 5.7},
+constexpr CeTile kCeTiles[3] = {{1, 2, 2, 0.30, 0.70, 5.4}, {2, 4, 1, 0.66, 0.92, 5.7},
                                 {4, 4, 1, 1.14, 1.62, 5.4}};
 
 static int64_t ceil_to(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -356,10 +357,10 @@ static double ce_cost(const CeTile &c, int64_t m, int64_t v, int64_t d) {
 }
 
 static int ce_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&out)[2]) {
-  double best = 1e300;
+  double best = HUGE_VAL;
   int count = 0;
   auto smallest = [&](int64_t cols, int upto, const CeTile *&c) {
-    double least = 1e300;
+    double least = HUGE_VAL;
     for (int i = 0; i < upto; ++i) {
       const double t = ce_cost(kCeTiles[i], m, cols, d);
       if (t < least) {
@@ -379,7 +380,7 @@ static int ce_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&out)[2]) {
     const int64_t rounds = T / cu_slots();
     const int64_t cols = rounds * cu_slots() / tl * (64 * a.nt);
     if (rounds == 0 || cols == 0 || cols >= v) continue;
-    const double t = ce_cost(a, m, cols, d) + smallest(v - cols, i, c);
+    const double t = ce_cost(a, m, cols, d) + smallest(v - cols, i, c) + 6.0;
     if (t < best) {
       best = t;
       out[0] = CeLaunch{a.mt, a.nt, cols};
@@ -408,6 +409,44 @@ struct CePlan {
   int64_t g_bytes, bwd_bytes;
 };
 
+// Tile height of dx and slices of its reduction over a piece, by the least of:
+// the rounds' time, as for the logits, joined with that of reading w by their
+// fourth powers (the larger one, a little more where they are close); what the
+// slices' fp32 sums move at 2.4 TB/s (written, read and written by each further
+// piece, read for the join).  Fitted to 1 to 4096 tokens, 8000 to 50021
+// columns, d = 1024 to 8192, all heights and 1 to 32 slices: 1 % from the best
+// on average, 6 % at most.  The gradients of 777 x 32000 x 4096: 659 us with 14
+// tiles of 128 rows x 2 slices, 663 with 256 rows x 4, 995 with 256 rows in one.
+constexpr CeTile kCeDxTiles[3] = {{1, 4, 2, 0.75, 0.97, 5.0}, {2, 4, 1, 0.61, 0.88, 5.0},
+                                  {4, 4, 1, 0.95, 1.03, 6.0}};
+static void ce_dx_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
+  const double pieces = (double)ceil_to(v, p.piece);
+  const int64_t steps = ceil_to(p.ldg, kGcStep);
+  double best = HUGE_VAL;
+  for (const CeTile &c : kCeDxTiles) {
+    const int64_t tl = ceil_to(m, 64 * c.mt), T = tl * ceil_to(d, 64 * c.nt);
+    const int64_t slots = (int64_t)cu_slots() * c.slots;
+    for (int64_t s = 1; s <= 32 && (s == 1 || steps >= 4 * s) && T * s <= kMaxTiles; ++s) {
+      const int64_t each = ceil_to(steps, s), n = T * ceil_to(steps, each);
+      const double part = (double)(n % slots) / (double)slots;
+      const double compute =
+          (double)each *
+          ((double)(n / slots) * c.hi + (part > 0.0 ? c.lo + (c.hi - c.lo) * part : 0.0));
+      const double memory =
+          2e-6 * (double)p.piece * (double)d / c.tbs * (0.75 + 0.25 * (double)tl);
+      const double sums = 8e-6 * (double)(n / T) * (double)m * (double)d / 2.4;
+      const double c2 = compute * compute, m2 = memory * memory;
+      const double cost = pieces * (sums + std::sqrt(std::sqrt(c2 * c2 + m2 * m2)));
+      if (cost < best) {
+        best = cost;
+        p.dx_mt = c.mt;
+        p.slice = each * kGcStep;
+      }
+    }
+  }
+  p.slices = ceil_to(p.ldg, p.slice);
+}
+
 static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
   if (m < 0 || v <= 0 || d <= 0)
     return fail(NF4S_ERR_INVALID_ARGUMENT, "bad cross-entropy shape m=%lld v=%lld d=%lld",
@@ -420,7 +459,8 @@ static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
     return fail(NF4S_ERR_UNSUPPORTED_SHAPE,
                 "cross entropy of m=%lld v=%lld d=%lld beyond m 2^24, v 2^28, d 2^20",
                 (long long)m, (long long)v, (long long)d);
-  if (ceil_to(m, 64) * ceil_to(v, 128) > kMaxTiles || ceil_to(v, 128) * ceil_to(d, 128) > kMaxTiles)
+  if (ceil_to(m, 64) * ceil_to(v, 128) > kMaxTiles ||
+      ceil_to(v, 128) * ceil_to(d, 128) > kMaxTiles || ceil_to(m, 64) * ceil_to(d, 256) > kMaxTiles)
     return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many tiles");
   p.tokens = m < kCeTokens ? m : kCeTokens;
   p.part_bytes = m > 0 ? ce_slices(p.tokens, v, d) * p.tokens : 0;
@@ -436,15 +476,7 @@ static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
   p.piece = up((v + pieces - 1) / pieces, 256);
   if (p.piece > v) p.piece = v;
   p.ldg = up(p.piece, 64);
-  // Slices of dx's reduction: as many as fill the chip, of at least 8 steps.
-  p.dx_mt = ce_dx_mt(m);
-  const int64_t tiles = ceil_to(m, 64 * p.dx_mt) * ceil_to(d, 256);
-  const int64_t slots = (int64_t)cu_slots() * (p.dx_mt == 1 ? 2 : 1);
-  int64_t s = tiles > 0 ? slots / tiles : 1;
-  const int64_t least = ceil_to(p.ldg, 8 * kGcStep);
-  s = s < 1 ? 1 : (s > least ? least : s);
-  p.slice = up(ceil_to(p.ldg, s), kGcStep);
-  p.slices = ceil_to(p.ldg, p.slice);
+  ce_dx_plan(m, v, d, p);
   p.g_bytes = up(m * p.ldg * 2, 256);
   p.bwd_bytes = p.g_bytes + p.slices * m * d * 4 + 16;  // G, dx's sums, c
   return NF4S_OK;
@@ -480,13 +512,13 @@ static int32_t ce_logits(CeLogits a, int64_t *slices, hipStream_t s) {
   return NF4S_OK;
 }
 
-template <int kMT, bool kLAcross, int kOut>
+template <int kMT, int kNT, bool kLAcross, int kOut>
 static int32_t ce_product(CeProduct a, hipStream_t s) {
-  a.tiles_l = (int32_t)((a.rows + 64 * kMT - 1) / (64 * kMT));
-  a.tiles_r = (int32_t)((a.cols + 255) / 256);
+  a.tiles_l = (int32_t)ceil_to(a.rows, 64 * kMT);
+  a.tiles_r = (int32_t)ceil_to(a.cols, 64 * kNT);
   a.strip = kCeStrip;
   const int64_t slices = (a.k + a.slice - 1) / a.slice;
-  auto *kernel = ce_product_kernel<kMT, kLAcross, kOut>;
+  auto *kernel = ce_product_kernel<kMT, kNT, kLAcross, kOut>;
   hipLaunchKernelGGL(kernel, dim3((uint32_t)(slices * a.tiles_l * a.tiles_r)), dim3(kGcThreads), 0,
                      s, a);
   return check_launch("ce_product_kernel");
@@ -494,9 +526,15 @@ static int32_t ce_product(CeProduct a, hipStream_t s) {
 
 template <int kOut>
 static int32_t ce_dx_piece(const CePlan &p, const CeProduct &a, hipStream_t s) {
-  return p.dx_mt == 4   ? ce_product<4, false, kOut>(a, s)
-         : p.dx_mt == 2 ? ce_product<2, false, kOut>(a, s)
-                        : ce_product<1, false, kOut>(a, s);
+  return p.dx_mt == 4   ? ce_product<4, 4, false, kOut>(a, s)
+         : p.dx_mt == 2 ? ce_product<2, 4, false, kOut>(a, s)
+                        : ce_product<1, 4, false, kOut>(a, s);
+}
+
+template <int kOut>
+static int32_t ce_dw_piece(const CeProduct &a, hipStream_t s) {
+  return a.k <= kCeFewTokens ? ce_product<2, 2, true, kOut>(a, s)
+                             : ce_product<4, 4, true, kOut>(a, s);
 }
 
 static int32_t ce_operands(const uint16_t *x, const uint16_t *w, const int64_t *targets, int64_t m,
@@ -647,9 +685,9 @@ int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *
                       : static_cast<void *>(static_cast<uint16_t *>(dw) + v0 * d);
     c.ld = d;
     c.common = common;
-    rc = accumulate  ? ce_product<4, true, kOutF32Add>(c, s)
-         : dw_is_f32 ? ce_product<4, true, kOutF32>(c, s)
-                     : ce_product<4, true, kOutBf16>(c, s);
+    rc = accumulate  ? ce_dw_piece<kOutF32Add>(c, s)
+         : dw_is_f32 ? ce_dw_piece<kOutF32>(c, s)
+                     : ce_dw_piece<kOutBf16>(c, s);
     if (rc != NF4S_OK) return rc;
   }
   const int64_t chunks = m * d / 4;
