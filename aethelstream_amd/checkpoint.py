@@ -20,8 +20,8 @@ import torch
 
 from . import _lib
 from .nf4 import _ptr, _require_cuda, _stream_ptr
-from .norm import EPS
 
+EPS = 1e-6   # of the norm (math.rs:45)
 BLOCK = 128  # elements of a row that share a scale
 
 
@@ -34,15 +34,17 @@ class Checkpoint8:
 
     def check(self) -> None:
         """Raises unless codes and scales belong together on one device."""
-        _require_cuda(self.codes, self.scales)
-        if self.codes.dtype != torch.int8 or self.scales.dtype != torch.float32:
+        c, s = self.codes, self.scales
+        if not (c.is_contiguous() and s.is_contiguous() and c.is_cuda):
+            _require_cuda(c, s)
+        if c.dtype is not torch.int8 or s.dtype is not torch.float32:
             raise ValueError("checkpoint codes must be int8 and scales float32")
-        if self.codes.dim() != 2 or self.codes.device != self.scales.device:
+        if c.dim() != 2 or c.device != s.device:
             raise ValueError("checkpoint codes must be [M, d], with scales on their device")
-        m, d = self.codes.shape
-        if list(self.scales.shape) != [m, (d + BLOCK - 1) // BLOCK]:
+        m, d = c.shape
+        if s.shape != (m, (d + BLOCK - 1) // BLOCK):
             raise ValueError(f"checkpoint scales must be [{m}, {(d + BLOCK - 1) // BLOCK}], got "
-                             f"{list(self.scales.shape)}")
+                             f"{list(s.shape)}")
 
 
 def encode(x: torch.Tensor, out: Optional[Checkpoint8] = None) -> Checkpoint8:
@@ -53,7 +55,7 @@ def encode(x: torch.Tensor, out: Optional[Checkpoint8] = None) -> Checkpoint8:
         raise ValueError("x must be a float32 or bfloat16 [M, d] tensor")
     m, d = int(x.shape[0]), int(x.shape[1])
     if out is None:
-        out = Checkpoint8(torch.empty(m, d, dtype=torch.int8, device=x.device),
+        out = Checkpoint8(torch.empty_like(x, dtype=torch.int8),
                           torch.empty(m, (d + BLOCK - 1) // BLOCK, dtype=torch.float32,
                                       device=x.device))
     else:
@@ -73,7 +75,7 @@ def decode(ckpt: Checkpoint8, dtype: torch.dtype = torch.float32,
     if out is None:
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("checkpoints decode to float32 or bfloat16")
-        out = torch.empty(ckpt.codes.shape, dtype=dtype, device=ckpt.codes.device)
+        out = torch.empty_like(ckpt.codes, dtype=dtype)
     _require_cuda(out)
     if out.dtype not in (torch.float32, torch.bfloat16) or out.shape != ckpt.codes.shape \
             or out.device != ckpt.codes.device:
@@ -96,8 +98,8 @@ def decode_norm(ckpt: Checkpoint8, w: torch.Tensor, eps: float = EPS, want_x: bo
     dev = ckpt.codes.device
     if w.dtype != torch.float32 or list(w.shape) != [d] or w.device != dev:
         raise ValueError(f"w must be float32 [{d}] on the checkpoint's device")
-    x = torch.empty(m, d, dtype=torch.float32, device=dev) if want_x else None
-    y = torch.empty(m, d, dtype=torch.bfloat16, device=dev)
+    x = torch.empty_like(ckpt.codes, dtype=torch.float32) if want_x else None
+    y = torch.empty_like(ckpt.codes, dtype=torch.bfloat16)
     rms = torch.empty(m, dtype=torch.float32, device=dev)
     _lib.check(_lib.load().nf4s_ckpt8_decode_norm(ckpt.codes.data_ptr(), ckpt.scales.data_ptr(),
                                                   w.data_ptr(), m, d, float(eps), _ptr(x),

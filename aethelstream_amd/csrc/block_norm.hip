@@ -28,9 +28,10 @@
 // memory.
 //
 // A thread holds up to 4 (8) chunks of four elements, a workgroup of up to 1024
-// threads a row.  Backward workgroups are persistent: workgroup b takes rows b,
-// b + G, ... and keeps its two column sums in registers, writes them once, and
-// a second kernel adds the G of them in order.
+// threads a row, or several short ones.  Workgroups are persistent, with the
+// next row on its way while one is worked on.  The backward's keep their column
+// sums in registers, join those of their rows through LDS and write them once;
+// a second kernel adds the workgroups' in order.
 #include "row_common.hpp"
 
 namespace nf4s {
@@ -40,70 +41,111 @@ struct BlockNormFwd {
   const float *res;
   const float *w_pre, *w_post, *gate;  // w_post, gate: NULL if absent
   float alpha, eps;
+  int64_t m;
   int32_t chunks;  // d / 4
   float *res_out;  // may be res
   uint16_t *y;
   float *rms_pre, *rms_post;
 };
 
-template <int kMaxThreads, int kChunks>
+// kKeep: rows of up to 4 chunks a thread; the weights stay in registers and the
+// next row is on its way while this one is normed.  Longer rows read the weights
+// again and load one row at a time.
+template <int kMaxThreads, int kChunks, bool kKeep>
 __global__ void __launch_bounds__(kMaxThreads) block_norm_fwd_kernel(const BlockNormFwd a) {
   __shared__ float part[2][16];
-  const int64_t base = (int64_t)blockIdx.x * a.chunks;
   const int threads = (int)blockDim.x;
-  const u32x2 *h = reinterpret_cast<const u32x2 *>(a.h) + base;
-  const floatx4 *res = reinterpret_cast<const floatx4 *>(a.res) + base;
+  const bool post = a.w_post != nullptr;
   const float inv_d = 1.0f / (float)(4 * a.chunks);
-  u32x2 hv[kChunks];
-  floatx4 r[kChunks];
+  const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto weight_k = [&](int c) {
+    floatx4 k = {a.alpha, a.alpha, a.alpha, a.alpha};
+    if (a.gate != nullptr) k *= reinterpret_cast<const floatx4 *>(a.gate)[c];
+    if (post) k *= reinterpret_cast<const floatx4 *>(a.w_post)[c];
+    return k;
+  };
+  floatx4 wp[kKeep ? kChunks : 1], wk[kKeep ? kChunks : 1];
+  if constexpr (kKeep) {
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int c = (int)threadIdx.x + i * threads;
-    hv[i] = (u32x2){0u, 0u};
-    r[i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < a.chunks) {
-      hv[i] = __builtin_nontemporal_load(h + c);
-      r[i] = __builtin_nontemporal_load(res + c);
+    for (int i = 0; i < kChunks; ++i) {
+      const int c = (int)threadIdx.x + i * threads;
+      wp[i] = wk[i] = zero;
+      if (c < a.chunks) {
+        wp[i] = reinterpret_cast<const floatx4 *>(a.w_pre)[c];
+        wk[i] = weight_k(c);
+      }
     }
   }
-  float scale = a.alpha;
-  if (a.w_post != nullptr) {
+  u32x2 hn[kChunks];
+  floatx4 rn[kChunks];
+  auto load = [&](int64_t row) {
+    const u32x2 *h = reinterpret_cast<const u32x2 *>(a.h) + row * a.chunks;
+    const floatx4 *res = reinterpret_cast<const floatx4 *>(a.res) + row * a.chunks;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int c = (int)threadIdx.x + i * threads;
+      hn[i] = (u32x2){0u, 0u};
+      rn[i] = zero;
+      if (c < a.chunks) {
+        hn[i] = __builtin_nontemporal_load(h + c);
+        rn[i] = __builtin_nontemporal_load(res + c);
+      }
+    }
+  };
+  if (kKeep && blockIdx.x < a.m) load(blockIdx.x);
+  int turn = 0;
+#pragma unroll 1
+  for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
+    const int64_t base = row * a.chunks;
+    if constexpr (!kKeep) load(row);
+    u32x2 hv[kChunks];
+    floatx4 r[kChunks];
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      hv[i] = hn[i];
+      r[i] = rn[i];
+    }
+    if (kKeep && row + gridDim.x < a.m) load(row + gridDim.x);
+    float scale = 1.0f;
+    if (post) {
+      float sum[1] = {0.0f};
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const floatx4 v = bf16x4_values(hv[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[0] += v[j] * v[j];
+      }
+      row_block_sum(sum, part[turn]);
+      turn ^= 1;
+      const float rms = __builtin_sqrtf(sum[0] * inv_d + a.eps);
+      if (threadIdx.x == 0) a.rms_post[row] = rms;
+      scale = 1.0f / rms;
+    }
     float sum[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const floatx4 v = bf16x4_values(hv[i]);
+      const int c = (int)threadIdx.x + i * threads;
+      if (c < a.chunks) {
+        const floatx4 k = kKeep ? wk[kKeep ? i : 0] : weight_k(c);
+        r[i] += bf16x4_values(hv[i]) * scale * k;
+        __builtin_nontemporal_store(r[i], reinterpret_cast<floatx4 *>(a.res_out) + base + c);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[0] += v[j] * v[j];
+        for (int j = 0; j < 4; ++j) sum[0] += r[i][j] * r[i][j];
+      }
     }
-    row_block_sum(sum, part[0]);
+    row_block_sum(sum, part[turn]);
+    turn ^= 1;
     const float rms = __builtin_sqrtf(sum[0] * inv_d + a.eps);
-    if (threadIdx.x == 0) a.rms_post[blockIdx.x] = rms;
-    scale /= rms;
-  }
-  float sum[1] = {0.0f};
+    if (threadIdx.x == 0) a.rms_pre[row] = rms;
+    const float inv = 1.0f / rms;
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int c = (int)threadIdx.x + i * threads;
-    if (c < a.chunks) {
-      floatx4 u = bf16x4_values(hv[i]) * scale;
-      if (a.w_post != nullptr) u *= reinterpret_cast<const floatx4 *>(a.w_post)[c];
-      if (a.gate != nullptr) u *= reinterpret_cast<const floatx4 *>(a.gate)[c];
-      r[i] += u;
-      __builtin_nontemporal_store(r[i], reinterpret_cast<floatx4 *>(a.res_out) + base + c);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum[0] += r[i][j] * r[i][j];
-    }
-  }
-  row_block_sum(sum, part[1]);
-  const float rms = __builtin_sqrtf(sum[0] * inv_d + a.eps);
-  if (threadIdx.x == 0) a.rms_pre[blockIdx.x] = rms;
-  const float inv = 1.0f / rms;
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int c = (int)threadIdx.x + i * threads;
-    if (c < a.chunks) {
-      const floatx4 o = r[i] * inv * reinterpret_cast<const floatx4 *>(a.w_pre)[c];
-      __builtin_nontemporal_store(bf16x4_pack(o), reinterpret_cast<u32x2 *>(a.y) + base + c);
+    for (int i = 0; i < kChunks; ++i) {
+      const int c = (int)threadIdx.x + i * threads;
+      if (c < a.chunks) {
+        const floatx4 w = kKeep ? wp[kKeep ? i : 0] : reinterpret_cast<const floatx4 *>(a.w_pre)[c];
+        const floatx4 o = r[i] * inv * w;
+        __builtin_nontemporal_store(bf16x4_pack(o), reinterpret_cast<u32x2 *>(a.y) + base + c);
+      }
     }
   }
 }
@@ -120,17 +162,39 @@ struct BlockNormBwd {
   float alpha;
   int64_t m;
   int32_t chunks, blocks;  // d / 4, checkpoint blocks a row
+  int32_t row_threads;     // threads of a row; a workgroup may have several rows
   float *dres_out;         // may be dres
   uint16_t *dh;
   float *part;  // [G][2][d] column sums: dy r^, g h^
 };
 
-// kKeep: the row's operands and the weights stay in registers between the sums
-// and the outputs.  Rows past 16384 elements read them again instead.
-template <int kMaxThreads, int kChunks, bool kH, bool kKeep>
+// What stays in registers between a row's sums and its outputs.
+enum {
+  kReload,  // nothing: both passes read the row and the weights
+  kRow,     // the row
+  kAhead,   // the row and the weights, with the next row on its way
+};
+
+// A row's operands, one chunk of four elements a thread.
+struct NormChunk {
+  floatx4 r;  // r', or its codes in r[0] and their scale in r[1]
+  floatx4 g;  // dr'
+  u32x2 dy, h;
+};
+
+// With f = 1 / rms_pre and q = 1 / rms_post the sums are taken over raw values,
+//   A = f sum e r,  B = q sum k h (dr' + f e),  C = f q sum k h r,
+// and the outputs from two factors a row: g = dr' + f e - (A / d) f^2 r and
+// dh = q k g - (E / d) q^2 h, E = B - (A / d) f C: 21 vector instructions an
+// element, which two waves a SIMD overlap with the memory.
+template <int kMaxThreads, int kChunks, bool kH, int kMode>
 __global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(const BlockNormBwd a) {
   __shared__ float part[2][48];
-  const int threads = (int)blockDim.x;
+  extern __shared__ floatx4 joined[];  // [2][chunks] where a workgroup has several rows
+  const int tid = (int)threadIdx.x % a.row_threads;
+  const int team = __builtin_amdgcn_readfirstlane((int)threadIdx.x / a.row_threads);
+  const int teams = (int)blockDim.x / a.row_threads;
+  const int threads = a.row_threads;
   const bool post = kH && a.w_post != nullptr;
   const float inv_d = 1.0f / (float)(4 * a.chunks);
   const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -142,97 +206,169 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(const Block
     if (a.w_post != nullptr) k *= reinterpret_cast<const floatx4 *>(a.w_post)[c];
     return k;
   };
-  floatx4 wp[kChunks], wk[kChunks], sum_pre[kChunks], sum_h[kChunks];
+  constexpr bool kWeights = kMode == kAhead;
+  floatx4 wp[kWeights ? kChunks : 1], wk[kWeights ? kChunks : 1];
+  floatx4 sum_pre[kChunks], sum_h[kChunks];
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    const int c = (int)threadIdx.x + i * threads;
+    const int c = tid + i * threads;
     sum_pre[i] = sum_h[i] = zero;
-    wp[i] = wk[i] = zero;
-    if (kKeep && c < a.chunks) {
-      wp[i] = weight_pre(c);
-      if (kH) wk[i] = weight_k(c);
+    if constexpr (kWeights) {
+      wp[i] = wk[i] = zero;
+      if (c < a.chunks) {
+        wp[i] = weight_pre(c);
+        if (kH) wk[i] = weight_k(c);
+      }
     }
   }
-
-  int turn = 0;
-#pragma unroll 1
-  for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
-    const int64_t base = row * a.chunks;
-    const float inv_pre = 1.0f / a.rms_pre[row];
-    const float inv_post = post ? 1.0f / a.rms_post[row] : 1.0f;
-    floatx4 r[kChunks], g[kChunks];
-    u32x2 dy[kChunks], h[kChunks];
-    auto load = [&](int i, int c) {
-      r[i] = g[i] = zero;
-      dy[i] = h[i] = (u32x2){0u, 0u};
-      if (c < a.chunks) {
-        if (a.res != nullptr)
-          r[i] = reinterpret_cast<const floatx4 *>(a.res)[base + c];
-        else
-          r[i] = ckpt_values(a.codes[base + c], a.scales[row * a.blocks + (c >> kCkptBlockShift)]);
-        if (a.dres != nullptr) g[i] = reinterpret_cast<const floatx4 *>(a.dres)[base + c];
-        dy[i] = reinterpret_cast<const u32x2 *>(a.dy)[base + c];
-        if (kH) h[i] = reinterpret_cast<const u32x2 *>(a.h)[base + c];
+  auto load = [&](int64_t row, int c) {
+    NormChunk v;
+    v.r = v.g = zero;
+    v.dy = v.h = (u32x2){0u, 0u};
+    if (row < a.m && c < a.chunks) {
+      const int64_t at = row * a.chunks + c;
+      if (a.res != nullptr) {
+        v.r = __builtin_nontemporal_load(reinterpret_cast<const floatx4 *>(a.res) + at);
+      } else {
+        v.r[0] = __builtin_bit_cast(float, a.codes[at]);
+        v.r[1] = a.scales[row * a.blocks + (c >> kCkptBlockShift)];
       }
-    };
-    if constexpr (kKeep) {
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i) load(i, (int)threadIdx.x + i * threads);
+      if (a.dres != nullptr)
+        v.g = __builtin_nontemporal_load(reinterpret_cast<const floatx4 *>(a.dres) + at);
+      v.dy = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(a.dy) + at);
+      if (kH) v.h = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(a.h) + at);
     }
+    return v;
+  };
+  auto residual = [&](const NormChunk &v) {
+    if (a.res != nullptr) return v.r;
+    const float codes = v.r[0];
+    return ckpt_values(__builtin_bit_cast(uint32_t, codes), v.r[1]);
+  };
+  auto fma4 = [](const floatx4 &x, const floatx4 &y, const floatx4 &z) {
+    return __builtin_elementwise_fma(x, y, z);
+  };
+  auto all = [](float v) { return (floatx4){v, v, v, v}; };
+
+  constexpr bool kHold = kMode != kReload;
+  constexpr int kHeld = kHold ? kChunks : 1;
+  auto load_row = [&](NormChunk (&v)[kHeld], int64_t row) {
+    if constexpr (kHold) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) v[i] = load(row, tid + i * threads);
+    }
+  };
+  auto work = [&](NormChunk (&v)[kHeld], int64_t row, float *sums) {
+    const bool here = row < a.m;
+    const float f = here ? 1.0f / a.rms_pre[row] : 0.0f;
+    const float q = here && post ? 1.0f / a.rms_post[row] : 1.0f;
     float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int c = (int)threadIdx.x + i * threads;
-      floatx4 p = wp[i], k = wk[i];
-      if constexpr (!kKeep) {
-        load(i, c);
-        p = c < a.chunks ? weight_pre(c) : zero;
-        if (kH) k = c < a.chunks ? weight_k(c) : zero;
-      }
-      const floatx4 rh = r[i] * inv_pre, e = bf16x4_values(dy[i]) * p;
+      const int c = tid + i * threads;
+      const bool in = c < a.chunks;
+      const NormChunk x = kHold ? v[kHold ? i : 0] : load(row, c);
+      const floatx4 p = kWeights ? wp[kWeights ? i : 0] : in ? weight_pre(c) : zero;
+      const floatx4 r = residual(x), e = bf16x4_values(x.dy) * p;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[0] += e[j] * rh[j];
+      for (int j = 0; j < 4; ++j) s[0] = __builtin_fmaf(e[j], r[j], s[0]);
       if (post) {
-        const floatx4 kh = bf16x4_values(h[i]) * inv_post * k;
-        const floatx4 b = g[i] + e * inv_pre;
+        const floatx4 k = kWeights ? wk[kWeights ? i : 0] : in ? weight_k(c) : zero;
+        const floatx4 kh = bf16x4_values(x.h) * k;
+        const floatx4 b = fma4(e, all(f), x.g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[1] += kh[j] * b[j];
-          s[2] += kh[j] * rh[j];
+          s[1] = __builtin_fmaf(kh[j], b[j], s[1]);
+          s[2] = __builtin_fmaf(kh[j], r[j], s[2]);
         }
       }
     }
-    row_block_sum(s, part[turn]);
-    turn ^= 1;
-    const float mean_pre = s[0] * inv_d;
-    const float mean_post = (s[1] - mean_pre * s[2] * inv_pre) * inv_d;
+    row_team_sum(s, sums, team, threads >> 6);
+    if constexpr (kHold) {
+      // Opaque: products and conversions of the first pass are made again rather
+      // than held.
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i)
+        asm volatile("" : "+v"(v[i].r), "+v"(v[i].dy), "+v"(v[i].h));
+    }
+    if (!here) return;
+    const float mean = s[0] * f * inv_d;                               // A / d
+    const float mean_post = (s[1] - mean * f * f * s[2]) * q * inv_d;  // E / d
+    const float cr = -mean * f * f, ch = -mean_post * q * q;
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int c = (int)threadIdx.x + i * threads;
-      floatx4 p = wp[i], k = wk[i];
-      if constexpr (!kKeep) {
-        load(i, c);
-        p = c < a.chunks ? weight_pre(c) : zero;
-        if (kH) k = c < a.chunks ? weight_k(c) : zero;
-      }
+      const int c = tid + i * threads;
       if (c >= a.chunks) continue;
-      const floatx4 rh = r[i] * inv_pre, v = bf16x4_values(dy[i]);
-      const floatx4 t = g[i] + (v * p - rh * mean_pre) * inv_pre;
-      sum_pre[i] += v * rh;
-      __builtin_nontemporal_store(t, reinterpret_cast<floatx4 *>(a.dres_out) + base + c);
+      const NormChunk x = kHold ? v[kHold ? i : 0] : load(row, c);
+      const floatx4 p = kWeights ? wp[kWeights ? i : 0] : weight_pre(c);
+      const floatx4 r = residual(x), dy = bf16x4_values(x.dy);
+      const floatx4 t = fma4(r, all(cr), fma4(dy * p, all(f), x.g));
+      sum_pre[i] = fma4(dy * f, r, sum_pre[i]);
+      const int64_t at = row * a.chunks + c;
+      __builtin_nontemporal_store(t, reinterpret_cast<floatx4 *>(a.dres_out) + at);
       if constexpr (kH) {
-        const floatx4 hh = bf16x4_values(h[i]) * inv_post;
-        sum_h[i] += t * hh;
+        const floatx4 k = kWeights ? wk[kWeights ? i : 0] : weight_k(c);
+        const floatx4 h = bf16x4_values(x.h);
+        sum_h[i] = fma4(t * q, h, sum_h[i]);
         floatx4 o = t * k;
-        if (post) o = (o - hh * mean_post) * inv_post;
-        __builtin_nontemporal_store(bf16x4_pack(o), reinterpret_cast<u32x2 *>(a.dh) + base + c);
+        if (post) o = fma4(h, all(ch), o * q);
+        __builtin_nontemporal_store(bf16x4_pack(o), reinterpret_cast<u32x2 *>(a.dh) + at);
+      }
+    }
+  };
+
+  // Every team of a workgroup takes as many rows, those past the last as zeros.
+  const int64_t stride = (int64_t)gridDim.x * teams;
+  int64_t row = (int64_t)blockIdx.x * teams;  // the first team's
+  NormChunk v0[kHeld], v1[kHeld];
+  if (kMode == kAhead) load_row(v0, row + team);
+#pragma unroll 1
+  for (; row < a.m; row += 2 * stride) {
+    if (kMode == kAhead)
+      load_row(v1, row + stride + team);
+    else
+      load_row(v0, row + team);
+    work(v0, row + team, part[0]);
+    if (row + stride >= a.m) break;
+    if (kMode == kAhead) {
+      load_row(v0, row + 2 * stride + team);
+      work(v1, row + stride + team, part[1]);
+    } else {
+      load_row(v0, row + stride + team);
+      work(v0, row + stride + team, part[1]);
+    }
+  }
+
+  // The other teams' sums into the first's, one after the other.
+  for (int t = 1; t < teams; ++t) {
+    __syncthreads();
+    if (team == t) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = tid + i * threads;
+        if (c < a.chunks) {
+          joined[c] = sum_pre[i];
+          if (kH) joined[a.chunks + c] = sum_h[i];
+        }
+      }
+    }
+    __syncthreads();
+    if (team == 0) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = tid + i * threads;
+        if (c < a.chunks) {
+          sum_pre[i] += joined[c];
+          if (kH) sum_h[i] += joined[a.chunks + c];
+        }
       }
     }
   }
+  if (team != 0) return;
   floatx4 *out = reinterpret_cast<floatx4 *>(a.part) + (int64_t)blockIdx.x * 2 * a.chunks;
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    const int c = (int)threadIdx.x + i * threads;
+    const int c = tid + i * threads;
     if (c < a.chunks) {
       out[c] = sum_pre[i];
       if (kH) out[a.chunks + c] = sum_h[i];
@@ -253,6 +389,7 @@ __global__ void __launch_bounds__(256) block_norm_columns_kernel(
   floatx4 s = {0.0f, 0.0f, 0.0f, 0.0f};
   if (c < chunks) {
     const floatx4 *p = reinterpret_cast<const floatx4 *>(part) + (int64_t)which * chunks + c;
+#pragma unroll 8
     for (int i = group; i < parts; i += 16) s += p[(int64_t)i * 2 * chunks];
   }
   lds[group][lane] = s;
@@ -277,6 +414,10 @@ __global__ void __launch_bounds__(256) block_norm_columns_kernel(
   }
 }
 
+// Waves of the persistent kernels on a CU.
+constexpr int kFwdWaves = 8, kBwdWaves = 16;
+constexpr int kBwdRows = 4;
+
 // Threads of a row of `chunks` chunks: four chunks a thread up to 1024 threads,
 // then eight.
 static int row_chunks_per_thread(int64_t chunks) { return chunks <= 4096 ? 4 : 8; }
@@ -285,12 +426,29 @@ static int row_threads(int64_t chunks) {
   return (int)(((chunks + per - 1) / per + 63) / 64 * 64);
 }
 
-// Workgroups of the backward: 16 waves a CU, and at least 4 rows each, as every
-// one writes two rows of column sums.
+// The backward holds more a thread: up to 8192 elements 2 chunks and the next
+// row (8192 rows of 8192: 219 us; 4 chunks on half as many threads 222, without
+// the next row 253), up to 12288 3 chunks (with the next row only without a
+// block, whose registers it takes; 4096 rows of 12288: 206 us, 427 with the next
+// row, 259 with 8 chunks), up to 16384 8 chunks on half as many threads, then 8
+// on 1024 and the row read twice.
+static int bwd_threads(int64_t chunks) {
+  const int64_t per = chunks <= 2048 ? 2 : (chunks <= 3072 ? 3 : 8);
+  return (int)(((chunks + per - 1) / per + 63) / 64 * 64);
+}
+
+// Rows of a backward workgroup side by side: up to 512 threads.
+static int bwd_teams(int64_t chunks) {
+  const int t = bwd_threads(chunks);
+  return t >= 512 ? 1 : 512 / t;
+}
+
+// Workgroups of the backward: as many as run at once (16 waves a CU), and at least 4 rows a team, as every one
+// writes two rows of column sums.
 static int64_t bwd_groups(int64_t m, int64_t d) {
-  const int64_t waves = row_threads(d / 4) / 64;
-  const int64_t most = (int64_t)cu_slots() * (waves >= 16 ? 1 : 16 / waves);
-  const int64_t rows = (m + 3) / 4;
+  const int64_t teams = bwd_teams(d / 4), waves = teams * (bwd_threads(d / 4) / 64);
+  const int64_t most = (int64_t)cu_slots() * (waves >= kBwdWaves ? 1 : kBwdWaves / waves);
+  const int64_t rows = (m + kBwdRows * teams - 1) / (kBwdRows * teams);
   return rows < most ? rows : most;
 }
 
@@ -330,13 +488,15 @@ int32_t nf4s_block_norm_fwd(const uint16_t *h, const float *res, const float *w_
       !aligned(rms_post, 4))
     return fail(NF4S_ERR_MISALIGNED,
                 "block norm: fp32 rows and weights must be 16-byte aligned, h and y 8-byte");
-  const BlockNormFwd a{h,   res, w_pre,   w_post, gate,    alpha,
-                       eps, (int32_t)(d / 4), res_out, y,      rms_pre, rms_post};
+  const BlockNormFwd a{h,   res, w_pre, w_post, gate, alpha, eps, m, (int32_t)(d / 4), res_out,
+                       y,   rms_pre, rms_post};
   const int threads = row_threads(d / 4);
-  auto *kernel = row_chunks_per_thread(d / 4) == 8 ? block_norm_fwd_kernel<1024, 8>
-                 : threads <= 512                  ? block_norm_fwd_kernel<512, 4>
-                                                   : block_norm_fwd_kernel<1024, 4>;
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)m), dim3(threads), 0, as_stream(stream), a);
+  auto *kernel = row_chunks_per_thread(d / 4) == 8 ? block_norm_fwd_kernel<1024, 8, false>
+                 : threads <= 512                  ? block_norm_fwd_kernel<512, 4, true>
+                                                   : block_norm_fwd_kernel<1024, 4, true>;
+  const int64_t most = (int64_t)cu_slots() * (threads >= 64 * kFwdWaves ? 1 : 64 * kFwdWaves / threads);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)(m < most ? m : most)), dim3(threads), 0,
+                     as_stream(stream), a);
   return check_launch("block_norm_fwd_kernel");
 }
 
@@ -412,20 +572,26 @@ int32_t nf4s_block_norm_bwd(const uint16_t *dy, const float *dres, const float *
                          m,
                          chunks,
                          (int32_t)((d + kCkptBlock - 1) / kCkptBlock),
+                         bwd_threads(chunks),
                          dres_out,
                          dh,
                          static_cast<float *>(workspace)};
-    const int threads = row_threads(chunks);
+    const int threads = bwd_threads(chunks);
     const bool blk = h != nullptr;
-    auto *kernel = blk ? block_norm_bwd_kernel<512, 4, true, true>
-                       : block_norm_bwd_kernel<512, 4, false, true>;
-    if (row_chunks_per_thread(chunks) == 8)
-      kernel = blk ? block_norm_bwd_kernel<1024, 8, true, false>
-                   : block_norm_bwd_kernel<1024, 8, false, false>;
-    else if (threads > 512)
-      kernel = blk ? block_norm_bwd_kernel<1024, 4, true, true>
-                   : block_norm_bwd_kernel<1024, 4, false, true>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)groups), dim3(threads), 0, s, a);
+    auto *kernel = blk ? block_norm_bwd_kernel<1024, 2, true, kAhead>
+                       : block_norm_bwd_kernel<1024, 2, false, kAhead>;
+    if (chunks > 4096)
+      kernel = blk ? block_norm_bwd_kernel<1024, 8, true, kReload>
+                   : block_norm_bwd_kernel<1024, 8, false, kReload>;
+    else if (chunks > 2048 && chunks <= 3072)
+      kernel = blk ? block_norm_bwd_kernel<1024, 3, true, kRow>
+                   : block_norm_bwd_kernel<1024, 3, false, kAhead>;
+    else if (chunks > 3072)
+      kernel = blk ? block_norm_bwd_kernel<512, 8, true, kRow>
+                   : block_norm_bwd_kernel<512, 8, false, kRow>;
+    const int teams = bwd_teams(chunks);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)groups), dim3(threads * teams),
+                       teams > 1 ? (uint32_t)(32 * chunks) : 0, s, a);
     const int32_t rc2 = check_launch("block_norm_bwd_kernel");
     if (rc2 != NF4S_OK) return rc2;
   }

@@ -63,6 +63,26 @@ __device__ __forceinline__ void row_block_sum(float (&v)[kN], float *part) {
   }
 }
 
+// kN sums over each team of `waves` waves of the workgroup, in every thread of
+// the team.  Every wave of the workgroup calls it.
+template <int kN>
+__device__ __forceinline__ void row_team_sum(float (&v)[kN], float *part, int team, int waves) {
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = row_wave_sum(v[i]);
+  if (waves == 1) return;
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) part[16 * i + (threadIdx.x >> 6)] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    float tot = 0.0f;
+    for (int w = 0; w < waves; ++w) tot += part[16 * i + team * waves + w];
+    v[i] = tot;
+  }
+}
+
 __device__ __forceinline__ float bf16_low(uint32_t v) {
   return __builtin_bit_cast(float, v << 16);
 }

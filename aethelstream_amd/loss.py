@@ -12,6 +12,7 @@ targets int64 [M]; losses and log-sum-exp are fp32.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -25,6 +26,11 @@ IGNORE_INDEX = -100
 
 def workspace_bytes(m: int, v: int, d: int, backward: bool) -> int:
     """Workspace of the forward, or of the gradients, for M tokens and a [V, d] head."""
+    return _workspace_bytes(m, v, d, backward, torch.cuda.current_device())
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(m: int, v: int, d: int, backward: bool, device: int) -> int:
     out = ctypes.c_int64(0)
     _lib.check(_lib.load().nf4s_linear_ce_workspace_size(m, v, d, int(backward),
                                                          ctypes.byref(out)))
@@ -55,8 +61,8 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     _check_head(x, w, targets)
     m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
     loss = torch.empty(m, dtype=torch.float32, device=x.device)
-    lse = torch.empty(m, dtype=torch.float32, device=x.device)
-    workspace = _workspace_for(workspace_bytes(m, v, d, False), workspace, x)
+    lse = torch.empty_like(loss)
+    workspace = _workspace_for(_workspace_bytes(m, v, d, False, x.get_device()), workspace, x)
     _lib.check(_lib.load().nf4s_linear_ce_fwd(
         x.data_ptr(), w.data_ptr(), targets.data_ptr(), m, v, d, ignore_index, loss.data_ptr(),
         lse.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
@@ -82,14 +88,14 @@ def linear_cross_entropy_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Te
     if dw is None:
         if accumulate:
             raise ValueError("accumulate needs an existing float32 dw")
-        dw = torch.empty(v, d, dtype=torch.bfloat16, device=x.device)
+        dw = torch.empty_like(w)
     if dw.dtype not in (torch.bfloat16, torch.float32) or list(dw.shape) != [v, d] \
             or dw.device != x.device:
         raise ValueError(f"dw must be bfloat16 or float32 [{v}, {d}] on x's device")
     if accumulate and dw.dtype != torch.float32:
         raise ValueError("accumulate needs a float32 dw")
-    dx = torch.empty(m, d, dtype=torch.bfloat16, device=x.device)
-    workspace = _workspace_for(workspace_bytes(m, v, d, True), workspace, x)
+    dx = torch.empty_like(x)
+    workspace = _workspace_for(_workspace_bytes(m, v, d, True, x.get_device()), workspace, x)
     _lib.check(_lib.load().nf4s_linear_ce_bwd(
         x.data_ptr(), w.data_ptr(), targets.data_ptr(), lse.data_ptr(), dloss.data_ptr(), m, v, d,
         ignore_index, dx.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32),

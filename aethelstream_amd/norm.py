@@ -14,12 +14,14 @@ Without a block ``block_norm_bwd`` is rms_norm_bwd (math.rs:61-88).
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
+from .checkpoint import Checkpoint8
 from .gemm import _workspace_for
 from .nf4 import _ptr, _require_cuda, _stream_ptr
 
@@ -78,14 +80,22 @@ class BlockNormGrad:
     dgate: Optional[torch.Tensor]     # float32 [d]
 
 
-def _check_rows(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape,
+def _check_rows(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape: tuple,
                 device: torch.device) -> None:
-    if t is None:
+    """Raises unless t is None or a contiguous tensor of that type, shape and device."""
+    if t is None or (t.dtype is dtype and t.shape == shape and t.device == device
+                     and t.is_contiguous()):
         return
     _require_cuda(t)
-    if t.dtype != dtype or list(t.shape) != list(shape) or t.device != device:
-        raise ValueError(f"{name} must be {str(dtype)[6:]} {list(shape)} on {device}, got "
-                         f"{str(t.dtype)[6:]} {list(t.shape)} on {t.device}")
+    raise ValueError(f"{name} must be {str(dtype)[6:]} {list(shape)} on {device}, got "
+                     f"{str(t.dtype)[6:]} {list(t.shape)} on {t.device}")
+
+
+@functools.lru_cache(maxsize=256)
+def _bwd_workspace_bytes(m: int, d: int, device: int) -> int:
+    size = ctypes.c_int64()
+    _lib.check(_lib.load().nf4s_block_norm_bwd_workspace_size(m, d, ctypes.byref(size)))
+    return size.value
 
 
 def block_norm_fwd(h: torch.Tensor, res: torch.Tensor, w_pre: torch.Tensor,
@@ -101,21 +111,22 @@ def block_norm_fwd(h: torch.Tensor, res: torch.Tensor, w_pre: torch.Tensor,
 
     in one pass.  w_pre, w_post and gate are fp32 [d].  The new residual goes to
     ``out`` if given, which may be ``res``."""
-    _require_cuda(h, res)
+    _require_cuda(h)
     if h.dim() != 2:
         raise ValueError(f"h must be [M, d], got {list(h.shape)}")
-    m, d = int(h.shape[0]), int(h.shape[1])
+    m, d = rows = h.shape
     dev = h.device
-    _check_rows(h, "h", torch.bfloat16, (m, d), dev)
-    _check_rows(res, "res", torch.float32, (m, d), dev)
+    _check_rows(h, "h", torch.bfloat16, rows, dev)
+    _check_rows(res, "res", torch.float32, rows, dev)
     for t, name in ((w_pre, "w_pre"), (w_post, "w_post"), (gate, "gate")):
         _check_rows(t, name, torch.float32, (d,), dev)
     if out is None:
-        out = torch.empty(m, d, dtype=torch.float32, device=dev)
-    _check_rows(out, "out", torch.float32, (m, d), dev)
-    y = torch.empty(m, d, dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(res)
+    else:
+        _check_rows(out, "out", torch.float32, rows, dev)
+    y = torch.empty_like(h)
     rms_pre = torch.empty(m, dtype=torch.float32, device=dev)
-    rms_post = None if w_post is None else torch.empty(m, dtype=torch.float32, device=dev)
+    rms_post = None if w_post is None else torch.empty_like(rms_pre)
     _lib.check(_lib.load().nf4s_block_norm_fwd(
         h.data_ptr(), res.data_ptr(), w_pre.data_ptr(), _ptr(w_post), _ptr(gate), float(alpha), m,
         d, float(eps), out.data_ptr(), y.data_ptr(), rms_pre.data_ptr(), _ptr(rms_post),
@@ -135,23 +146,22 @@ def block_norm_bwd(dy: torch.Tensor, dres: Optional[torch.Tensor], res, rms_pre:
     rms_pre the rms of what ``res`` stands for.  Without ``h`` there is no block:
     the RMSNorm backward of res.  The residual's gradient goes to ``out`` if
     given, which may be ``dres``."""
-    from .checkpoint import Checkpoint8
-    _require_cuda(dy, h, rms_post, w_post, gate)
+    _require_cuda(dy)
     if dy.dim() != 2:
         raise ValueError(f"dy must be [M, d], got {list(dy.shape)}")
-    m, d = int(dy.shape[0]), int(dy.shape[1])
+    m, d = rows = dy.shape
     dev = dy.device
-    _check_rows(dy, "dy", torch.bfloat16, (m, d), dev)
-    _check_rows(dres, "dres", torch.float32, (m, d), dev)
+    _check_rows(dy, "dy", torch.bfloat16, rows, dev)
+    _check_rows(dres, "dres", torch.float32, rows, dev)
     codes = scales = None
     if isinstance(res, Checkpoint8):
         res.check()
         codes, scales, res = res.codes, res.scales, None
-        if list(codes.shape) != [m, d] or codes.device != dev:
+        if codes.shape != rows or codes.device != dev:
             raise ValueError(f"the checkpoint must be [{m}, {d}] on dy's device")
     elif res is None:
         raise ValueError("res must be a float32 tensor or a Checkpoint8")
-    _check_rows(res, "res", torch.float32, (m, d), dev)
+    _check_rows(res, "res", torch.float32, rows, dev)
     _check_rows(rms_pre, "rms_pre", torch.float32, (m,), dev)
     for t, name in ((w_pre, "w_pre"), (w_post, "w_post"), (gate, "gate")):
         _check_rows(t, name, torch.float32, (d,), dev)
@@ -159,22 +169,18 @@ def block_norm_bwd(dy: torch.Tensor, dres: Optional[torch.Tensor], res, rms_pre:
         raise ValueError("w_post and gate need h")
     if w_post is not None and rms_post is None:
         raise ValueError("w_post needs rms_post")
-    _check_rows(h, "h", torch.bfloat16, (m, d), dev)
+    _check_rows(h, "h", torch.bfloat16, rows, dev)
     _check_rows(rms_post, "rms_post", torch.float32, (m,), dev)
     if out is None:
         out = torch.empty(m, d, dtype=torch.float32, device=dev)
-    _check_rows(out, "out", torch.float32, (m, d), dev)
-
-    def column_sum(of):
-        return None if of is None else torch.empty(d, dtype=torch.float32, device=dev)
-
-    dh = None if h is None else torch.empty(m, d, dtype=torch.bfloat16, device=dev)
-    dw_pre, dw_post, dgate = column_sum(w_pre), column_sum(w_post), column_sum(gate)
-    lib = _lib.load()
-    size = ctypes.c_int64()
-    _lib.check(lib.nf4s_block_norm_bwd_workspace_size(m, d, ctypes.byref(size)))
-    workspace = _workspace_for(size.value, workspace, dy)
-    _lib.check(lib.nf4s_block_norm_bwd(
+    else:
+        _check_rows(out, "out", torch.float32, rows, dev)
+    dh = None if h is None else torch.empty_like(h)
+    dw_pre = torch.empty_like(w_pre)
+    dw_post = None if w_post is None else torch.empty_like(w_post)
+    dgate = None if gate is None else torch.empty_like(gate)
+    workspace = _workspace_for(_bwd_workspace_bytes(m, d, dev.index), workspace, dy)
+    _lib.check(_lib.load().nf4s_block_norm_bwd(
         dy.data_ptr(), _ptr(dres), _ptr(res), _ptr(codes), _ptr(scales), rms_pre.data_ptr(),
         w_pre.data_ptr(), _ptr(h), _ptr(rms_post), _ptr(w_post), _ptr(gate), float(alpha), m, d,
         out.data_ptr(), _ptr(dh), dw_pre.data_ptr(), _ptr(dw_post), _ptr(dgate),
