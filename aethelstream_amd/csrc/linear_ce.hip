@@ -459,9 +459,6 @@ static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
     return fail(NF4S_ERR_UNSUPPORTED_SHAPE,
                 "cross entropy of m=%lld v=%lld d=%lld beyond m 2^24, v 2^28, d 2^20",
                 (long long)m, (long long)v, (long long)d);
-  if (ceil_to(m, 64) * ceil_to(v, 128) > kMaxTiles ||
-      ceil_to(v, 128) * ceil_to(d, 128) > kMaxTiles || ceil_to(m, 64) * ceil_to(d, 256) > kMaxTiles)
-    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many tiles");
   p.tokens = m < kCeTokens ? m : kCeTokens;
   p.part_bytes = m > 0 ? ce_slices(p.tokens, v, d) * p.tokens : 0;
   if (m > 0 && m % p.tokens != 0) {
@@ -476,6 +473,13 @@ static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
   p.piece = up((v + pieces - 1) / pieces, 256);
   if (p.piece > v) p.piece = v;
   p.ldg = up(p.piece, 64);
+  // Tiles of the forward, of a piece's logits and dw, and of dx, at the smallest
+  // tiles of each.
+  if (ceil_to(p.tokens, 64) * ceil_to(v, 128) > kMaxTiles ||
+      ceil_to(m, 64) * ceil_to(p.piece, 128) > kMaxTiles ||
+      ceil_to(p.piece, 128) * ceil_to(d, 128) > kMaxTiles ||
+      ceil_to(m, 64) * ceil_to(d, 256) > kMaxTiles)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "too many tiles");
   ce_dx_plan(m, v, d, p);
   p.g_bytes = up(m * p.ldg * 2, 256);
   p.bwd_bytes = p.g_bytes + p.slices * m * d * 4 + 16;  // G, dx's sums, c

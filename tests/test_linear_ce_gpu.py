@@ -79,7 +79,7 @@ def _check_backward(x, w, t, dl, lse, dx, dw, accumulated=None):
 
 SHAPES = [(1, 1, 8), (1, 5, 64), (1, 1000, 72), (3, 257, 128), (17, 3001, 520), (64, 512, 256),
           (65, 129, 1000), (100, 4099, 192), (128, 640, 64), (129, 1023, 320), (257, 513, 136),
-          (300, 2000, 1032), (600, 777, 2048)]
+          (300, 2000, 1032), (600, 777, 2048), (1000, 17000, 2048), (1500, 9001, 520)]
 
 
 @pytest.mark.parametrize("m,v,d", SHAPES)
