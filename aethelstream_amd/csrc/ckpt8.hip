@@ -11,7 +11,11 @@
 // own.  A block that holds an infinity or a NaN has a NaN scale and so reads
 // back as NaN throughout: it is not hidden.
 //
-// All kernels are bound by memory.
+// All kernels are bound by memory.  Measured at 8192 x 8192: fp32 encode 52 us
+// (6.4 TB/s; 60 with one unit a lane, 53 with four), decode 47 (7.1); bf16
+// encode 33 (6.1; 45 in units of 4 elements, where the vector instructions of
+// maximum, reciprocal and codes set the time), decode 29 (6.9); decode and norm
+// 68 (6.9).  Past the Infinity Cache (16384 x 8192) the last writes at 4.6.
 #include <type_traits>
 
 #include "row_common.hpp"

@@ -21,9 +21,17 @@
 // fits kCePieceBytes.  The common factor c stays out of G: the tokens of a mean
 // all have dloss = c, whose rounding error would be that of every target's
 // entry (up to 2^-8 at once); divided by c those entries are close to -1.  Per
-// piece: logits again, turned into G in the epilogue;
-// dx += G . w in fp32; the piece's rows of dw.  The four products of a training
-// step are matrix-rate bound, the forward of few tokens reads w at memory rate.
+// piece: logits again, turned into G in the epilogue; dx += G . w in fp32; the
+// piece's rows of dw.
+//
+// Measured at 4096 tokens, 128000 x 8192: forward 6.2 ms (1377 TFLOP/s), a piece
+// of 32000 columns 1643 us for G (1307), 1585 for dx (1354), 1581 for dw (1358);
+// hipBLASLt's products of these shapes run at 1490, 1328 and 1147.  The matrix
+// pipe is busy 77-79 % of the cycles, at a clock that has fallen to 1.62-1.75
+// GHz: the products are bound by power (an order of loads that hid the first
+// loads of each tile behind the previous epilogue changed nothing).  Few tokens
+// read w once for each product and write dw: one token over 128000 x 8192,
+// gradients 1127 us (5.6 TB/s), forward 363 us (5.8).
 #include <cmath>
 
 #include "bf16_gemm_core.hpp"
@@ -418,7 +426,7 @@ struct CePlan {
 // on average, 6 % at most.  The gradients of 777 x 32000 x 4096: 659 us with 14
 // tiles of 128 rows x 2 slices, 663 with 256 rows x 4, 995 with 256 rows in one.
 constexpr CeTile kCeDxTiles[3] = {{1, 4, 2, 0.75, 0.97, 5.0}, {2, 4, 1, 0.61, 0.88, 5.0},
-                                  {4, 4, 1, 0.95, 1.03, 6.0}};
+                                  {4, 4, 1, 0.95, 1.03, 5.0}};
 static void ce_dx_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
   const double pieces = (double)ceil_to(v, p.piece);
   const int64_t steps = ceil_to(p.ldg, kGcStep);
