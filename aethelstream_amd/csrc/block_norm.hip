@@ -447,8 +447,8 @@ static int bwd_teams(int64_t chunks) {
   return t >= 512 ? 1 : 512 / t;
 }
 
-// Workgroups of the backward: as many as run at once (16 waves a CU), and at least 4 rows a team, as every one
-// writes two rows of column sums.
+// Workgroups of the backward: as many as run at once (16 waves a CU), and at
+// least 4 rows a team, as every one writes two rows of column sums.
 static int64_t bwd_groups(int64_t m, int64_t d) {
   const int64_t teams = bwd_teams(d / 4), waves = teams * (bwd_threads(d / 4) / 64);
   const int64_t most = (int64_t)cu_slots() * (waves >= kBwdWaves ? 1 : kBwdWaves / waves);
@@ -498,7 +498,8 @@ int32_t nf4s_block_norm_fwd(const uint16_t *h, const float *res, const float *w_
   auto *kernel = row_chunks_per_thread(d / 4) == 8 ? block_norm_fwd_kernel<1024, 8, false>
                  : threads <= 512                  ? block_norm_fwd_kernel<512, 4, true>
                                                    : block_norm_fwd_kernel<1024, 4, true>;
-  const int64_t most = (int64_t)cu_slots() * (threads >= 64 * kFwdWaves ? 1 : 64 * kFwdWaves / threads);
+  const int wgs = threads >= 64 * kFwdWaves ? 1 : 64 * kFwdWaves / threads;
+  const int64_t most = (int64_t)cu_slots() * wgs;
   hipLaunchKernelGGL(kernel, dim3((uint32_t)(m < most ? m : most)), dim3(threads), 0,
                      as_stream(stream), a);
   return check_launch("block_norm_fwd_kernel");

@@ -26,7 +26,7 @@
 //
 // Measured at 4096 tokens, 128000 x 8192: forward 6.2 ms (1377 TFLOP/s), a piece
 // of 32000 columns 1643 us for G (1307), 1585 for dx (1354), 1581 for dw (1358);
-// hipBLASLt's products of these shapes run at 1490, 1328 and 1147.  The matrix
+// library products of these shapes run at 1490, 1328 and 1147.  The matrix
 // pipe is busy 77-79 % of the cycles, at a clock that has fallen to 1.62-1.75
 // GHz: the products are bound by power (an order of loads that hid the first
 // loads of each tile behind the previous epilogue changed nothing).  Few tokens
@@ -42,7 +42,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // G of a piece: what the Infinity Cache (256 MB) holds between the kernel that
-// writes it and the two that read it.
+// writes it and the two that read it.  Gradients of 8192 x 32000 x 4096: 4975 us
+// with 256 MB, 5185 with half, 4902 with four times as much.
 constexpr int64_t kCePieceBytes = (int64_t)256 << 20;
 // Tokens of one forward launch, which bounds its partial sums.
 constexpr int64_t kCeTokens = 16384;
@@ -268,12 +269,13 @@ __global__ void __launch_bounds__(kGcThreads, kMT * kNT == 4 ? 2 : 1) ce_product
     const int64_t row = l0 + row0 + 32 * mt;
     const int64_t at = slice * a.slice_stride + row * a.ld + c0;
     if constexpr (kOut == kOutBf16)
-      gc_store_bf16<kNT, true>(value, lds + 2048 * kNT * wave, static_cast<uint16_t *>(a.out) + at, a.ld,
-                       a.rows - row, a.cols - c0, lane);
+      gc_store_bf16<kNT, true>(value, lds + 2048 * kNT * wave,
+                               static_cast<uint16_t *>(a.out) + at, a.ld, a.rows - row,
+                               a.cols - c0, lane);
     else
-      gc_store_f32<kNT, kOut == kOutF32Add, kLAcross>(value, lds + 4096 * kNT * wave,
-                                          static_cast<float *>(a.out) + at, a.ld, a.rows - row,
-                                          a.cols - c0, lane);
+      gc_store_f32<kNT, kOut == kOutF32Add, kLAcross>(
+          value, lds + 4096 * kNT * wave, static_cast<float *>(a.out) + at, a.ld, a.rows - row,
+          a.cols - c0, lane);
   }
 }
 
@@ -332,16 +334,17 @@ struct CeLaunch {
   int64_t cols;
 };
 
-// The tiles of m > 0 tokens by v > 0 columns of length d, as one launch, or as whole
-// rounds of large tiles and the rest in smaller ones.  Cost of a launch in us:
-// each round takes, per step of 64, `lo` when few tiles run to `hi` when the
+// The tiles of m > 0 tokens by v > 0 columns of length d, as one launch, or as
+// whole rounds of large tiles and the rest in smaller ones.  Cost of a launch in
+// us: each round takes, per step of 64, `lo` when few tiles run to `hi` when the
 // chip is full (less traffic and a higher clock when it is not); w is read at
 // `tbs`, again by part for each further row of tiles; 8 us beside, 14 for a
-// second launch.  Fitted to forwards of 1 to 1500 tokens over 1000 to 128000 columns, d = 1024 to 8192
-// (times in us at d = 4096 with 64 x 128, 128 x 256 and 256 x 256 tiles):
+// second launch.  Fitted to forwards of 1 to 1500 tokens over 1000 to 128000
+// columns, d = 1024 to 8192 (times in us at d = 4096 with 64 x 128, 128 x 256
+// and 256 x 256 tiles):
 //   1 token, 32000 columns 45, 52, 81;  128 tokens 65, 62, 89;
 //   256 tokens 97, 70, 96;  512 tokens 163, 126, 114;
-//   1000 tokens, 50021 columns 556, 409, 398.
+//   1000 tokens, 50021 columns 556, 409, 398 (three rounds and the rest 351).
 // 128 x 128 and 128 x 64 tiles were within 3 % of the best of the three at
 // most, and are not built.
 struct CeTile {
