@@ -420,7 +420,6 @@ __global__ void __launch_bounds__(256) block_norm_columns_kernel(
 
 // Waves of the persistent kernels on a CU.
 constexpr int kFwdWaves = 8, kBwdWaves = 16;
-constexpr int kBwdRows = 4;
 
 // Threads of a row of `chunks` chunks: four chunks a thread up to 1024 threads,
 // then eight.
@@ -447,13 +446,17 @@ static int bwd_teams(int64_t chunks) {
   return t >= 512 ? 1 : 512 / t;
 }
 
-// Workgroups of the backward: as many as run at once (16 waves a CU), and at
-// least 4 rows a team, as every one writes two rows of column sums.
+// Workgroups of the backward: at most as many as run at once (16 waves a CU).
+// Every one writes two rows of column sums, so one row a team only up to one
+// workgroup a CU, then two (64 rows of 4096: 9.5 us with one row a team, 13.1
+// with four; 512 rows: 16.0 us with two, 21.3 with one).
 static int64_t bwd_groups(int64_t m, int64_t d) {
   const int64_t teams = bwd_teams(d / 4), waves = teams * (bwd_threads(d / 4) / 64);
-  const int64_t most = (int64_t)cu_slots() * (waves >= kBwdWaves ? 1 : kBwdWaves / waves);
-  const int64_t rows = (m + kBwdRows * teams - 1) / (kBwdRows * teams);
-  return rows < most ? rows : most;
+  const int64_t cus = cu_slots();
+  const int64_t most = cus * (waves >= kBwdWaves ? 1 : kBwdWaves / waves);
+  const int64_t one = (m + teams - 1) / teams, two = (m + 2 * teams - 1) / (2 * teams);
+  const int64_t n = one < cus ? one : (two > cus ? two : cus);
+  return n < most ? n : most;
 }
 
 static int32_t row_shape(int64_t m, int64_t d) {
