@@ -1,12 +1,11 @@
 // block_norm.hip - the norms around a block with its gate and residual scale,
 // forward and backward, for gfx950 (MI355X).
 //
-// Between two blocks of a decoder layer the reference adds the block's output
-// to the residual and norms the sum for the next block
-// (doublepass/src/forward.rs:246-249; rms_norm_fwd and rms_norm_bwd,
-// doublepass/src/math.rs:28-88).  Here that boundary is one kernel, with an
-// optional norm of the block's output, an optional gate per channel and a
-// residual scale:
+// Between two blocks of a decoder layer the reference adds the block's output to
+// the residual and norms the sum for the next block (rms_norm_fwd,
+// doublepass/src/math.rs:28-59, at doublepass/src/forward.rs:173 and :249).  Here
+// that boundary is one kernel, with an optional norm of the block's output, an
+// optional gate per channel and a residual scale:
 //   h^ = h / rms(h),  u = w_post h^          (or h^ = u = h without w_post)
 //   r' = r + alpha gate u                    (gate 1 without one)
 //   y  = w_pre r' / rms(r'),  rms(v) = sqrt(mean(v^2) + eps)

@@ -27,7 +27,7 @@
 // Measured at 4096 tokens, 128000 x 8192: forward 6.2 ms (1377 TFLOP/s), a piece
 // of 32000 columns 1643 us for G (1307), 1585 for dx (1354), 1581 for dw (1358);
 // library products of these shapes run at 1490, 1328 and 1147.  The matrix
-// pipe is busy 77-79 % of the cycles, at a clock that has fallen to 1.62-1.75
+// pipe is busy 70-79 % of the cycles, at a clock that has fallen to 1.62-1.77
 // GHz: the products are bound by power (an order of loads that hid the first
 // loads of each tile behind the previous epilogue changed nothing).  Few tokens
 // read w once for each product and write dw: one token over 128000 x 8192,

@@ -8,8 +8,8 @@ rms as fp32 (x_hat = x / rms is recomputed where the backward needs it).
 
 ``block_norm_fwd`` / ``block_norm_bwd`` are the whole boundary between two
 blocks: an optional norm of the block's output, a gate per channel and a
-residual scale, the residual add (forward.rs:246-248) and the next block's norm.
-Without a block ``block_norm_bwd`` is rms_norm_bwd (math.rs:61-88).
+residual scale, the residual add and the next block's norm (forward.rs:249).
+Without a block ``block_norm_bwd`` is the backward of rms_norm_fwd.
 """
 from __future__ import annotations
 

@@ -350,8 +350,8 @@ int32_t nf4s_rmsnorm_fwd(const float *x, const float *w, int64_t m, int64_t d, f
  *   y = bf16(w_pre * res_out / rms_pre),  rms = sqrt(mean of squares + eps)
  * h and y are bf16 [m, d], res and res_out fp32 [m, d], the weights and the
  * gate fp32 [d], rms_pre and rms_post (set iff w_post is) fp32 [m].  res_out may
- * be res.  Replaces the residual add and the next rms_norm_fwd of
- * single_layer_forward (doublepass/src/forward.rs:246-249).
+ * be res.  Takes the place of the residual add and the rms_norm_fwd after it in
+ * single_layer_forward (doublepass/src/forward.rs:249).
  * Requires d % 4 == 0, d <= 32768, fp32 buffers of rows and weights 16-byte
  * aligned, bf16 ones 8-byte.
  */
@@ -366,8 +366,8 @@ int32_t nf4s_block_norm_fwd(const uint16_t *h, const float *res, const float *w_
  * its 8-bit checkpoint (res_codes, res_scales: nf4s_ckpt8_encode), exactly one
  * of them.  Writes dres_out = the gradient of res (fp32, may be dres), dh (bf16,
  * set iff h is), and the column sums dw_pre, dw_post (set iff w_post is) and
- * dgate (set iff gate is), all fp32 [d], zero when m = 0.  h = NULL is the plain
- * RMSNorm backward (rms_norm_bwd, doublepass/src/math.rs:61-88), without w_post
+ * dgate (set iff gate is), all fp32 [d], zero when m = 0.  h = NULL is the
+ * backward of the plain RMSNorm (doublepass/src/math.rs:28-59), without w_post
  * and gate.  The workspace holds the column sums of the launch's workgroups,
  * which a second kernel adds in order: results do not depend on timing.
  */
