@@ -7,20 +7,22 @@
 //   dW      P^T . X   both across
 //
 // Workgroup = 4 waves in 2 x 2, tile = 64 kMT rows (l) x 64 kNT columns (r);
-// each wave owns 32 kMT x 32 kNT in kMT x kNT accumulators of
-// v_mfma_f32_32x32x16_bf16, R as the instruction's first operand: a lane holds
-// one row l of the output and groups of four adjacent columns.
+// each wave owns 32 kMT x 32 kNT in 2 kMT x 2 kNT accumulators of
+// v_mfma_f32_16x16x32_bf16, R as the instruction's first operand: a lane holds
+// one row l of each accumulator and four adjacent columns.  (These products are
+// bound by power, and 32x32x16 takes more: from registers alone random operands
+// sustain 2.05 PFLOP/s with 16x16x32 and 1.81 with 32x32x16, with the LDS reads
+// of 128 x 128 a wave 1.71 and 1.63.)
 // Per 64-long step both operands' tiles move into LDS with direct-to-LDS loads,
 // into rings of kNL and kNR stages: while step t computes, L of step t + kNL - 1
-// and R of step t + kNR - 1 are on their way.  An operand along the reduction is read with
-// ds_read_b128, 8 consecutive k of one row a lane; one across it with the
-// transposing reads of tr_tile.hpp.
+// and R of step t + kNR - 1 are on their way.  An operand along the reduction is
+// read with ds_read_b128, 8 consecutive k of one row a lane; one across it with
+// the transposing ds_read_b64_tr_b16.
 #pragma once
 
 #include "abi_common.hpp"
 #include "gemm_common.hpp"
 #include "nf4_device.hpp"
-#include "tr_tile.hpp"
 
 namespace nf4s {
 
@@ -52,32 +54,64 @@ __device__ __forceinline__ GcOperand gc_across(const uint16_t *p, int64_t ld, in
 // multiple of 16 over all 64.
 __device__ __forceinline__ int gc_swz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
+// Fragment (8 k of one column) of an operand across the reduction, whose rows are
+// kUnits 16-byte units long.
+template <int kUnits>
+__device__ __forceinline__ u32x4 gc_tr_frag(const char *base, uint32_t off) {
+  typedef __attribute__((address_space(3))) char lds_char_t;
+  typedef __attribute__((address_space(3))) v4i16 lds_v4i16_t;
+  lds_char_t *p = (lds_char_t *)const_cast<char *>(base) + off;
+  const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t *)p);
+  const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t *)(p + 64 * kUnits));
+  const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+  return (u32x4){l2.x, l2.y, h2.x, h2.y};
+}
+
+// LDS tile of an operand across it: k rows of kUnits (32 or 16) units.  Unit u
+// of row r lives at physical unit (u & 16) | ((u & 15) ^ s(r)): each 32-lane half
+// of a transposed fragment read, 8 rows of 2 units each, covers 16 distinct units
+// of one half-row's 64 banks, and each 16-lane quarter of a DMA writes one row's
+// 16 contiguous units.
+__device__ __forceinline__ int gc_unit(int row, int u) {
+  return (u & 16) | ((u & 15) ^ (5 * (row & 3)) ^ (2 * ((row >> 3) & 1)));
+}
+
 template <int kTiles, bool kAcross>
 struct GcSide {
   static constexpr int kBytes = 8192 * kTiles;   // of one stage
   static constexpr int kUnits = 8 * kTiles;      // across: units of a k row
   static constexpr int kDmas = 2 * kTiles;       // per wave and step
-  static constexpr int kAddrs = kAcross ? kTiles : 4;
+  static constexpr int kFrags = 2 * kTiles;      // of 16 rows, per wave and sub-step
+  static constexpr int kAddrs = kAcross ? 1 : 2;
+  static_assert(!kAcross || kUnits >= 16, "gc_unit");
 
-  // Lane addresses of the fragment reads: across one per fragment, along one per
-  // sub-step of 16 (fragments are 32 rows = 4096 bytes apart).
+  // Lane addresses of the fragment reads: lane l reads row (along) or column
+  // (across) l % 16 of its fragment, k = 8 (l / 16) + 0..7 of the sub-step of 32.
+  // Across (transposing reads): lane 4e + c of a 16-lane group addresses k row e,
+  // columns 4c..4c+3, and receives the four rows of column l % 16; a second read
+  // 4 rows lower completes the 8.  Fragment j, 2 units further on, is 32 j away in
+  // bits 5 to 7, which nothing but the unit sets (a row is a multiple of 256
+  // bytes, a stage of 8192).  Along one address per sub-step, fragments are 16
+  // rows = 2048 bytes apart.
   static __device__ __forceinline__ void read_addrs(uint32_t (&a)[kAddrs], int lane, int half) {
     if constexpr (kAcross) {
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) a[j] = wg_read_off<kUnits>(lane, half, j);
+      const int l16 = lane & 15;
+      const int row = 8 * (lane >> 4) + (l16 >> 2);
+      const int u = kUnits / 2 * half + ((l16 >> 1) & 1);
+      a[0] = (uint32_t)(16 * (kUnits * row + gc_unit(row, u)) + 8 * (l16 & 1));
     } else {
-      const int row = 32 * kTiles * half + (lane & 31);
+      const int row = 32 * kTiles * half + (lane & 15);
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-        a[s] = (uint32_t)(128 * row + 16 * ((2 * s + (lane >> 5)) ^ gc_swz(row)));
+      for (int s = 0; s < 2; ++s)
+        a[s] = (uint32_t)(128 * row + 16 * ((4 * s + (lane >> 4)) ^ gc_swz(row)));
     }
   }
   static __device__ __forceinline__ u32x4 frag(const char *base, const uint32_t (&a)[kAddrs],
                                                int s, int j) {
     if constexpr (kAcross)
-      return wg_frag<kUnits>(base, a[j], s);
+      return gc_tr_frag<kUnits>(base, (a[0] ^ (32 * j)) + 512 * kUnits * s);
     else
-      return *reinterpret_cast<const u32x4 *>(base + a[s] + 4096 * j);
+      return *reinterpret_cast<const u32x4 *>(base + a[s] + 2048 * j);
   }
 
   // Byte offsets of this wave's DMAs from the operand's place at a step.
@@ -88,7 +122,7 @@ struct GcSide {
       if constexpr (kAcross) {
         constexpr int kRows = 64 / kUnits;  // k rows per instruction
         const int r = 16 * wave + kRows * q + lane / kUnits;
-        v[q] = (uint32_t)(r * ld * 2 + 16 * wg_unit(r, lane % kUnits));
+        v[q] = (uint32_t)(r * ld * 2 + 16 * gc_unit(r, lane % kUnits));
       } else {
         const int r = 8 * (kDmas * wave + q) + (lane >> 3);
         v[q] = (uint32_t)(r * ld * 2 + 16 * ((lane & 7) ^ gc_swz(r)));
@@ -149,20 +183,30 @@ struct GcCore {
   static constexpr int kInFlight = kNR == 3 ? LSide::kDmas + RSide::kDmas
                                             : (kNL == 3 ? LSide::kDmas : 0);
   static constexpr int kLdsBytes = kNL * LSide::kBytes + kNR * RSide::kBytes;
-  static constexpr int kSub = kMT * kNT;       // MFMAs per sub-step
-  static constexpr int kPost = kSub / 2;       // those that open the next step
-  static constexpr int kFront = 4 * kSub - kPost;
-  static constexpr int kReads = kMT + kNT;
+  static constexpr int kFL = LSide::kFrags, kFR = RSide::kFrags;
+  static constexpr int kSub = kFL * kFR;       // MFMAs per sub-step of 32
+  static constexpr int kPost = 3 * kSub / 8;   // those that open the next step
+  static constexpr int kFront = 2 * kSub - kPost;
+  static constexpr int kReads = kFL + kFR;
+  // From 128 accumulator registers on, the instruction is written out with the
+  // sum's registers as its own source.  Left to the compiler the sums move: from
+  // 50 to 200 copies a step of 128 MFMAs, and 4096 x 32000 x 8192 logits took 1970 us
+  // (1535 tied).  The compiler does not know that the block is an MFMA, so the
+  // waits that it would add are this file's: the fragments come from LDS reads,
+  // which it waits for, never from an instruction of the two before; the sums
+  // stay where they are until run() has waited for the last of them.
+  // (Checked in the listing by test_loss_listing.py.)
+  static constexpr bool kTied = kSub >= 32;
   static constexpr int kDmas = LSide::kDmas + RSide::kDmas;
-  // MFMAs from one DMA to the next.  Reads and DMAs together keep LDS busy for
-  // three quarters of a 256 x 256 step at the MFMA rate: spread over the step
-  // (3) they ran 4096 x 32000 x 8192 logits at 1294 TFLOP/s, every 2 MFMAs
-  // 1259, every one 1156.
+  // MFMAs from one DMA to the next: spread over what follows the opening, as the
+  // reads and the DMAs together keep LDS busy for three quarters of a 256 x 256
+  // step at the MFMA rate.  4096 x 32000 x 8192 logits: 1535 us, with a gap of 4
+  // and the opening a half 1587.
   static constexpr int kGap = (kFront - 1) / kDmas;
   static_assert(kDmas <= kFront, "one DMA per MFMA slot at most");
 
-  floatx16 acc[kMT][kNT];
-  u32x4 fl[2][kMT], fr[2][kNT];
+  floatx4 acc[kFL][kFR];
+  u32x4 fl[2][kFL], fr[2][kFR];
   uint32_t al[LSide::kAddrs], ar[RSide::kAddrs];
   uint32_t vl[LSide::kDmas], vr[RSide::kDmas];
   GcPlace pl, pr;
@@ -170,8 +214,8 @@ struct GcCore {
   // Fragment read q of a sub-step, in the order its MFMAs use them: l0, r0, r1,
   // .., l1, ..
   __device__ __forceinline__ void read(const char *lds, int s, int b, int q) {
-    if (q == 0 || q > kNT) {
-      const int j = q == 0 ? 0 : q - kNT;
+    if (q == 0 || q > kFR) {
+      const int j = q == 0 ? 0 : q - kFR;
       fl[b][j] = LSide::frag(lds, al, s, j);
     } else {
       fr[b][q - 1] = RSide::frag(lds, ar, s, q - 1);
@@ -179,10 +223,15 @@ struct GcCore {
   }
   template <int kI>
   __device__ __forceinline__ void mfma(int b) {
-    constexpr int mt = kI / kNT, nt = kI % kNT;
-    acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-        __builtin_bit_cast(bf16x8, fr[b][nt]), __builtin_bit_cast(bf16x8, fl[b][mt]), acc[mt][nt],
-        0, 0, 0);
+    constexpr int mt = kI / kFR, nt = kI % kFR;
+    if constexpr (kTied)
+      asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
+                   : "+a"(acc[mt][nt])
+                   : "v"(fr[b][nt]), "v"(fl[b][mt]));
+    else
+      acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+          __builtin_bit_cast(bf16x8, fr[b][nt]), __builtin_bit_cast(bf16x8, fl[b][mt]), acc[mt][nt],
+          0, 0, 0);
   }
   // DMA d of a step: R's, which are needed first, then L's.
   template <int kD>
@@ -200,9 +249,9 @@ struct GcCore {
     }
   }
 
-  // One step from the stages that al and ar address: the previous step's last kPost MFMAs with
-  // the reads of sub-step 0 between them, then 4 sub-steps of kSub, the
-  // fragments of sub-step s + 1 read during sub-step s, the DMAs of the steps
+  // One step from the stages that al and ar address: the previous step's last
+  // kPost MFMAs with the reads of sub-step 0 between them, then 2 sub-steps of kSub, the
+  // fragments of sub-step 1 read during sub-step 0, the DMAs of the steps
   // ahead (if they exist) into stages `nl`/`nr` between the first MFMAs.  Those
   // stages were last read in step t - 1, whose reads ended before the barrier
   // that closed it.  The __restrict__ stages tell the compiler that DMAs into
@@ -224,10 +273,10 @@ struct GcCore {
       constexpr int n = decltype(N)::value;
       constexpr int s = n / kSub, i = n % kSub;
       mfma<i>(s & 1);
-      if constexpr (s < 3) {
+      if constexpr (s == 0) {
         static_for<0, kReads>([&](auto Q) {
           constexpr int q = decltype(Q)::value;
-          if constexpr ((q < kSub ? q : kSub - 1) == i) read(lds, s + 1, (s + 1) & 1, q);
+          if constexpr (q * kSub / kReads == i) read(lds, 1, 1, q);
         });
       }
       if constexpr (n % kGap == 0 && n / kGap < kDmas) {
@@ -297,16 +346,14 @@ struct GcCore {
       if (t < kNR - 1) pr.advance();
     });
 #pragma unroll
-    for (int mt = 0; mt < kMT; ++mt)
+    for (int mt = 0; mt < kFL; ++mt)
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) acc[mt][nt][v] = 0.0f;
+      for (int nt = 0; nt < kFR; ++nt) acc[mt][nt] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
     // The first step's opening MFMAs multiply zeros.
 #pragma unroll
-    for (int i = 0; i < kMT; ++i) fl[1][i] = (u32x4){0u, 0u, 0u, 0u};
+    for (int i = 0; i < kFL; ++i) fl[1][i] = (u32x4){0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int i = 0; i < kNT; ++i) fr[1][i] = (u32x4){0u, 0u, 0u, 0u};
+    for (int i = 0; i < kFR; ++i) fr[1][i] = (u32x4){0u, 0u, 0u, 0u};
     close_step(-1, nsteps);
     int t = 0;
     auto one = [&](auto P) {
@@ -328,6 +375,13 @@ struct GcCore {
       if (t < nsteps) one(P);
     });
     static_for<0, kPost>([&](auto I) { mfma<kSub - kPost + decltype(I)::value>(1); });
+    if constexpr (kTied) {
+      asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+#pragma unroll
+      for (int mt = 0; mt < kFL; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < kFR; ++nt) asm volatile("" : "+a"(acc[mt][nt]));
+    }
   }
 
   template <bool kAcross>
@@ -363,22 +417,23 @@ __device__ __forceinline__ void gc_wave_sync() {
 }
 
 // Stores 32 rows x 32 kNT columns of a wave as bf16 through its 32 * 64 * kNT
-// bytes of LDS, whole rows of 64 kNT bytes: value(nt, v) is the lane's register
-// v of column tile nt, already final.  `out` points at row 0, column 0 of the
+// bytes of LDS, whole rows of 64 kNT bytes: value(h, nt, i) is the lane's register
+// i of row half h and column tile nt, already final.  `out` points at row 0, column 0 of the
 // block; `rows` and `cols` (a multiple of 8) bound it.
 template <int kNT, bool kNt, class F>
 __device__ __forceinline__ void gc_store_bf16(F &&value, char *lds, uint16_t *out, int64_t ld,
                                               int64_t rows, int64_t cols, int lane) {
   constexpr int kChunks = 4 * kNT;  // 16-byte chunks of a row
-  const int row = lane & 31, grp = lane >> 5;
+  const int grp = lane >> 4;
 #pragma unroll
-  for (int nt = 0; nt < kNT; ++nt)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const u32x2 w = {pack_bf16x2(value(nt, 4 * j), value(nt, 4 * j + 1)),
-                       pack_bf16x2(value(nt, 4 * j + 2), value(nt, 4 * j + 3))};
-      const int c = (4 * nt + j) ^ (row & (kChunks - 1));
-      *reinterpret_cast<u32x2 *>(lds + 16 * kChunks * row + 16 * c + 8 * grp) = w;
+    for (int nt = 0; nt < 2 * kNT; ++nt) {
+      const int row = 16 * h + (lane & 15);
+      const u32x2 w = {pack_bf16x2(value(h, nt, 0), value(h, nt, 1)),
+                       pack_bf16x2(value(h, nt, 2), value(h, nt, 3))};
+      const int c = (2 * nt + (grp >> 1)) ^ (row & (kChunks - 1));
+      *reinterpret_cast<u32x2 *>(lds + 16 * kChunks * row + 16 * c + 8 * (grp & 1)) = w;
     }
   gc_wave_sync();
   constexpr int kRows = 64 / kChunks;  // rows per store instruction
@@ -405,15 +460,15 @@ template <int kNT, bool kAdd, bool kNt, class F>
 __device__ __forceinline__ void gc_store_f32(F &&value, char *lds, float *out, int64_t ld,
                                              int64_t rows, int64_t cols, int lane) {
   constexpr int kChunks = 8 * kNT;
-  const int row = lane & 31, grp = lane >> 5;
+  const int grp = lane >> 4;
 #pragma unroll
-  for (int nt = 0; nt < kNT; ++nt)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = (8 * nt + 2 * j + grp) ^ (row & (kChunks - 1));
+    for (int nt = 0; nt < 2 * kNT; ++nt) {
+      const int row = 16 * h + (lane & 15);
+      const int c = (4 * nt + grp) ^ (row & (kChunks - 1));
       *reinterpret_cast<floatx4 *>(lds + 16 * kChunks * row + 16 * c) =
-          (floatx4){value(nt, 4 * j), value(nt, 4 * j + 1), value(nt, 4 * j + 2),
-                    value(nt, 4 * j + 3)};
+          (floatx4){value(h, nt, 0), value(h, nt, 1), value(h, nt, 2), value(h, nt, 3)};
     }
   gc_wave_sync();
   constexpr int kRows = 64 / kChunks;

@@ -68,19 +68,24 @@ struct CeLogits {
   int64_t ldg, gcols;  // row length of G, columns of it from g on
 };
 
-__device__ __forceinline__ float other_half(float v) {
+// The largest, or the sum, over the four lanes l % 16 + 16 g that hold a token's
+// columns, in each of them.
+template <class F>
+__device__ __forceinline__ float over_groups(float v, F &&f) {
   const uint32_t b = __builtin_bit_cast(uint32_t, v);
-  const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-  // s[0]: lanes 0-31's value in both halves, s[1]: lanes 32-63's.
-  return __builtin_bit_cast(float, (uint32_t)((threadIdx.x & 32) ? s[0] : s[1]));
+  const auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  v = f(__builtin_bit_cast(float, (uint32_t)s[0]), __builtin_bit_cast(float, (uint32_t)s[1]));
+  const uint32_t c = __builtin_bit_cast(uint32_t, v);
+  const auto t = __builtin_amdgcn_permlane32_swap(c, c, false, false);
+  return f(__builtin_bit_cast(float, (uint32_t)t[0]), __builtin_bit_cast(float, (uint32_t)t[1]));
 }
 
 __device__ __forceinline__ float exp_of(float x) {
   return __builtin_amdgcn_exp2f(x * kLog2e);
 }
 
-// Column of the wave's block (0 .. 32 kNT - 1) of the lane's register v of
-// column tile nt is 32 nt + 8 (v / 4) + 4 (lane / 32) + v % 4.
+// Column of the wave's block (0 .. 32 kNT - 1) of the lane's register i of column
+// tile nt is 16 nt + 4 (lane / 16) + i, its token of row tile mt 16 mt + lane % 16.
 template <int kMT, int kNT, bool kGrad>
 __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_logits_kernel(const CeLogits a) {
   using Core = GcCore<kMT, kNT, false, false>;
@@ -101,51 +106,50 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_logits_kernel
   const int c0 = 32 * kNT * (wave & 1);              // and its first column in the tile
   const int cols = rrows - c0;                       // its columns that exist (may be <= 0)
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt) {
-    // One 32-token block at a time: interleaved, the blocks spill.
+  for (int mt = 0; mt < 2 * kMT; ++mt) {
+    // One block of 16 tokens at a time: interleaved, the blocks spill.
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" : "+v"(lane));
-    floatx16 (&z)[kNT] = core.acc[mt];
+    floatx4 (&z)[2 * kNT] = core.acc[mt];
+    const int grp = lane >> 4;
     if (cols < 32 * kNT) {  // columns past the vocabulary
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+      for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (32 * nt + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3) >= cols)
-            z[nt][v] = -__builtin_inff();
+        for (int i = 0; i < 4; ++i)
+          if (16 * nt + 4 * grp + i >= cols) z[nt][i] = -__builtin_inff();
     }
-    const int grp = lane >> 5;
-    const int64_t row = row0 + 32 * mt + (lane & 31);
+    const int64_t row = row0 + 16 * mt + (lane & 15);
     const bool here = row < a.M;
     const int64_t t = here ? a.targets[row] : a.ignore;
     // The target's register among this lane's, or -1.
     const int64_t rel = t - (a.v0 + r0 + c0);
     const bool mine = t != a.ignore && rel >= 0 && rel < 32 * kNT && rel < cols &&
-                      (((int)rel >> 2) & 1) == grp;
-    const int at = mine ? 16 * ((int)rel >> 5) + 4 * (((int)rel >> 3) & 3) + ((int)rel & 3) : -1;
+                      (((int)rel >> 2) & 3) == grp;
+    const int at = mine ? 4 * ((int)rel >> 4) + ((int)rel & 3) : -1;
     if constexpr (!kGrad) {
       if (__ballot(mine) != 0) {
         float zt = 0.0f;
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
+        for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) zt = at == 16 * nt + v ? z[nt][v] : zt;
+          for (int i = 0; i < 4; ++i) zt = at == 4 * nt + i ? z[nt][i] : zt;
         if (mine) a.zt[row] = zt;
       }
       float top = -__builtin_inff();
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+      for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) top = fmaxf(top, z[nt][v]);
-      top = fmaxf(top, other_half(top));
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, z[nt][i]);
+      top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
       // Nothing but -inf: any finite reference gives a sum of 0.
       const float ref = top == -__builtin_inff() ? 0.0f : top;
       float sum = 0.0f;
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+      for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) sum += exp_of(z[nt][v] - ref);
-      sum += other_half(sum);
+        for (int i = 0; i < 4; ++i) sum += exp_of(z[nt][i] - ref);
+      sum = over_groups(sum, [](float x, float y) { return x + y; });
       if (here && grp == 0)
         a.part[(int64_t)(2 * tr + (wave & 1)) * a.M + row] = make_float2(top, sum);
     } else {
@@ -154,20 +158,27 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_logits_kernel
       float dl = here && !skip ? a.dloss[row] / *a.common : 0.0f;
       if (!skip && (t < 0 || t >= a.V)) dl = __builtin_nanf("");
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+      for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) z[nt][v] = exp_of(z[nt][v] - lse);
+        for (int i = 0; i < 4; ++i) z[nt][i] = exp_of(z[nt][i] - lse);
       if (__ballot(mine) != 0) {
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
+        for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) z[nt][v] -= at == 16 * nt + v ? 1.0f : 0.0f;
+          for (int i = 0; i < 4; ++i) z[nt][i] -= at == 4 * nt + i ? 1.0f : 0.0f;
       }
+#pragma unroll
+      for (int nt = 0; nt < 2 * kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[nt][i] = skip ? 0.0f : fp32_rounded(z[nt][i] * dl);
       // Columns of the piece's last, partial 64 hold zeros: G is read in steps of 64.
-      gc_store_bf16<kNT, false>(
-          [&](int nt, int v) { return skip ? 0.0f : fp32_rounded(z[nt][v] * dl); },
-          lds + 32 * 64 * kNT * wave, a.g + (row0 + 32 * mt) * a.ldg + r0 + c0, a.ldg,
-          a.M - (row0 + 32 * mt), a.gcols - (r0 + c0), lane);
+      if (mt % 2 == 1) {
+        const int64_t first = row0 + 16 * (mt - 1);
+        gc_store_bf16<kNT, false>(
+            [&](int h, int nt, int i) { return core.acc[mt - 1 + h][nt][i]; },
+            lds + 32 * 64 * kNT * wave, a.g + first * a.ldg + r0 + c0, a.ldg, a.M - first,
+            a.gcols - (r0 + c0), lane);
+      }
     }
   }
 }
@@ -263,8 +274,9 @@ __global__ void __launch_bounds__(kGcThreads, kMT * kNT == 4 ? 2 : 1) ce_product
   const float common = kLAcross ? *a.common : 1.0f;
 #pragma unroll
   for (int mt = 0; mt < kMT; ++mt) {
-    auto value = [&](int nt, int v) {
-      return kLAcross ? fp32_rounded(core.acc[mt][nt][v] * common) : core.acc[mt][nt][v];
+    auto value = [&](int h, int nt, int i) {
+      const float v = core.acc[2 * mt + h][nt][i];
+      return kLAcross ? fp32_rounded(v * common) : v;
     };
     const int64_t row = l0 + row0 + 32 * mt;
     const int64_t at = slice * a.slice_stride + row * a.ld + c0;
