@@ -198,7 +198,7 @@ struct GcCore {
   // From 128 accumulator registers on, the instruction is written out with the
   // sum's registers as its own source.  Left to the compiler the sums move: from
   // 50 to 200 copies a step of 128 MFMAs, and 4096 x 32000 x 8192 logits took 1970 us
-  // (1535 tied).  The compiler does not know that the block is an MFMA, so the
+  // (1538 tied).  The compiler does not know that the block is an MFMA, so the
   // waits that it would add are this file's: the fragments come from LDS reads,
   // which it waits for, never from an instruction of the two before; the sums
   // stay where they are until run() has waited for the last of them.
@@ -207,8 +207,8 @@ struct GcCore {
   static constexpr int kDmas = LSide::kDmas + RSide::kDmas;
   // MFMAs from one DMA to the next: spread over what follows the opening, as the
   // reads and the DMAs together keep LDS busy for three quarters of a 256 x 256
-  // step at the MFMA rate.  4096 x 32000 x 8192 logits: 1535 us, with a gap of 4
-  // and the opening a half 1587.
+  // step at the MFMA rate.  4096 x 32000 x 8192 logits: 1538 us; with half a
+  // sub-step in the opening, a gap of 5 1544 and of 4 1587.
   static constexpr int kGap = (kFront - 1) / kDmas;
   static_assert(kDmas <= kFront, "one DMA per MFMA slot at most");
 
@@ -257,9 +257,9 @@ struct GcCore {
   }
 
   // One step from the stages that al and ar address: the previous step's last
-  // kPost MFMAs with the reads of sub-step 0 between them, then 2 sub-steps of kSub, the
-  // fragments of sub-step 1 read during sub-step 0, the DMAs of the steps
-  // ahead (if they exist) into stages `nl`/`nr` between the first MFMAs.  Those
+  // kPost MFMAs with the reads of sub-step 0 between them, then 2 sub-steps of
+  // kSub, the fragments of sub-step 1 read during sub-step 0, the DMAs of the
+  // steps ahead (if they exist) into stages `nl`/`nr` between the MFMAs.  Those
   // stages were last read in step t - 1, whose reads ended before the barrier
   // that closed it.  The __restrict__ stages tell the compiler that DMAs into
   // one never alias reads of the other, so that it waits for them at the

@@ -24,14 +24,13 @@
 // piece: logits again, turned into G in the epilogue; dx += G . w in fp32; the
 // piece's rows of dw.
 //
-// Measured at 4096 tokens, 128000 x 8192: forward 6.2 ms (1377 TFLOP/s), a piece
-// of 32000 columns 1643 us for G (1307), 1585 for dx (1354), 1581 for dw (1358);
+// Measured at 4096 tokens, 128000 x 8192: forward 6.1 ms (1404 TFLOP/s), a piece
+// of 32000 columns 1640 us for G (1309), 1530 for dx (1403), 1595 for dw (1346);
 // library products of these shapes run at 1490, 1328 and 1147.  The matrix
-// pipe is busy 70-79 % of the cycles, at a clock that has fallen to 1.62-1.77
-// GHz: the products are bound by power (an order of loads that hid the first
-// loads of each tile behind the previous epilogue changed nothing).  Few tokens
-// read w once for each product and write dw: one token over 128000 x 8192,
-// gradients 1127 us (5.6 TB/s), forward 363 us (5.8).
+// pipe is busy 65-72 % of the cycles, at a clock that has fallen to 1.77-1.91
+// GHz: power sets the rate (bf16_gemm_core.hpp), and waves wait 13-18 % of their
+// time.  Few tokens read w once for each product and write dw: one token over
+// 128000 x 8192, gradients 1130 us (5.6 TB/s), forward 354 us (5.9).
 #include <cmath>
 
 #include "bf16_gemm_core.hpp"
@@ -42,8 +41,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // G of a piece: what the Infinity Cache (256 MB) holds between the kernel that
-// writes it and the two that read it.  Gradients of 8192 x 32000 x 4096: 4975 us
-// with 256 MB, 5185 with half, 4902 with four times as much.
+// writes it and the two that read it.  Gradients of 8192 x 32000 x 4096: 4804 us
+// with 256 MB, 4 % more with half, 1.5 % less with four times as much.
 constexpr int64_t kCePieceBytes = (int64_t)256 << 20;
 // Tokens of one forward launch, which bounds its partial sums.
 constexpr int64_t kCeTokens = 16384;
@@ -334,8 +333,8 @@ __global__ void ce_zero_kernel(T *p, int64_t n) {
 
 constexpr int64_t kCeFewTokens = 128;
 
-// Tile columns of a strip (gc_tile): 4096 x 32000 x 8192 logits 1601 us with 4,
-// 1627 with 6, 1659 with 8, 2056 with 16 (that one before the third L stage).
+// Tile columns of a strip (gc_tile): 4096 x 32000 x 8192 logits 1566 us with 4,
+// 1595 with 6, 1629 with 8, 1716 with 16.
 constexpr int kCeStrip = 4;
 
 static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -354,9 +353,9 @@ struct CeLaunch {
 // second launch.  Fitted to forwards of 1 to 1500 tokens over 1000 to 128000
 // columns, d = 1024 to 8192 (times in us at d = 4096 with 64 x 128, 128 x 256
 // and 256 x 256 tiles):
-//   1 token, 32000 columns 45, 52, 81;  128 tokens 65, 62, 89;
-//   256 tokens 97, 70, 96;  512 tokens 163, 126, 114;
-//   1000 tokens, 50021 columns 556, 409, 398 (three rounds and the rest 351).
+//   1 token, 32000 columns 43, 58, 86;  128 tokens 53, 59, 88;
+//   256 tokens 93, 66, 95;  512 tokens 171, 124, 106;
+//   1000 tokens, 50021 columns 553, 416, 382 (three rounds and the rest 343).
 // 128 x 128 and 128 x 64 tiles were within 3 % of the best of the three at
 // most, and are not built.
 struct CeTile {
@@ -438,8 +437,9 @@ struct CePlan {
 // slices' fp32 sums move at 2.4 TB/s (written, read and written by each further
 // piece, read for the join).  Fitted to 1 to 4096 tokens, 8000 to 50021
 // columns, d = 1024 to 8192, all heights and 1 to 32 slices: 1 % from the best
-// on average, 6 % at most.  The gradients of 777 x 32000 x 4096: 659 us with 14
-// tiles of 128 rows x 2 slices, 663 with 256 rows x 4, 995 with 256 rows in one.
+// on average, 6 % at most.  The gradients of 777 x 32000 x 4096: 642 us with 14
+// tiles of 128 rows x 2 slices, 1 % more with 256 rows x 4, half as much again
+// with 256 rows in one.
 constexpr CeTile kCeDxTiles[3] = {{1, 4, 2, 0.75, 0.97, 5.0}, {2, 4, 1, 0.61, 0.88, 5.0},
                                   {4, 4, 1, 0.95, 1.03, 5.0}};
 static void ce_dx_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {

@@ -1,6 +1,6 @@
 // tr_tile.hpp - LDS tiles whose reduction index is the row (a row-major operand
 // whose columns are MFMA operands) and their transposing fragment reads, for
-// the gfx950 products dY^T . X and P . W.
+// the gfx950 product dY^T . X.
 #pragma once
 
 #include "gemm_common.hpp"
