@@ -64,22 +64,20 @@ def step(model: Model, x: torch.Tensor, targets: torch.Tensor) -> dict:
     """Losses and every gradient for embeddings x (fp32 [M, d])."""
     layers = len(model.pinned)
     current = torch.cuda.current_stream()
-    kept = [None] * (layers + 1)  # checkpoints of the residual
-    rms_pre, rms_post = [None] * (layers + 1), [None] * layers
+    kept = []  # checkpoints of the residual that each layer starts from
 
     # First pass: one residual, overwritten at every boundary.
     res = x.clone()
-    kept[0] = checkpoint.encode(res)
-    y, rms_pre[0] = norm.rms_norm_fwd(res, model.w_pre[0])
-    state = {"y": y}
+    y, rms = norm.rms_norm_fwd(res, model.w_pre[0])
+    state = {"y": y, "rms": rms}
 
     def forward(l, w):
+        kept.append(checkpoint.encode(res))
         hidden = gemm.linear_swiglu(state["y"], w[0], w[1])
         h = gemm.linear_fwd(hidden, w[2])
         b = norm.block_norm_fwd(h, res, model.w_pre[l + 1], model.w_post[l], model.gate[l], ALPHA,
                                 out=res)
-        kept[l + 1] = checkpoint.encode(res)
-        rms_pre[l + 1], rms_post[l], state["y"] = b.rms_pre, b.rms_post, b.y
+        state["y"], state["rms"] = b.y, b.rms_pre
 
     stream.run_stack(model.pinned, model.layout, model.dbuf, forward, current)
 
@@ -91,18 +89,22 @@ def step(model: Model, x: torch.Tensor, targets: torch.Tensor) -> dict:
     dy, dhead = loss.linear_cross_entropy_bwd(y, model.head, targets, lse, dloss)
     grads = {"head": dhead, "w_pre": [None] * (layers + 1), "w_post": [None] * layers,
              "gate": [None] * layers, "layers": [None] * layers}
-    state = {"dy": dy, "dres": None}
+    # Second pass, in reverse: recompute from the checkpoint, then backward.  Every
+    # norm's backward gets the rms of the values it gets: of the last residual,
+    # which is still there, then of the checkpoints as they read back, and of the
+    # recomputed h.
+    state = {"dy": dy, "dres": None, "res": res, "rms": state["rms"]}
 
-    # Second pass, in reverse: recompute from the checkpoint, then backward.
     def backward(i, w):
         l = layers - 1 - i
-        _, y, _ = checkpoint.decode_norm(kept[l], model.w_pre[l], want_x=False)
+        _, y, rms = checkpoint.decode_norm(kept[l], model.w_pre[l], want_x=False)
         g, u = (t.float() for t in gemm.linear_fwd_grouped(y, w[:2]))
         s = torch.sigmoid(g)
         hidden = (g * s * u).to(torch.bfloat16)
         h = gemm.linear_fwd(hidden, w[2])
-        b = norm.block_norm_bwd(state["dy"], state["dres"], kept[l + 1], rms_pre[l + 1],
-                                model.w_pre[l + 1], h=h, rms_post=rms_post[l],
+        rms_post = (h.float().square().mean(1) + norm.EPS).sqrt()
+        b = norm.block_norm_bwd(state["dy"], state["dres"], state["res"], state["rms"],
+                                model.w_pre[l + 1], h=h, rms_post=rms_post,
                                 w_post=model.w_post[l], gate=model.gate[l], alpha=ALPHA,
                                 out=state["dres"])
         dhidden = gemm.linear_dgrad(b.dh, w[2]).float()
@@ -112,9 +114,11 @@ def step(model: Model, x: torch.Tensor, targets: torch.Tensor) -> dict:
                               gemm.linear_wgrad(b.dh, hidden)]
         grads["w_pre"][l + 1], grads["w_post"][l], grads["gate"][l] = b.dw_pre, b.dw_post, b.dgate
         state["dy"], state["dres"] = gemm.linear_dgrad_sum([dg, du], w[:2]), b.dres
+        state["res"], state["rms"] = kept[l], rms
 
     stream.run_stack(model.pinned[::-1], model.layout, model.dbuf, backward, current)
-    b = norm.block_norm_bwd(state["dy"], state["dres"], kept[0], rms_pre[0], model.w_pre[0])
+    b = norm.block_norm_bwd(state["dy"], state["dres"], state["res"], state["rms"],
+                            model.w_pre[0])
     grads["w_pre"][0], grads["x"] = b.dw_pre, b.dres
     return {"losses": losses, "loss": losses.sum() / count, "grads": grads}
 
