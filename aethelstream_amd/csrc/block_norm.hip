@@ -189,7 +189,8 @@ struct NormChunk {
 //   A = f sum e r,  B = q sum k h (dr' + f e),  C = f q sum k h r,
 // and the outputs from two factors a row: g = dr' + f e - (A / d) f^2 r and
 // dh = q k g - (E / d) q^2 h, E = B - (A / d) f C: 21 vector instructions an
-// element, which two waves a SIMD overlap with the memory.
+// element, which the waves of a SIMD (four up to 12288 columns) overlap with the
+// memory.
 template <int kMaxThreads, int kChunks, bool kH, int kMode>
 __global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(const BlockNormBwd a) {
   __shared__ float part[2][48];
@@ -417,8 +418,8 @@ __global__ void __launch_bounds__(256) block_norm_columns_kernel(
   }
 }
 
-// Waves of the persistent kernels on a CU.
-constexpr int kFwdWaves = 8, kBwdWaves = 16;
+// Waves of the persistent forward on a CU.
+constexpr int kFwdWaves = 8;
 
 // Threads of a row of `chunks` chunks: four chunks a thread up to 1024 threads,
 // then eight.
@@ -439,20 +440,25 @@ static int bwd_threads(int64_t chunks) {
   return (int)(((chunks + per - 1) / per + 63) / 64 * 64);
 }
 
+// Waves of the backward that a CU holds: two a SIMD of the kernel of 12292 to
+// 16384 columns, which takes up to 256 registers, four of the others.  (1000 rows
+// of 16384: 84 us; with 16 waves, twice the workgroups in two rounds, 94.)
+static int bwd_waves(int64_t chunks) { return chunks > 3072 && chunks <= 4096 ? 8 : 16; }
+
 // Rows of a backward workgroup side by side: up to 512 threads.
 static int bwd_teams(int64_t chunks) {
   const int t = bwd_threads(chunks);
   return t >= 512 ? 1 : 512 / t;
 }
 
-// Workgroups of the backward: at most as many as run at once (16 waves a CU).
+// Workgroups of the backward: at most as many as run at once (bwd_waves).
 // Every one writes two rows of column sums, so one row a team only up to one
 // workgroup a CU, then two (64 rows of 4096: 9.5 us with one row a team, 13.1
 // with four; 512 rows: 16.0 us with two, 21.3 with one).
 static int64_t bwd_groups(int64_t m, int64_t d) {
   const int64_t teams = bwd_teams(d / 4), waves = teams * (bwd_threads(d / 4) / 64);
-  const int64_t cus = cu_slots();
-  const int64_t most = cus * (waves >= kBwdWaves ? 1 : kBwdWaves / waves);
+  const int64_t cus = cu_slots(), fit = bwd_waves(d / 4);
+  const int64_t most = cus * (waves >= fit ? 1 : fit / waves);
   const int64_t one = (m + teams - 1) / teams, two = (m + 2 * teams - 1) / (2 * teams);
   const int64_t n = one < cus ? one : (two > cus ? two : cus);
   return n < most ? n : most;
