@@ -349,21 +349,25 @@ struct CeLaunch {
 // whole rounds of large tiles and the rest in smaller ones.  Cost of a launch in
 // us: each round takes, per step of 64, `lo` when few tiles run to `hi` when the
 // chip is full (less traffic and a higher clock when it is not); w is read at
-// `tbs`, again by part for each further row of tiles; 8 us beside, 14 for a
-// second launch.  Fitted to forwards of 1 to 1500 tokens over 1000 to 128000
-// columns, d = 1024 to 8192 (times in us at d = 4096 with 64 x 128, 128 x 256
-// and 256 x 256 tiles):
-//   1 token, 32000 columns 43, 58, 86;  128 tokens 53, 59, 88;
-//   256 tokens 93, 66, 95;  512 tokens 171, 124, 106;
-//   1000 tokens, 50021 columns 553, 416, 382 (three rounds and the rest 343).
+// `tbs`, again by part for each further row of tiles; 8 us beside for each launch.
+// Fitted to all choices at 615 forwards of 1 to 2000 tokens over 1000 to 150000
+// columns, d = 512 to 8192, and 54 gradients, with w from memory (in turn from
+// copies that no cache holds together): 0.2 % from the best on average, within
+// 2 % at 645 of them, 10 % at most.  Times in us at d = 4096 with 64 x 128, 128 x
+// 256 and 256 x 256 tiles:
+//   1 token, 32000 columns 61, 66, 98;  50021 columns 80, 91, 109;
+//   77 tokens, 32000 columns 66, 69, 100;  50021 columns 111, 92, 110;
+//   128 tokens, 32000 columns 71, 70, 100;  256 tokens 115, 72, 100;
+//   512 tokens 204, 122, 107;
+//   1000 tokens, 50021 columns 567, 411, 382 (three rounds and the rest 327).
 // 128 x 128 and 128 x 64 tiles were within 3 % of the best of the three at
 // most, and are not built.
 struct CeTile {
   int mt, nt, slots;  // slots: workgroups a CU
   double lo, hi, tbs;
 };
-constexpr CeTile kCeTiles[3] = {{1, 2, 2, 0.30, 0.70, 5.4}, {2, 4, 1, 0.66, 0.92, 5.7},
-                                {4, 4, 1, 1.14, 1.62, 5.4}};
+constexpr CeTile kCeTiles[3] = {{1, 2, 2, 0.21, 0.74, 6.9}, {2, 4, 1, 0.98, 0.99, 6.8},
+                                {4, 4, 1, 1.23, 1.51, 5.3}};
 
 static int64_t ceil_to(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -374,7 +378,7 @@ static double ce_cost(const CeTile &c, int64_t m, int64_t v, int64_t d) {
   const double part = (double)(T % slots) / (double)slots;
   const double compute =
       steps * ((double)(T / slots) * c.hi + (part > 0.0 ? c.lo + (c.hi - c.lo) * part : 0.0));
-  const double memory = 2e-6 * (double)v * (double)d / c.tbs * (0.75 + 0.25 * (double)tl);
+  const double memory = 2e-6 * (double)v * (double)d / c.tbs * (0.79 + 0.21 * (double)tl);
   return 8.0 + (compute > memory ? compute : memory);
 }
 
@@ -402,7 +406,7 @@ static int ce_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&out)[2]) {
     const int64_t rounds = T / cu_slots();
     const int64_t cols = rounds * cu_slots() / tl * (64 * a.nt);
     if (rounds == 0 || cols == 0 || cols >= v) continue;
-    const double t = ce_cost(a, m, cols, d) + smallest(v - cols, i, c) + 6.0;
+    const double t = ce_cost(a, m, cols, d) + smallest(v - cols, i, c);
     if (t < best) {
       best = t;
       out[0] = CeLaunch{a.mt, a.nt, cols};
