@@ -23,6 +23,7 @@
 #include "abi_common.hpp"
 #include "gemm_common.hpp"
 #include "nf4_device.hpp"
+#include "tr_tile.hpp"
 
 namespace nf4s {
 
@@ -58,19 +59,6 @@ __device__ __forceinline__ GcOperand gc_across(const uint16_t *p, int64_t ld, in
 template <bool kWide>
 __device__ __forceinline__ int gc_swz(int row) {
   return (row & 7) ^ (kWide ? (row >> 3) & 1 : 0);
-}
-
-// Fragment (8 k of one column) of an operand across the reduction, whose rows are
-// kUnits 16-byte units long.
-template <int kUnits>
-__device__ __forceinline__ u32x4 gc_tr_frag(const char *base, uint32_t off) {
-  typedef __attribute__((address_space(3))) char lds_char_t;
-  typedef __attribute__((address_space(3))) v4i16 lds_v4i16_t;
-  lds_char_t *p = (lds_char_t *)const_cast<char *>(base) + off;
-  const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t *)p);
-  const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t *)(p + 64 * kUnits));
-  const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-  return (u32x4){l2.x, l2.y, h2.x, h2.y};
 }
 
 // LDS tile of an operand across it: k rows of kUnits (32 or 16) units.  Unit u
@@ -115,7 +103,7 @@ struct GcSide {
   static __device__ __forceinline__ u32x4 frag(const char *base, const uint32_t (&a)[kAddrs],
                                                int s, int j) {
     if constexpr (kAcross)
-      return gc_tr_frag<kUnits>(base, (a[0] ^ (32 * j)) + 512 * kUnits * s);
+      return tr_frag<kUnits>(base, (a[0] ^ (32 * j)) + 512 * kUnits * s);
     else
       return *reinterpret_cast<const u32x4 *>(base + a[s] + 2048 * j);
   }

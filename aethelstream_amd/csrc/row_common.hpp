@@ -41,30 +41,10 @@ __device__ __forceinline__ float row_wave_sum(float v) {
   return __builtin_bit_cast(float, (uint32_t)t[0]) + __builtin_bit_cast(float, (uint32_t)t[1]);
 }
 
-// kN sums over the workgroup, in every thread.  `part` holds kN values for each
-// of up to 16 waves; a caller that comes again before every wave has passed
-// another barrier takes another one.
-template <int kN>
-__device__ __forceinline__ void row_block_sum(float (&v)[kN], float *part) {
-#pragma unroll
-  for (int i = 0; i < kN; ++i) v[i] = row_wave_sum(v[i]);
-  const int waves = (int)(blockDim.x >> 6);
-  if (waves == 1) return;
-  if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) part[16 * i + (threadIdx.x >> 6)] = v[i];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    float tot = 0.0f;
-    for (int w = 0; w < waves; ++w) tot += part[16 * i + w];
-    v[i] = tot;
-  }
-}
-
 // kN sums over each team of `waves` waves of the workgroup, in every thread of
-// the team.  Every wave of the workgroup calls it.
+// the team.  Every wave of the workgroup calls it.  `part` holds kN values for
+// each of up to 16 waves; a caller that comes again before every wave has passed
+// another barrier takes another one.
 template <int kN>
 __device__ __forceinline__ void row_team_sum(float (&v)[kN], float *part, int team, int waves) {
 #pragma unroll
@@ -81,6 +61,12 @@ __device__ __forceinline__ void row_team_sum(float (&v)[kN], float *part, int te
     for (int w = 0; w < waves; ++w) tot += part[16 * i + team * waves + w];
     v[i] = tot;
   }
+}
+
+// kN sums over the workgroup, in every thread.
+template <int kN>
+__device__ __forceinline__ void row_block_sum(float (&v)[kN], float *part) {
+  row_team_sum(v, part, 0, (int)(blockDim.x >> 6));
 }
 
 __device__ __forceinline__ float bf16_low(uint32_t v) {
