@@ -49,6 +49,9 @@ constexpr int64_t kCeTokens = 16384;
 // A launch counts its threads in 32 bits.
 constexpr int64_t kMaxTiles = 0xffffffffll / kGcThreads;
 
+// Maximum and sum of exponentials of part of a token's logits.
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+
 struct CeLogits {
   const uint16_t *x, *w;  // w at the piece's first row
   const int64_t *targets;
@@ -58,7 +61,7 @@ struct CeLogits {
   int64_t V, ignore;
   int32_t tiles_l, tiles_r, strip;
   // forward
-  float2 *part;      // [2 tiles_r][M]: maximum, sum of exponentials
+  floatx2 *part;     // [2 tiles_r][M]
   float *zt;         // [M] logit of the target
   // backward
   const float *lse, *dloss;
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_logits_kernel
         for (int i = 0; i < 4; ++i) sum += exp_of(z[nt][i] - ref);
       sum = over_groups(sum, [](float x, float y) { return x + y; });
       if (here && grp == 0)
-        a.part[(int64_t)(2 * tr + (wave & 1)) * a.M + row] = make_float2(top, sum);
+        a.part[(int64_t)(2 * tr + (wave & 1)) * a.M + row] = (floatx2){top, sum};
     } else {
       const float lse = here ? a.lse[row] : 0.0f;
       const bool skip = t == a.ignore;
@@ -185,24 +188,24 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) ce_logits_kernel
 // Joins a token's partial sums: 256 / kTokens threads a token take every so many
 // slices, four loads ahead, then meet in a fixed order.
 template <int kTokens>
-__global__ void __launch_bounds__(256) ce_join_kernel(const float2 *part, const float *zt,
+__global__ void __launch_bounds__(256) ce_join_kernel(const floatx2 *part, const float *zt,
                                                       const int64_t *targets, int64_t M,
                                                       int32_t slices, int64_t V, int64_t ignore,
                                                       float *loss, float *lse) {
   constexpr int kGroups = 256 / kTokens;
-  __shared__ float2 lds[kGroups][kTokens];
+  __shared__ floatx2 lds[kGroups][kTokens];
   const int tok = threadIdx.x % kTokens, grp = threadIdx.x / kTokens;
   const int64_t row = (int64_t)blockIdx.x * kTokens + tok;
-  auto join = [](float2 a, float2 b) {
+  auto join = [](floatx2 a, floatx2 b) {
     const float top = fmaxf(a.x, b.x);
     const float ref = top == -__builtin_inff() ? 0.0f : top;
-    return make_float2(top, a.y * exp_of(a.x - ref) + b.y * exp_of(b.x - ref));
+    return (floatx2){top, a.y * exp_of(a.x - ref) + b.y * exp_of(b.x - ref)};
   };
-  const float2 none = make_float2(-__builtin_inff(), 0.0f);
-  float2 s = none;
+  const floatx2 none = {-__builtin_inff(), 0.0f};
+  floatx2 s = none;
   if (row < M)
     for (int i = grp; i < slices; i += 4 * kGroups) {
-      float2 v[4];
+      floatx2 v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int n = i + j * kGroups;
@@ -619,7 +622,7 @@ int32_t nf4s_linear_ce_fwd(const uint16_t *x, const uint16_t *w, const int64_t *
   a.vn = (int32_t)v;
   a.V = v;
   a.ignore = ignore_index;
-  a.part = static_cast<float2 *>(workspace);
+  a.part = static_cast<floatx2 *>(workspace);
   a.zt = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.part_bytes);
   for (int64_t m0 = 0; m0 < m; m0 += p.tokens) {
     a.M = m - m0 < p.tokens ? m - m0 : p.tokens;
