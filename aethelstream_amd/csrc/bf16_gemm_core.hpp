@@ -51,11 +51,13 @@ __device__ __forceinline__ GcOperand gc_across(const uint16_t *p, int64_t ld, in
 
 // LDS tile of an operand along the reduction: rows of 128 bytes, 8 units of 16.
 // Unit u of row r lives at physical unit u ^ gc_swz(r).  With r & 7 the fragment
-// reads (16 rows of 4 units a wave) have no bank conflicts: 77 x 32000 x 4096
-// logits 56 us, with a second term 58.  Tiles of 256 x 256 have the second term,
-// which doubles half the banks' accesses and is faster there nonetheless: 4096 x
-// 32000 x 8192 logits 1580 us and 1608 without, gradients 4870 and 4893, in four
-// orders of running them.
+// reads (16 rows of 4 units a wave) have no bank conflicts.  Tiles of 256 x 256
+// have a second term, which doubles half the banks' accesses and is faster there
+// nonetheless: 4096 x 32000 x 8192 forward 1520 us and 1521 without, the median of
+// five 1536 and 1559, gradients 4641 and 4693.  In smaller tiles it makes no
+// difference while w comes from memory (77 x 32000 x 4096 67 us either way), 2 to 4
+// % where it is in the caches.  (Times of this file: whole calls, the variants in
+// turn on one card, the least of five.)
 template <bool kWide>
 __device__ __forceinline__ int gc_swz(int row) {
   return (row & 7) ^ (kWide ? (row >> 3) & 1 : 0);
@@ -185,8 +187,8 @@ struct GcCore {
   static constexpr int kReads = kFL + kFR;
   // From 128 accumulator registers on, the instruction is written out with the
   // sum's registers as its own source.  Left to the compiler the sums move: from
-  // 50 to 200 copies a step of 128 MFMAs, and 4096 x 32000 x 8192 logits took 1970 us
-  // (1538 tied).  The compiler does not know that the block is an MFMA, so the
+  // 50 to 200 copies a step of 128 MFMAs, and 4096 x 32000 x 8192 logits take 1946 us
+  // (1520 tied).  The compiler does not know that the block is an MFMA, so the
   // waits that it would add are this file's: the fragments come from LDS reads,
   // which it waits for, never from an instruction of the two before; the sums
   // stay where they are until run() has waited for the last of them.
@@ -195,8 +197,8 @@ struct GcCore {
   static constexpr int kDmas = LSide::kDmas + RSide::kDmas;
   // MFMAs from one DMA to the next: spread over what follows the opening, as the
   // reads and the DMAs together keep LDS busy for three quarters of a 256 x 256
-  // step at the MFMA rate.  4096 x 32000 x 8192 logits: 1538 us; with half a
-  // sub-step in the opening, a gap of 5 1544 and of 4 1587.
+  // step at the MFMA rate.  4096 x 32000 x 8192 logits: 1520 us; with half a
+  // sub-step in the opening, a gap of 5 1526 and of 4 1568.
   static constexpr int kGap = (kFront - 1) / kDmas;
   static_assert(kDmas <= kFront, "one DMA per MFMA slot at most");
 

@@ -32,9 +32,16 @@
 // sums in registers, join those of their rows through LDS and write them once;
 // a second kernel adds the workgroups' in order.
 //
-// Measured at 8192 x 8192: forward 131 us (6.2 TB/s; 154 with a workgroup a row,
-// which reads the weights for every row), backward 215 us (5.6) and 4.6 for the
-// columns; from a checkpoint at 4096 x 4096 52 us (4.8).  One row of 4096: 4 us.
+// Measured at 8192 x 8192: forward 132 us (6.1 TB/s; 154 with a workgroup a row,
+// which reads the weights for every row), backward 215 to 221 us (5.5) and 4.6 for
+// the columns; from a checkpoint at 4096 x 4096 52 us (4.8).  One row of 4096: 4
+// us.  Whole calls there: without the block's norm and gate 134 and 213 us,
+// without dres 181, without a block 165.
+// Longer rows do not fit the registers: the forward past 16384 columns keeps 20 of
+// a lane in scratch, the backward 52 (with a block) and 54, that of a block of
+// 12292 to 16384 columns 8.  Whole calls of 4096 rows, forward and backward: 13824
+// columns 121 and 271 us (5.6 and 3.8 TB/s), 16384 145 and 286 (5.6, 4.2), 28672
+// 290 and 833 (4.9, 2.5), 32768 341 and 905 (4.7, 2.7; without a block 557).
 #include "row_common.hpp"
 
 namespace nf4s {

@@ -7,9 +7,10 @@
 //   z = x . w^T,  lse_m = log sum_c exp z_mc,  loss_m = lse_m - z_m,t(m)
 //   G_mc = (exp(z_mc - lse_m) - [c = t(m)]) dloss_m / c
 //   dx = c G . w,   dw = c G^T . x,   c = max |dloss|
-// An ignored target gives loss 0 and a row of G that is 0; one outside [0, V)
-// that is not the ignored value gives NaN.  Products accumulate in fp32;
-// maxima, sums, lse and loss are fp32.
+// An ignored target gives loss 0 and a row of G that is 0 (times its row of x in
+// dw: what is not finite there reaches dw); one outside [0, V) that is not the
+// ignored value gives NaN.  Products accumulate in fp32; maxima, sums, lse and
+// loss are fp32.
 //
 // Forward: a tile of logits (tokens x vocabulary) stays in its accumulators; a
 // lane holds one token's columns, so the tile's maximum and sum of exponentials
@@ -18,19 +19,27 @@
 // 256 x 256 tiles, where the logits would be 2 M V.
 // Backward: the vocabulary in pieces whose G (bf16, the operand of both
 // products: one rounding of each value, as of every dY of the weight gradients)
-// fits kCePieceBytes.  The common factor c stays out of G: the tokens of a mean
-// all have dloss = c, whose rounding error would be that of every target's
-// entry (up to 2^-8 at once); divided by c those entries are close to -1.  Per
-// piece: logits again, turned into G in the epilogue; dx += G . w in fp32; the
-// piece's rows of dw.
+// fits kCePieceBytes.  G in two bf16 terms would double two of the four products.
+// The common factor c stays out of G: the tokens of a mean all have dloss = c,
+// whose rounding error would be that of every target's entry (up to 2^-8 at once);
+// divided by c those entries are close to -1.  What the rounding costs, relative
+// errors of 77 to 512 tokens over 4000 to 32000 columns: of a mean, dx and the
+// rows of dw that are some token's target 0.0017, as a bf16 result alone; the
+// other rows of dw 0.0023; in an fp32 dw 0.0001 and 0.0016.  With a weight for each
+// token its target's entry is rounded like any other: dx and the targets' rows
+// 0.0022, in an fp32 dw 0.0013.  Per piece: logits again, turned into G in the
+// epilogue; dx += G . w in fp32; the piece's rows of dw.
 //
-// Measured at 4096 tokens, 128000 x 8192: forward 6.1 ms (1404 TFLOP/s), a piece
-// of 32000 columns 1640 us for G (1309), 1530 for dx (1403), 1595 for dw (1346);
+// Measured at 4096 tokens, 128000 x 8192: forward 5.95 ms (1443 TFLOP/s), a piece
+// of 32000 columns 1627 us for G (1320), 1519 for dx (1414), 1576 for dw (1363);
 // library products of these shapes run at 1490, 1328 and 1147.  The matrix
 // pipe is busy 65-72 % of the cycles, at a clock that has fallen to 1.77-1.91
 // GHz: power sets the rate (bf16_gemm_core.hpp), and waves wait 13-18 % of their
 // time.  Few tokens read w once for each product and write dw: one token over
-// 128000 x 8192, gradients 1130 us (5.6 TB/s), forward 354 us (5.9).
+// 128000 x 8192, gradients 1142 us (5.5 TB/s), forward 363 us (5.8).  dw in fp32
+// instead of bf16, stored and accumulated: 1486 and 2908 us there; 224 and 401
+// for 77 tokens, 32000 x 4096 (bf16 202); 18.9 and 20.7 ms for 4096 tokens, 128000
+// x 8192 (18.6).
 #include <cmath>
 
 #include "bf16_gemm_core.hpp"
@@ -41,8 +50,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // G of a piece: what the Infinity Cache (256 MB) holds between the kernel that
-// writes it and the two that read it.  Gradients of 8192 x 32000 x 4096: 4804 us
-// with 256 MB, 4 % more with half, 1.5 % less with four times as much.
+// writes it and the two that read it.  Gradients of 8192 x 32000 x 4096: 4813 us
+// with 256 MB, 4941 with half, 4772 with four times as much; of 4096 x 128000 x
+// 8192 18.9, 19.1 and 18.6 ms.
 constexpr int64_t kCePieceBytes = (int64_t)256 << 20;
 // Tokens of one forward launch, which bounds its partial sums.
 constexpr int64_t kCeTokens = 16384;
@@ -245,7 +255,7 @@ struct CeProduct {
 
 // Output of a product: dx partials (fp32, stored or added) along the vocabulary,
 // dw (fp32 or bf16) along the tokens.  dw is not read again and leaves by
-// non-temporal stores: 77 tokens, 32000 x 4096, gradients 228 -> 203 us.
+// non-temporal stores: 77 tokens, 32000 x 4096, gradients 236 -> 207 us.
 enum { kOutF32, kOutF32Add, kOutBf16 };
 
 template <int kMT, int kNT, bool kLAcross, int kOut>
@@ -336,8 +346,8 @@ __global__ void ce_zero_kernel(T *p, int64_t n) {
 
 constexpr int64_t kCeFewTokens = 128;
 
-// Tile columns of a strip (gc_tile): 4096 x 32000 x 8192 logits 1566 us with 4,
-// 1595 with 6, 1629 with 8, 1716 with 16.
+// Tile columns of a strip (gc_tile): 4096 x 32000 x 8192 forward 1520 us with 4,
+// 1549 with 6, 1577 with 8, 1666 with 16.
 constexpr int kCeStrip = 4;
 
 static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -443,10 +453,11 @@ struct CePlan {
 // fourth powers (the larger one, a little more where they are close); what the
 // slices' fp32 sums move at 2.4 TB/s (written, read and written by each further
 // piece, read for the join).  Fitted to 1 to 4096 tokens, 8000 to 50021
-// columns, d = 1024 to 8192, all heights and 1 to 32 slices: 1 % from the best
-// on average, 6 % at most.  The gradients of 777 x 32000 x 4096: 642 us with 14
-// tiles of 128 rows x 2 slices, 1 % more with 256 rows x 4, half as much again
-// with 256 rows in one.
+// columns, d = 1024 to 8192, all heights and 1 to 32 slices; measured again with
+// the present products at 72 shapes of 1 to 4096 tokens, 8000 to 128000 columns:
+// 0.1 % from the best on average, 3 % at most.  The gradients of 777 x 32000 x
+// 4096: 615 us with tiles of 128 rows x 2 slices, 616 with 256 rows x 4, 938 and
+// 999 with 64 and 256 rows in one.
 constexpr CeTile kCeDxTiles[3] = {{1, 4, 2, 0.75, 0.97, 5.0}, {2, 4, 1, 0.61, 0.88, 5.0},
                                   {4, 4, 1, 0.95, 1.03, 5.0}};
 static void ce_dx_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {

@@ -364,7 +364,8 @@ int32_t nf4s_block_norm_fwd(const uint16_t *h, const float *res, const float *w_
  * Its backward.  dy (bf16) is the gradient of y, dres (fp32, NULL: zero) the one
  * that reaches res_out by the residual path.  res_out comes as fp32 (res) or as
  * its 8-bit checkpoint (res_codes, res_scales: nf4s_ckpt8_encode), exactly one
- * of them.  Writes dres_out = the gradient of res (fp32, may be dres), dh (bf16,
+ * of them; rms_pre and rms_post are those of the values given, of a checkpoint
+ * what it reads back as (nf4s_ckpt8_decode_norm gives that rms).  Writes dres_out = the gradient of res (fp32, may be dres), dh (bf16,
  * set iff h is), and the column sums dw_pre, dw_post (set iff w_post is) and
  * dgate (set iff gate is), all fp32 [d], zero when m = 0.  h = NULL is the
  * backward of the plain RMSNorm (doublepass/src/math.rs:28-59), without w_post
@@ -409,8 +410,9 @@ int32_t nf4s_ckpt8_decode_norm(const uint8_t *codes, const float *scales, const 
  * Cross entropy of a linear head, without keeping the logits z = x . w^T:
  *   lse[i] = log sum_c exp z[i, c],  loss[i] = lse[i] - z[i, targets[i]]
  * x [m, d] and w [v, d] bf16 row-major, targets int64 [m], loss and lse fp32
- * [m].  A target equal to ignore_index gives loss 0 and no gradient, any other
- * outside [0, v) gives NaN.  Takes the place of the reference's two passes over
+ * [m].  A target equal to ignore_index gives loss 0 and no gradient (its row of
+ * x, times 0, is part of dw's sum and has to be finite), any other outside [0, v)
+ * gives NaN.  Takes the place of the reference's two passes over
  * vocabulary tiles (doublepass/src/loss.rs,
  * doublepass/kernels/fused_ce.cu:71-207).
  * Requires d % 8 == 0, m <= 2^24, v <= 2^28, d <= 2^20; x, w, dx, dw and the
@@ -425,8 +427,9 @@ int32_t nf4s_linear_ce_fwd(const uint16_t *x, const uint16_t *w, const int64_t *
  *   G[i, c] = (exp(z[i, c] - lse[i]) - [c = targets[i]]) * dloss[i]
  *   dx = G . w (bf16 [m, d]),  dw = G^T . x (bf16 [v, d], or fp32 with
  *   dw_is_f32; accumulate, fp32 only, adds to dw)
- * G is computed in pieces of the vocabulary and rounded to bf16 as an operand
- * of both products, which accumulate in fp32.
+ * G is computed in pieces of the vocabulary, divided by the largest |dloss| and
+ * rounded to bf16 as an operand of both products, which accumulate in fp32: a
+ * relative error of up to 2^-8 for each entry of G, also in an fp32 dw.
  */
 int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
                            const float *lse, const float *dloss, int64_t m, int64_t v, int64_t d,
