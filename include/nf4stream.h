@@ -407,6 +407,45 @@ int32_t nf4s_ckpt8_decode_norm(const uint8_t *codes, const float *scales, const 
                                float *rms, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Queries and keys between their products (doublepass/src/forward.rs:174-176) and
+ * attention: an optional norm of every head and the rotation by position, in one
+ * pass.  For each token and head, over d elements:
+ *   n = w x / sqrt(mean x^2 + eps)  (n = x where w_q and w_k are NULL)
+ *   pair i < rot / 2 of n turned by positions[token] * f_i and scaled by `scale`:
+ *   elements (i, i + rot / 2), or (2 i, 2 i + 1) if interleaved
+ * and elements from rot on as they are in n.  turns[i] is f_i as turns a position
+ * in units of 2^-64 (modulo 2^64): the angle is exact at every 64-bit position.
+ * q and k are bf16 or fp32 with hq and hk heads (hk = 0: no keys, k NULL), w_q and
+ * w_k fp32 [d], both or neither.  `strides` is a host array of the distances, in
+ * elements, of tokens and of heads: {q token, q head, k token, k head, q_out token,
+ * q_out head, k_out token, k_out head}; a head's elements are adjacent.  An output
+ * may be its input, with the same strides; else it must not overlap any input.
+ * Requires even d <= 1024, even rot in 2 .. d, up to 4096 heads each, m <= 2^32.
+ * ------------------------------------------------------------------------- */
+int32_t nf4s_rotary_fwd(const void *q, const void *k, int32_t is_bf16, int64_t m, int64_t hq,
+                        int64_t hk, int64_t d, const int64_t *strides, const float *w_q,
+                        const float *w_k, float eps, const int64_t *positions,
+                        const int64_t *turns, int64_t rot, int32_t interleaved, float scale,
+                        void *q_out, void *k_out, void *stream);
+/*
+ * Gradients: dq and dk of the results become dq_out and dk_out of q and k.  With
+ * norms q and k are the forward's inputs, and dw_q and dw_k (fp32 [d]) get the
+ * weights' gradients, summed in a fixed order; without, q, k, dw_q and dw_k are
+ * NULL.  strides: {dq, dk, q, k, dq_out, dk_out} x {token, head}.  dq_out may be dq
+ * or q, dk_out dk or k, with the same strides.
+ */
+int32_t nf4s_rotary_bwd(const void *dq, const void *dk, const void *q, const void *k,
+                        int32_t is_bf16, int64_t m, int64_t hq, int64_t hk, int64_t d,
+                        const int64_t *strides, const float *w_q, const float *w_k, float eps,
+                        const int64_t *positions, const int64_t *turns, int64_t rot,
+                        int32_t interleaved, float scale, void *dq_out, void *dk_out, float *dw_q,
+                        float *dw_k, void *workspace, int64_t workspace_bytes, void *stream);
+/* Workspace bytes of the gradients with norms (without: none is needed).  Calls
+ * that share a workspace must not overlap. */
+int32_t nf4s_rotary_bwd_workspace_size(int64_t m, int64_t hq, int64_t hk, int64_t d,
+                                       int64_t *bytes);
+
+/* ---------------------------------------------------------------------------
  * Cross entropy of a linear head, without keeping the logits z = x . w^T:
  *   lse[i] = log sum_c exp z[i, c],  loss[i] = lse[i] - z[i, targets[i]]
  * x [m, d] and w [v, d] bf16 row-major, targets int64 [m], loss and lse fp32

@@ -196,6 +196,20 @@ extern "C" {
     pub fn nf4s_ckpt8_decode_norm(codes: *const u8, scales: *const f32, w: *const f32, m: i64,
                                   d: i64, eps: f32, x: *mut f32, y: *mut u16, rms: *mut f32,
                                   stream: *mut c_void) -> i32;
+    pub fn nf4s_rotary_fwd(q: *const c_void, k: *const c_void, is_bf16: i32, m: i64, hq: i64,
+                           hk: i64, d: i64, strides: *const i64, w_q: *const f32,
+                           w_k: *const f32, eps: f32, positions: *const i64, turns: *const i64,
+                           rot: i64, interleaved: i32, scale: f32, q_out: *mut c_void,
+                           k_out: *mut c_void, stream: *mut c_void) -> i32;
+    pub fn nf4s_rotary_bwd(dq: *const c_void, dk: *const c_void, q: *const c_void,
+                           k: *const c_void, is_bf16: i32, m: i64, hq: i64, hk: i64, d: i64,
+                           strides: *const i64, w_q: *const f32, w_k: *const f32, eps: f32,
+                           positions: *const i64, turns: *const i64, rot: i64, interleaved: i32,
+                           scale: f32, dq_out: *mut c_void, dk_out: *mut c_void, dw_q: *mut f32,
+                           dw_k: *mut f32, workspace: *mut c_void, workspace_bytes: i64,
+                           stream: *mut c_void) -> i32;
+    pub fn nf4s_rotary_bwd_workspace_size(m: i64, hq: i64, hk: i64, d: i64, bytes: *mut i64)
+                                          -> i32;
     pub fn nf4s_linear_ce_fwd(x: *const u16, w: *const u16, targets: *const i64, m: i64, v: i64,
                               d: i64, ignore_index: i64, loss: *mut f32, lse: *mut f32,
                               workspace: *mut c_void, workspace_bytes: i64,
