@@ -139,6 +139,8 @@ SIGNATURES = {
     "nf4s_rotary_bwd": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _F32, _P,
                                _P, _I64, _I32, _F32, _P, _P, _P, _P, _P, _I64, _P]),
     "nf4s_rotary_bwd_workspace_size": (_I32, [_I64, _I64, _I64, _I64, ctypes.POINTER(_I64)]),
+    "nf4s_adamw_step": (_I32, [_P, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "nf4s_adamw_moments": (_I32, [_P, _P, _P, _P, _I64, _P, _P, _P]),
     "nf4s_linear_ce_fwd": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
     "nf4s_linear_ce_bwd": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I32, _I32,
                                   _P, _I64, _P]),

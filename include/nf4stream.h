@@ -446,6 +446,39 @@ int32_t nf4s_rotary_bwd_workspace_size(int64_t m, int64_t hq, int64_t hk, int64_
                                        int64_t *bytes);
 
 /* ---------------------------------------------------------------------------
+ * An AdamW step over `count` tensors at once (the reference steps them one by one,
+ * galore/kernels/quantize_state.cu:7-98).  `params`, `grads`, `copies` (NULL, or
+ * with NULL entries), `sizes` (elements) and `types` are host arrays; types[i] is 1
+ * for a bf16 parameter plus 2 for a bf16 gradient, fp32 otherwise.  copies[i] gets
+ * the updated fp32 parameter in bf16.  In fp32, for every element:
+ *   g = grad * grad_scale[0]                       (device; NULL: 1)
+ *   m = hyper[0] m + hyper[1] g                    beta1, 1 - beta1
+ *   v = hyper[2] v + hyper[3] g g                  beta2, 1 - beta2
+ *   p = p hyper[4] - m / (sqrt(v) hyper[6] + hyper[7]) hyper[5]
+ * with hyper[4] = 1 - lr wd, hyper[5] = lr / (1 - beta1^t), hyper[6] =
+ * 1 / sqrt(1 - beta2^t), hyper[7] = eps: 8 floats of the host, or of the device in
+ * device_hyper, which is read by the kernel (a captured step follows it).
+ * Tensor i's moments begin at element 128 * sum of ceil(sizes[j] / 128), j < i, of m
+ * and v.  They are fp32 (m_scale and v_scale NULL), or 8-bit codes with one fp32
+ * scale for each 128 elements, the largest |m| and sqrt(v) of them (2^-126 at
+ * least): x is held as the magnitude
+ *   (bits(|x| / scale + 2^-15) - bits(2^-15)) >> s,  to nearest, ties to even,
+ * m with s = 20 in a signed byte, sqrt(v) with s = 19, at least 1 unless v is 0.  A
+ * block with an infinity or a NaN has a NaN scale.  The step uses m and v before
+ * they are rounded.
+ * m and v 16-byte aligned, the tensors to their elements; what is written must not
+ * overlap.
+ * ------------------------------------------------------------------------- */
+int32_t nf4s_adamw_step(void *const *params, const void *const *grads, uint16_t *const *copies,
+                        const int64_t *sizes, const int32_t *types, int32_t count, void *m,
+                        void *v, float *m_scale, float *v_scale, const float *hyper,
+                        const float *device_hyper, const float *grad_scale, void *stream);
+/* What `blocks` blocks of 8-bit moments stand for, in fp32 [128 blocks] each. */
+int32_t nf4s_adamw_moments(const uint8_t *m, const uint8_t *v, const float *m_scale,
+                           const float *v_scale, int64_t blocks, float *m_out, float *v_out,
+                           void *stream);
+
+/* ---------------------------------------------------------------------------
  * Cross entropy of a linear head, without keeping the logits z = x . w^T:
  *   lse[i] = log sum_c exp z[i, c],  loss[i] = lse[i] - z[i, targets[i]]
  * x [m, d] and w [v, d] bf16 row-major, targets int64 [m], loss and lse fp32

@@ -210,6 +210,14 @@ extern "C" {
                            stream: *mut c_void) -> i32;
     pub fn nf4s_rotary_bwd_workspace_size(m: i64, hq: i64, hk: i64, d: i64, bytes: *mut i64)
                                           -> i32;
+    pub fn nf4s_adamw_step(params: *const *mut c_void, grads: *const *const c_void,
+                           copies: *const *mut u16, sizes: *const i64, types: *const i32,
+                           count: i32, m: *mut c_void, v: *mut c_void, m_scale: *mut f32,
+                           v_scale: *mut f32, hyper: *const f32, device_hyper: *const f32,
+                           grad_scale: *const f32, stream: *mut c_void) -> i32;
+    pub fn nf4s_adamw_moments(m: *const u8, v: *const u8, m_scale: *const f32,
+                              v_scale: *const f32, blocks: i64, m_out: *mut f32,
+                              v_out: *mut f32, stream: *mut c_void) -> i32;
     pub fn nf4s_linear_ce_fwd(x: *const u16, w: *const u16, targets: *const i64, m: i64, v: i64,
                               d: i64, ignore_index: i64, loss: *mut f32, lse: *mut f32,
                               workspace: *mut c_void, workspace_bytes: i64,
