@@ -42,26 +42,15 @@
 // x 8192 (18.6).
 #include <cmath>
 
-#include "bf16_gemm_core.hpp"
+#include "linear_head.hpp"
 
 namespace nf4s {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // G of a piece: what the Infinity Cache (256 MB) holds between the kernel that
 // writes it and the two that read it.  Gradients of 8192 x 32000 x 4096: 4813 us
 // with 256 MB, 4941 with half, 4772 with four times as much; of 4096 x 128000 x
 // 8192 18.9, 19.1 and 18.6 ms.
 constexpr int64_t kCePieceBytes = (int64_t)256 << 20;
-// Tokens of one forward launch, which bounds its partial sums.
-constexpr int64_t kCeTokens = 16384;
-// A launch counts its threads in 32 bits.
-constexpr int64_t kMaxTiles = 0xffffffffll / kGcThreads;
-
-// Maximum and sum of exponentials of part of a token's logits.
-typedef float floatx2 __attribute__((ext_vector_type(2)));
-
 struct CeLogits {
   const uint16_t *x, *w;  // w at the piece's first row
   const int64_t *targets;
@@ -79,22 +68,6 @@ struct CeLogits {
   uint16_t *g;       // [M, ldg]
   int64_t ldg, gcols;  // row length of G, columns of it from g on
 };
-
-// The largest, or the sum, over the four lanes l % 16 + 16 g that hold a token's
-// columns, in each of them.
-template <class F>
-__device__ __forceinline__ float over_groups(float v, F &&f) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, v);
-  const auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-  v = f(__builtin_bit_cast(float, (uint32_t)s[0]), __builtin_bit_cast(float, (uint32_t)s[1]));
-  const uint32_t c = __builtin_bit_cast(uint32_t, v);
-  const auto t = __builtin_amdgcn_permlane32_swap(c, c, false, false);
-  return f(__builtin_bit_cast(float, (uint32_t)t[0]), __builtin_bit_cast(float, (uint32_t)t[1]));
-}
-
-__device__ __forceinline__ float exp_of(float x) {
-  return __builtin_amdgcn_exp2f(x * kLog2e);
-}
 
 // Column of the wave's block (0 .. 32 kNT - 1) of the lane's register i of column
 // tile nt is 16 nt + 4 (lane / 16) + i, its token of row tile mt 16 mt + lane % 16.
@@ -346,18 +319,6 @@ __global__ void ce_zero_kernel(T *p, int64_t n) {
 
 constexpr int64_t kCeFewTokens = 128;
 
-// Tile columns of a strip (gc_tile): 4096 x 32000 x 8192 forward 1520 us with 4,
-// 1549 with 6, 1577 with 8, 1666 with 16.
-constexpr int kCeStrip = 4;
-
-static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-
-// A logits launch: 64 mt x 64 nt tiles over the next `cols` columns.
-struct CeLaunch {
-  int mt, nt;
-  int64_t cols;
-};
-
 // The tiles of m > 0 tokens by v > 0 columns of length d, as one launch, or as
 // whole rounds of large tiles and the rest in smaller ones.  Cost of a launch in
 // us: each round takes, per step of 64, `lo` when few tiles run to `hi` when the
@@ -382,8 +343,6 @@ struct CeTile {
 constexpr CeTile kCeTiles[3] = {{1, 2, 2, 0.21, 0.74, 6.9}, {2, 4, 1, 0.98, 0.99, 6.8},
                                 {4, 4, 1, 1.23, 1.51, 5.3}};
 
-static int64_t ceil_to(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 static double ce_cost(const CeTile &c, int64_t m, int64_t v, int64_t d) {
   const int64_t tl = ceil_to(m, 64 * c.mt), T = tl * ceil_to(v, 64 * c.nt);
   const int64_t slots = (int64_t)cu_slots() * c.slots;
@@ -395,7 +354,7 @@ static double ce_cost(const CeTile &c, int64_t m, int64_t v, int64_t d) {
   return 8.0 + (compute > memory ? compute : memory);
 }
 
-static int ce_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&out)[2]) {
+int ce_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&out)[2]) {
   double best = HUGE_VAL;
   int count = 0;
   auto smallest = [&](int64_t cols, int upto, const CeTile *&c) {
@@ -431,22 +390,13 @@ static int ce_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&out)[2]) {
 }
 
 // Partial sums a token leaves: one for each half tile.
-static int64_t ce_slices(int64_t m, int64_t v, int64_t d) {
+int64_t ce_slices(int64_t m, int64_t v, int64_t d) {
   CeLaunch l[2];
   const int n = ce_tiles(m, v, d, l);
   int64_t s = 0;
   for (int i = 0; i < n; ++i) s += 2 * ceil_to(l[i].cols, 64 * l[i].nt);
   return s;
 }
-
-struct CePlan {
-  int64_t tokens;        // forward: tokens of one launch
-  int64_t part_bytes, fwd_bytes;
-  int64_t piece, ldg;    // backward: columns of a piece, row length of G
-  int dx_mt;
-  int64_t slices, slice; // of dx's reduction over a piece
-  int64_t g_bytes, bwd_bytes;
-};
 
 // Tile height of dx and slices of its reduction over a piece, by the least of:
 // the rounds' time, as for the logits, joined with that of reading w by their
@@ -488,7 +438,7 @@ static void ce_dx_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
   p.slices = ceil_to(p.ldg, p.slice);
 }
 
-static int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
+int32_t ce_plan(int64_t m, int64_t v, int64_t d, CePlan &p) {
   if (m < 0 || v <= 0 || d <= 0)
     return fail(NF4S_ERR_INVALID_ARGUMENT, "bad cross-entropy shape m=%lld v=%lld d=%lld",
                 (long long)m, (long long)v, (long long)d);
@@ -582,7 +532,75 @@ static int32_t ce_dw_piece(const CeProduct &a, hipStream_t s) {
                              : ce_product<4, 4, true, kOut>(a, s);
 }
 
-static int32_t ce_operands(const uint16_t *x, const uint16_t *w, const int64_t *targets, int64_t m,
+// The gradients from G: dx += G . w and the rows of dw = G^T . x piece by piece.
+int32_t head_gradients(const HeadGrad &h, const CePlan &p, HeadLogits logits, const void *ctx,
+                       hipStream_t s) {
+  uint16_t *g = static_cast<uint16_t *>(h.workspace);
+  float *part = reinterpret_cast<float *>(static_cast<char *>(h.workspace) + p.g_bytes);
+  const float *common = head_common(h, p);
+  for (int64_t v0 = 0; v0 < h.v; v0 += p.piece) {
+    const int64_t vn = h.v - v0 < p.piece ? h.v - v0 : p.piece;
+    int32_t rc = logits(ctx, HeadPiece{v0, vn, g, p.ldg, common, s});
+    if (rc != NF4S_OK) return rc;
+    CeProduct b{};  // dx += G . w
+    b.l = g;
+    b.ldl = p.ldg;
+    b.r = h.w + v0 * h.d;
+    b.ldr = h.d;
+    b.rows = h.m;
+    b.cols = h.d;
+    b.k = vn;
+    b.slice = p.slice;
+    b.out = part;
+    b.ld = h.d;
+    b.slice_stride = h.m * h.d;
+    rc = v0 == 0 ? ce_dx_piece<kOutF32>(p, b, s) : ce_dx_piece<kOutF32Add>(p, b, s);
+    if (rc != NF4S_OK) return rc;
+    CeProduct c{};  // the piece's rows of dw = G^T . x
+    c.l = g;
+    c.ldl = p.ldg;
+    c.r = h.x;
+    c.ldr = h.d;
+    c.rows = vn;
+    c.cols = h.d;
+    c.k = h.m;
+    c.slice = up(h.m, kGcStep);
+    c.out = h.dw_is_f32 ? static_cast<void *>(static_cast<float *>(h.dw) + v0 * h.d)
+                        : static_cast<void *>(static_cast<uint16_t *>(h.dw) + v0 * h.d);
+    c.ld = h.d;
+    c.common = common;
+    rc = h.accumulate  ? ce_dw_piece<kOutF32Add>(c, s)
+         : h.dw_is_f32 ? ce_dw_piece<kOutF32>(c, s)
+                       : ce_dw_piece<kOutBf16>(c, s);
+    if (rc != NF4S_OK) return rc;
+  }
+  const int64_t chunks = h.m * h.d / 4;
+  const int64_t blocks = (chunks + 255) / 256;
+  hipLaunchKernelGGL(ce_dx_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0,
+                     s, reinterpret_cast<const floatx4 *>(part), (int32_t)p.slices, chunks,
+                     common, reinterpret_cast<u32x2 *>(h.dx));
+  return check_launch("ce_dx_kernel");
+}
+
+int32_t head_zero_dw(void *dw, bool f32, int64_t n, hipStream_t s) {
+  hipLaunchKernelGGL(ce_zero_kernel<uint32_t>, dim3(4096), dim3(256), 0, s,
+                     static_cast<uint32_t *>(dw), f32 ? n : n / 2);
+  return check_launch("ce_zero_kernel");
+}
+
+// G of a piece of the cross entropy.
+static int32_t ce_grad_logits(const void *ctx, const HeadPiece &p) {
+  CeLogits a = *static_cast<const CeLogits *>(ctx);
+  a.w += p.v0 * a.d;
+  a.v0 = p.v0;
+  a.vn = (int32_t)p.vn;
+  a.common = p.common;
+  a.g = p.g;
+  a.ldg = a.gcols = p.ldg;
+  return ce_logits<true>(a, nullptr, p.stream);
+}
+
+int32_t ce_operands(const uint16_t *x, const uint16_t *w, const int64_t *targets, int64_t m,
                            void *workspace, int64_t workspace_bytes, int64_t need) {
   if (w == nullptr || (m > 0 && (x == nullptr || targets == nullptr)))
     return fail(NF4S_ERR_INVALID_ARGUMENT, "NULL buffer");
@@ -670,77 +688,23 @@ int32_t nf4s_linear_ce_bwd(const uint16_t *x, const uint16_t *w, const int64_t *
   if (!aligned(dw, 16) || (m > 0 && (!aligned(dx, 16) || !aligned(lse, 4) || !aligned(dloss, 4))))
     return fail(NF4S_ERR_MISALIGNED, "dx and dw must be 16-byte aligned, lse and dloss 4-byte");
   const hipStream_t s = as_stream(stream);
-  if (m == 0) {
-    if (accumulate) return NF4S_OK;
-    const int64_t n = dw_is_f32 ? v * d : v * d / 2;  // 32-bit words
-    hipLaunchKernelGGL(ce_zero_kernel<uint32_t>, dim3(4096), dim3(256), 0, s,
-                       static_cast<uint32_t *>(dw), n);
-    return check_launch("ce_zero_kernel");
-  }
-  uint16_t *g = static_cast<uint16_t *>(workspace);
-  float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.g_bytes);
-  float *common = part + p.slices * m * d;
+  if (m == 0) return accumulate ? NF4S_OK : head_zero_dw(dw, dw_is_f32 != 0, v * d, s);
+  const HeadGrad h{x, w, m, v, d, dx, dw, dw_is_f32 != 0, accumulate != 0, workspace};
   hipLaunchKernelGGL(ce_common_kernel, dim3(1), dim3(1024), 0, s, dloss, targets, ignore_index, m,
-                     common);
+                     head_common(h, p));
   rc = check_launch("ce_common_kernel");
   if (rc != NF4S_OK) return rc;
-  for (int64_t v0 = 0; v0 < v; v0 += p.piece) {
-    const int64_t vn = v - v0 < p.piece ? v - v0 : p.piece;
-    CeLogits a{};
-    a.x = x;
-    a.w = w + v0 * d;
-    a.targets = targets;
-    a.M = m;
-    a.d = d;
-    a.v0 = v0;
-    a.vn = (int32_t)vn;
-    a.V = v;
-    a.ignore = ignore_index;
-    a.lse = lse;
-    a.dloss = dloss;
-    a.common = common;
-    a.g = g;
-    a.ldg = a.gcols = p.ldg;
-    rc = ce_logits<true>(a, nullptr, s);
-    if (rc != NF4S_OK) return rc;
-    CeProduct b{};  // dx += G . w
-    b.l = g;
-    b.ldl = p.ldg;
-    b.r = w + v0 * d;
-    b.ldr = d;
-    b.rows = m;
-    b.cols = d;
-    b.k = vn;
-    b.slice = p.slice;
-    b.out = part;
-    b.ld = d;
-    b.slice_stride = m * d;
-    rc = v0 == 0 ? ce_dx_piece<kOutF32>(p, b, s) : ce_dx_piece<kOutF32Add>(p, b, s);
-    if (rc != NF4S_OK) return rc;
-    CeProduct c{};  // the piece's rows of dw = G^T . x
-    c.l = g;
-    c.ldl = p.ldg;
-    c.r = x;
-    c.ldr = d;
-    c.rows = vn;
-    c.cols = d;
-    c.k = m;
-    c.slice = up(m, kGcStep);
-    c.out = dw_is_f32 ? static_cast<void *>(static_cast<float *>(dw) + v0 * d)
-                      : static_cast<void *>(static_cast<uint16_t *>(dw) + v0 * d);
-    c.ld = d;
-    c.common = common;
-    rc = accumulate  ? ce_dw_piece<kOutF32Add>(c, s)
-         : dw_is_f32 ? ce_dw_piece<kOutF32>(c, s)
-                     : ce_dw_piece<kOutBf16>(c, s);
-    if (rc != NF4S_OK) return rc;
-  }
-  const int64_t chunks = m * d / 4;
-  const int64_t blocks = (chunks + 255) / 256;
-  hipLaunchKernelGGL(ce_dx_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0,
-                     s, reinterpret_cast<const floatx4 *>(part), (int32_t)p.slices, chunks,
-                     common, reinterpret_cast<u32x2 *>(dx));
-  return check_launch("ce_dx_kernel");
+  CeLogits a{};
+  a.x = x;
+  a.w = w;
+  a.targets = targets;
+  a.M = m;
+  a.d = d;
+  a.V = v;
+  a.ignore = ignore_index;
+  a.lse = lse;
+  a.dloss = dloss;
+  return head_gradients(h, p, ce_grad_logits, &a, s);
 }
 
 }  // extern "C"

@@ -1,0 +1,709 @@
+// linear_logprob.hip - log probabilities of given tokens under a linear head, the
+// entropy of each token's distribution and its most likely alternatives, with the
+// gradients of the first two, without keeping the logits, for gfx950 (MI355X).
+//
+// x [M, d] and w [V, d] bf16 (the head of doublepass/src/loss.rs and
+// doublepass/kernels/fused_ce.cu:71-207, whose cross entropy is linear_ce.hip's):
+//   z = x . w^T,  L = log sum_c exp z_c,  logp = z_t - L,  l_c = z_c - L
+//   H = -sum_c exp(l_c) l_c
+//   top k: the k largest z_c, equal ones by their index, with their l_c
+//   G_c = ([c = t] a - exp(l_c) (a + h (l_c + H))) / C,  a = dlogp, h = dH,
+//   dx = C G . w,  dw = C G^T . x
+// C is the largest |a| (of |h| if there is none), kept out of the bf16 G as in the
+// cross entropy.  Products accumulate in fp32; maxima, sums and results are fp32.
+//
+// Forward: the tiles of the cross entropy, a lane holding one token's columns.  A
+// half tile leaves its maximum, its sum of exponentials and the sum of e y with y =
+// (z - maximum) log2(e) <= 0, terms of one sign, so that
+//   H = log S - ln 2 T / S
+// loses nothing to cancellation.
+// Alternatives: the k largest logits of a token lie in the k half tiles of largest
+// maximum (earlier ones first among equals): any other one has k logits before all
+// of its own.  So the logits of the present piece of the vocabulary are stored in
+// fp32, but for half tiles whose maximum does not exceed the k-th best of the pieces
+// before, and one wave a token picks half tiles by their maxima and reads k of
+// them.  Later columns lose a tie, so what is skipped is never needed.
+#include "linear_head.hpp"
+
+namespace nf4s {
+
+constexpr int kLpTop = 32;  // alternatives at most
+// Stored logits of a piece: what the Infinity Cache holds between the two kernels.
+constexpr int64_t kLpPieceBytes = (int64_t)256 << 20;
+// Columns of a piece, whose maxima (of 64 at least) a wave holds in LDS: 16 KB.
+constexpr int64_t kLpPieceCols = 1 << 18;
+constexpr int64_t kLpSelectLds = 64 << 10;
+constexpr int kLpWidth = 128;  // columns of a half tile at most
+
+struct LpLogits {
+  const uint16_t *x, *w;  // w at the launch's first row
+  const int64_t *targets;
+  int64_t M, d;
+  int64_t v0;   // first column of the launch
+  int32_t vn;   // its columns
+  int64_t V, ignore;
+  int32_t tiles_l, tiles_r;
+  // forward
+  floatx2 *part;  // [2 tiles_r][M] maximum, sum
+  float *ent;     // [2 tiles_r][M] sum of e y
+  float *zt;      // [M] logit of the target
+  float *z;       // [2 tiles_r][M][32 kNT] logits, or NULL
+  const uint64_t *best;  // [M][k] of the pieces before, or NULL
+  int32_t k;
+  // backward
+  const float *lse, *entropy, *dlogp, *dentropy;  // entropy, dentropy: NULL if none
+  const float *common;
+  uint16_t *g;
+  int64_t ldg, gcols;
+};
+
+// fp32 values in the order of unsigned integers from 1 on (NaN last); 0: none.
+__device__ __forceinline__ uint32_t lp_order(float v) {
+  const float u = v + 0.0f;  // -0 as 0
+  const uint32_t b = u != u ? 0x7fc00000u : __builtin_bit_cast(uint32_t, u);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float lp_value(uint32_t o) {
+  return __builtin_bit_cast(float, o ^ (o >> 31 != 0 ? 0x80000000u : 0xffffffffu));
+}
+// Larger values first, then smaller columns.
+__device__ __forceinline__ uint64_t lp_key(uint32_t order, uint32_t column) {
+  return order == 0 ? 0 : (uint64_t)order << 32 | (uint32_t)~column;
+}
+// At least -1e4, where exp2 is 0; NaN stays.
+__device__ __forceinline__ float lp_floor(float y) { return y < -1e4f ? -1e4f : y; }
+
+template <int kMT, int kNT, bool kGrad>
+__global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) lp_logits_kernel(const LpLogits a) {
+  using Core = GcCore<kMT, kNT, false, false>;
+  __shared__ __attribute__((aligned(16))) char lds[Core::kLdsBytes];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int lane = threadIdx.x & 63;
+  int tl, tr;
+  gc_tile(blockIdx.x, a.tiles_l, a.tiles_r, kCeStrip, tl, tr);
+  const int64_t l0 = (int64_t)tl * Core::kTileL;
+  const int r0 = tr * Core::kTileR;
+  const int64_t lrows = a.M - l0 < Core::kTileL ? a.M - l0 : Core::kTileL;
+  const int rrows = a.vn - r0 < Core::kTileR ? a.vn - r0 : Core::kTileR;
+  Core core;
+  core.run(gc_along(a.x + l0 * a.d, a.d, lrows, a.d),
+           gc_along(a.w + (int64_t)r0 * a.d, a.d, rrows, a.d), a.d, lds, lane, wave);
+
+  // Columns and tokens of a lane: as in ce_logits_kernel.
+  const int64_t row0 = l0 + 32 * kMT * (wave >> 1);
+  const int c0 = 32 * kNT * (wave & 1);
+  const int cols = rrows - c0;
+#pragma unroll
+  for (int mt = 0; mt < 2 * kMT; ++mt) {
+    // One block of 16 tokens at a time: interleaved, the blocks spill.
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "+v"(lane));
+    floatx4 (&z)[2 * kNT] = core.acc[mt];
+    const int grp = lane >> 4;
+    if (cols < 32 * kNT) {  // columns past the vocabulary
+#pragma unroll
+      for (int nt = 0; nt < 2 * kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * nt + 4 * grp + i >= cols) z[nt][i] = -__builtin_inff();
+    }
+    const int64_t row = row0 + 16 * mt + (lane & 15);
+    const bool here = row < a.M;
+    const int64_t t = here ? a.targets[row] : a.ignore;
+    // The target's register among this lane's, or -1.
+    const int64_t rel = t - (a.v0 + r0 + c0);
+    const bool mine = t != a.ignore && rel >= 0 && rel < 32 * kNT && rel < cols &&
+                      (((int)rel >> 2) & 3) == grp;
+    const int at = mine ? 4 * ((int)rel >> 4) + ((int)rel & 3) : -1;
+    if constexpr (!kGrad) {
+      if (__ballot(mine) != 0) {
+        float zt = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < 2 * kNT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) zt = at == 4 * nt + i ? z[nt][i] : zt;
+        if (mine) a.zt[row] = zt;
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int nt = 0; nt < 2 * kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, z[nt][i]);
+      top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
+      const int64_t slice = (int64_t)(2 * tr + (wave & 1)) * a.M + row;
+      if (a.z != nullptr) {
+        const bool keep =
+            here && (a.best == nullptr ||
+                     lp_order(top) > (uint32_t)(a.best[row * a.k + a.k - 1] >> 32));
+        if (__ballot(keep) != 0 && keep) {
+          float *out = a.z + slice * (32 * kNT) + 4 * grp;
+#pragma unroll
+          for (int nt = 0; nt < 2 * kNT; ++nt)
+            *reinterpret_cast<floatx4 *>(out + 16 * nt) = z[nt];
+        }
+      }
+      // Nothing but -inf: any finite reference gives a sum of 0.
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
+      float sum = 0.0f, ent = 0.0f;
+#pragma unroll
+      for (int nt = 0; nt < 2 * kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = lp_floor((z[nt][i] - ref) * kLog2e);
+          const float e = __builtin_amdgcn_exp2f(y);
+          sum += e;
+          ent += e * y;
+        }
+      sum = over_groups(sum, [](float x, float y) { return x + y; });
+      ent = over_groups(ent, [](float x, float y) { return x + y; });
+      if (here && grp == 0) {
+        a.part[slice] = (floatx2){top, sum};
+        a.ent[slice] = ent;
+      }
+    } else {
+      const float lse = here ? a.lse[row] : 0.0f;
+      const bool given = t != a.ignore;
+      float da = here && given ? a.dlogp[row] / *a.common : 0.0f;
+      const float dh = here && a.dentropy != nullptr ? a.dentropy[row] / *a.common : 0.0f;
+      const bool none = da == 0.0f && dh == 0.0f;
+      if (given && (t < 0 || t >= a.V)) da = __builtin_nanf("");
+      const float base = dh == 0.0f ? da : da + dh * a.entropy[row];
+#pragma unroll
+      for (int nt = 0; nt < 2 * kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // Past -1e4 the exponential is zero whatever is behind it.
+          const float l = lp_floor(z[nt][i] - lse);
+          z[nt][i] = -exp_of(l) * (base + dh * l);
+        }
+      if (__ballot(mine) != 0) {
+#pragma unroll
+        for (int nt = 0; nt < 2 * kNT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z[nt][i] += at == 4 * nt + i ? da : 0.0f;
+      }
+      // A token without a gradient has none, whatever its logits are.
+#pragma unroll
+      for (int nt = 0; nt < 2 * kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[nt][i] = none ? 0.0f : fp32_rounded(z[nt][i]);
+      // Columns of the piece's last, partial 64 hold zeros: G is read in steps of 64.
+      if (mt % 2 == 1) {
+        const int64_t first = row0 + 16 * (mt - 1);
+        gc_store_bf16<kNT, false>(
+            [&](int h, int nt, int i) { return core.acc[mt - 1 + h][nt][i]; },
+            lds + 32 * 64 * kNT * wave, a.g + first * a.ldg + r0 + c0, a.ldg, a.M - first,
+            a.gcols - (r0 + c0), lane);
+      }
+    }
+  }
+}
+
+// The largest of a 64-bit key over the wave, in every lane.
+template <int kCtrl>
+__device__ __forceinline__ uint64_t dpp_max64(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kCtrl, 0xf, 0xf,
+                                                            true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), kCtrl, 0xf,
+                                                            0xf, true);
+  const uint64_t o = (uint64_t)hi << 32 | lo;
+  return o > v ? o : v;
+}
+__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
+  v = dpp_max64<0x128>(v);  // row_ror:8
+  v = dpp_max64<0x124>(v);
+  v = dpp_max64<0x122>(v);
+  v = dpp_max64<0x121>(v);
+  const auto l16 = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  const auto h16 =
+      __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  uint64_t a = (uint64_t)h16[0] << 32 | l16[0], b = (uint64_t)h16[1] << 32 | l16[1];
+  v = a > b ? a : b;
+  const auto l32 = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  const auto h32 =
+      __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  a = (uint64_t)h32[0] << 32 | l32[0];
+  b = (uint64_t)h32[1] << 32 | l32[1];
+  return a > b ? a : b;
+}
+
+// Half tiles of one launch of a piece.
+struct LpSegment {
+  int32_t slices, width;
+  int64_t column, columns;  // first one, and how many there are
+  const floatx2 *part;      // [slices][M]
+  const float *z;           // [slices][M][width]
+};
+
+struct LpSelect {
+  LpSegment seg[2];
+  int64_t M;
+  int32_t k, slices;  // of both segments
+  bool first;         // no pieces before
+  uint64_t *best;     // [M][k]
+};
+
+// One wave a token: k half tiles by their maxima, then the k best of their logits
+// and of the pieces before.  LDS: the maxima, the chosen ones' logits, both as
+// ordered integers, a lane's own every 64th.
+__global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
+  extern __shared__ uint32_t lp_lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
+  if (row >= a.M) return;
+  const int rounds = (a.slices + 63) / 64;
+  uint32_t *maxima = lp_lds + wave * (64 * rounds + a.k * (kLpWidth + 1));
+  uint32_t *logits = maxima + 64 * rounds;
+  int32_t *chosen = reinterpret_cast<int32_t *>(logits + a.k * kLpWidth);
+  uint64_t *best = a.best + row * a.k;
+  const uint32_t least = a.first ? 0 : (uint32_t)(best[a.k - 1] >> 32);
+
+  // A half tile is a candidate if its maximum exceeds the k-th best.
+  uint64_t own = 0;
+  for (int i = 0; i < rounds; ++i) {
+    const int s = 64 * i + lane;
+    uint32_t o = 0;
+    if (s < a.slices) {
+      const bool second = s >= a.seg[0].slices;
+      const floatx2 *p = second ? a.seg[1].part + (int64_t)(s - a.seg[0].slices) * a.M
+                                : a.seg[0].part + (int64_t)s * a.M;
+      o = lp_order(p[row].x);
+      if (o <= least) o = 0;
+    }
+    maxima[s] = o;
+    const uint64_t key = lp_key(o, (uint32_t)s);
+    own = key > own ? key : own;
+  }
+  int count = 0;
+  for (; count < a.k; ++count) {
+    const uint64_t top = wave_max64(own);
+    if (top == 0) break;
+    const int s = (int)~(uint32_t)top;
+    if (lane == 0) chosen[count] = s;
+    if (own == top) {
+      maxima[s] = 0;
+      own = 0;
+      for (int i = 0; i < rounds; ++i) {
+        const uint64_t key = lp_key(maxima[64 * i + lane], (uint32_t)(64 * i + lane));
+        own = key > own ? key : own;
+      }
+    }
+  }
+  if (count == 0) return;  // the pieces before had all
+
+  // Two logits a lane of every chosen half tile.
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  auto column = [&](int j, int h, bool &in) {
+    const int s = chosen[j];
+    const LpSegment &g = s >= a.seg[0].slices ? a.seg[1] : a.seg[0];
+    const int at = s >= a.seg[0].slices ? s - a.seg[0].slices : s;
+    const int64_t c = (int64_t)at * g.width + 64 * h + lane;
+    in = 64 * h + lane < g.width && c < g.columns;
+    return (uint32_t)(g.column + c);
+  };
+  own = 0;
+  for (int j = 0; j < count; ++j) {
+    const int s = chosen[j];
+    const bool second = s >= a.seg[0].slices;
+    const int width = second ? a.seg[1].width : a.seg[0].width;
+    const float *z = second ? a.seg[1].z + ((int64_t)(s - a.seg[0].slices) * a.M + row) * width
+                            : a.seg[0].z + ((int64_t)s * a.M + row) * width;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bool in;
+      const uint32_t c = column(j, h, in);
+      const uint32_t o = in ? lp_order(z[64 * h + lane]) : 0;
+      logits[(2 * j + h) * 64 + lane] = o;
+      const uint64_t key = lp_key(o, c);
+      own = key > own ? key : own;
+    }
+  }
+  uint64_t before = !a.first && lane < a.k ? best[lane] : 0;
+  for (int t = 0; t < a.k; ++t) {
+    const uint64_t top = wave_max64(own > before ? own : before);
+    if (lane == 0) best[t] = top;
+    if (top == 0) continue;
+    if (before == top) {
+      before = 0;
+    } else if (own == top) {
+      own = 0;
+      for (int j = 0; j < 2 * count; ++j) {
+        bool in;
+        const uint32_t c = column(j / 2, j % 2, in);
+        uint32_t o = logits[j * 64 + lane];
+        if (lp_key(o, c) == top) logits[j * 64 + lane] = o = 0;
+        const uint64_t key = lp_key(o, c);
+        own = key > own ? key : own;
+      }
+    }
+  }
+}
+
+struct LpJoin {
+  const floatx2 *part;
+  const float *ent, *zt;
+  const uint64_t *best;
+  const int64_t *targets;
+  int64_t M;
+  int32_t slices, k;
+  int64_t V, ignore;
+  float *logp, *lse, *entropy, *top_logp;
+  int64_t *top_ids;
+};
+
+// Joins a token's partial sums, as ce_join_kernel: 256 / kTokens threads a token take
+// every so many slices, then meet in a fixed order.
+template <int kTokens>
+__global__ void __launch_bounds__(256) lp_join_kernel(const LpJoin a) {
+  constexpr int kGroups = 256 / kTokens;
+  __shared__ float lds[3][kGroups][kTokens];
+  struct Sums {
+    float top, sum, ent;
+  };
+  const int tok = threadIdx.x % kTokens, grp = threadIdx.x / kTokens;
+  const int64_t row = (int64_t)blockIdx.x * kTokens + tok;
+  auto join = [](const Sums &x, const Sums &y) {
+    const float top = fmaxf(x.top, y.top);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    const float dx = lp_floor((x.top - ref) * kLog2e), dy = lp_floor((y.top - ref) * kLog2e);
+    const float ex = __builtin_amdgcn_exp2f(dx), ey = __builtin_amdgcn_exp2f(dy);
+    return Sums{top, x.sum * ex + y.sum * ey,
+                (x.ent + dx * x.sum) * ex + (y.ent + dy * y.sum) * ey};
+  };
+  const Sums none{-__builtin_inff(), 0.0f, 0.0f};
+  Sums s = none;
+  if (row < a.M)
+    for (int i = grp; i < a.slices; i += 4 * kGroups) {
+      Sums v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = i + j * kGroups;
+        v[j] = none;
+        if (n < a.slices) {
+          const floatx2 p = a.part[(int64_t)n * a.M + row];
+          v[j] = Sums{p.x, p.y, a.ent[(int64_t)n * a.M + row]};
+        }
+      }
+      s = join(s, join(join(v[0], v[1]), join(v[2], v[3])));
+    }
+  auto put = [&](const Sums &v) {
+    lds[0][grp][tok] = v.top;
+    lds[1][grp][tok] = v.sum;
+    lds[2][grp][tok] = v.ent;
+  };
+  auto get = [&](int g) { return Sums{lds[0][g][tok], lds[1][g][tok], lds[2][g][tok]}; };
+  put(s);
+#pragma unroll
+  for (int half = kGroups / 2; half >= 1; half /= 2) {
+    __syncthreads();
+    if (grp < half) put(join(get(grp), get(grp + half)));
+  }
+  __syncthreads();
+  if (row >= a.M) return;
+  s = get(0);
+  const float log_sum = __builtin_amdgcn_logf(s.sum) * kLn2;
+  if (grp == 0) {
+    a.lse[row] = s.top + log_sum;
+    a.entropy[row] = log_sum - s.ent / s.sum * kLn2;
+    const int64_t t = a.targets[row];
+    float v = 0.0f;
+    if (t != a.ignore)
+      v = t < 0 || t >= a.V ? __builtin_nanf("") : (a.zt[row] - s.top) - log_sum;
+    a.logp[row] = v;
+  }
+  for (int i = grp; i < a.k; i += kGroups) {
+    const uint64_t key = a.best[row * a.k + i];
+    a.top_ids[row * a.k + i] = (int64_t)(uint32_t)~(uint32_t)key;
+    a.top_logp[row * a.k + i] = (lp_value((uint32_t)(key >> 32)) - s.top) - log_sum;
+  }
+}
+
+// C = max |dlogp| over the tokens that have one, or max |dentropy|, or 1.
+__global__ void __launch_bounds__(1024) lp_common_kernel(const float *dlogp, const float *dentropy,
+                                                         const int64_t *targets, int64_t ignore,
+                                                         int64_t M, float *common) {
+  __shared__ float part[2][16];
+  float top[2] = {0.0f, 0.0f};
+  // A NaN counts as infinite: fmaxf would drop it.
+  auto size = [](float v) { return fabsf(v) < __builtin_inff() ? fabsf(v) : __builtin_inff(); };
+  for (int64_t i = threadIdx.x; i < M; i += 1024) {
+    if (targets[i] != ignore) top[0] = fmaxf(top[0], size(dlogp[i]));
+    if (dentropy != nullptr) top[1] = fmaxf(top[1], size(dentropy[i]));
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top[j] = fmaxf(top[j], __shfl_xor(top[j], off, 64));
+    if ((threadIdx.x & 63) == 0) part[j][threadIdx.x >> 6] = top[j];
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int j = 0; j < 2; ++j)
+    for (int i = 1; i < 16; ++i) top[j] = fmaxf(top[j], part[j][i]);
+  const float c = top[0] > 0.0f ? top[0] : top[1];
+  *common = c == 0.0f || c == __builtin_inff() ? 1.0f : c;
+}
+
+// Where the forward of M tokens keeps what.
+struct LpLayout {
+  int64_t piece;   // columns of a piece of the vocabulary
+  int64_t slices;  // partial sums of a token
+  int64_t ent, zt, best, z, bytes;
+};
+
+static LpLayout lp_layout(int64_t M, int64_t v, int64_t d, int64_t k) {
+  LpLayout l{};
+  l.piece = v;
+  if (k > 0) {
+    // Whole rounds of 256 x 256 tiles, as far as they fit.
+    int64_t cols = kLpPieceBytes / (4 * M);
+    if (cols > kLpPieceCols) cols = kLpPieceCols;
+    const int64_t tl = ceil_to(M, 256), round = cu_slots() > tl ? cu_slots() / tl * 256 : 256;
+    cols = cols >= round ? cols / round * round : cols / 256 * 256;
+    if (cols < 4096) cols = 4096;
+    if (cols < v) l.piece = cols;
+  }
+  int64_t z = 0;
+  for (int64_t v0 = 0; v0 < v; v0 += l.piece) {
+    const int64_t vn = v - v0 < l.piece ? v - v0 : l.piece;
+    // Whole pieces are alike.
+    const int64_t n = vn == l.piece ? v / l.piece : 1;
+    l.slices += n * ce_slices(M, vn, d);
+    CeLaunch t[2];
+    int64_t cols = 0;
+    const int launches = ce_tiles(M, vn, d, t);
+    for (int i = 0; i < launches; ++i) cols += up(t[i].cols, 64 * t[i].nt);
+    if (cols > z) z = cols;
+    v0 += (n - 1) * l.piece;
+  }
+  int64_t at = up(l.slices * M * 8, 256);
+  auto take = [&](int64_t n) {
+    const int64_t from = at;
+    at += up(n, 256);
+    return from;
+  };
+  l.ent = take(l.slices * M * 4);
+  l.zt = take(M * 4);
+  l.best = take(M * k * 8);
+  l.z = take(k > 0 ? z * M * 4 : 0);
+  l.bytes = at;
+  return l;
+}
+
+static int64_t lp_forward_bytes(const CePlan &p, int64_t m, int64_t v, int64_t d, int64_t k) {
+  if (m == 0) return 0;
+  int64_t bytes = lp_layout(p.tokens, v, d, k).bytes;
+  if (m % p.tokens != 0) {
+    const int64_t last = lp_layout(m % p.tokens, v, d, k).bytes;
+    if (last > bytes) bytes = last;
+  }
+  return bytes;
+}
+
+static int32_t lp_plan(int64_t m, int64_t v, int64_t d, int64_t k, CePlan &p) {
+  const int32_t rc = ce_plan(m, v, d, p);
+  if (rc != NF4S_OK) return rc;
+  if (k < 0) return fail(NF4S_ERR_INVALID_ARGUMENT, "negative number of alternatives");
+  if (k > kLpTop || k > v)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "%lld alternatives of %lld tokens: at most %d",
+                (long long)k, (long long)v, kLpTop);
+  return NF4S_OK;
+}
+
+// The logits of a.M tokens and a.vn columns, in one launch or two; with `seg` the
+// launches' half tiles.
+template <bool kGrad>
+static int32_t lp_logits(LpLogits a, int64_t *slices, LpSegment *seg, hipStream_t s) {
+  CeLaunch l[2];
+  const int n = ce_tiles(a.M, a.vn, a.d, l);
+  int64_t done = 0;
+  for (int i = 0; i < n; ++i) {
+    a.vn = (int32_t)l[i].cols;
+    a.tiles_l = (int32_t)ceil_to(a.M, 64 * l[i].mt);
+    a.tiles_r = (int32_t)ceil_to(a.vn, 64 * l[i].nt);
+    auto *kernel = l[i].mt == 4   ? lp_logits_kernel<4, 4, kGrad>
+                   : l[i].mt == 2 ? lp_logits_kernel<2, 4, kGrad>
+                                  : lp_logits_kernel<1, 2, kGrad>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)a.tiles_l * (uint32_t)a.tiles_r), dim3(kGcThreads),
+                       0, s, a);
+    const int32_t rc = check_launch("lp_logits_kernel");
+    if (rc != NF4S_OK) return rc;
+    if (seg != nullptr)
+      seg[i] = LpSegment{2 * a.tiles_r, 32 * l[i].nt, a.v0, a.vn, a.part, a.z};
+    a.w += a.vn * a.d;
+    a.v0 += a.vn;
+    if (kGrad) {
+      a.g += a.vn;
+      a.gcols -= a.vn;
+    } else {
+      a.part += 2 * a.tiles_r * a.M;
+      a.ent += 2 * a.tiles_r * a.M;
+      if (a.z != nullptr) a.z += (int64_t)a.tiles_r * (64 * l[i].nt) * a.M;
+    }
+    done += 2 * a.tiles_r;
+  }
+  if (slices != nullptr) *slices = done;
+  return NF4S_OK;
+}
+
+static int32_t lp_grad_logits(const void *ctx, const HeadPiece &p) {
+  LpLogits a = *static_cast<const LpLogits *>(ctx);
+  a.w += p.v0 * a.d;
+  a.v0 = p.v0;
+  a.vn = (int32_t)p.vn;
+  a.common = p.common;
+  a.g = p.g;
+  a.ldg = a.gcols = p.ldg;
+  return lp_logits<true>(a, nullptr, nullptr, p.stream);
+}
+
+}  // namespace nf4s
+
+using namespace nf4s;
+
+extern "C" {
+
+int32_t nf4s_linear_logprob_workspace_size(int64_t m, int64_t v, int64_t d, int64_t top_k,
+                                           int32_t backward, int64_t *bytes) {
+  clear_error();
+  if (bytes == nullptr) return fail(NF4S_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  *bytes = 0;
+  CePlan p;
+  const int32_t rc = lp_plan(m, v, d, top_k, p);
+  if (rc == NF4S_OK && m > 0)
+    *bytes = backward ? p.bwd_bytes : lp_forward_bytes(p, m, v, d, top_k);
+  return rc;
+}
+
+int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
+                                int64_t m, int64_t v, int64_t d, int64_t top_k,
+                                int64_t ignore_index, float *logp, float *lse, float *entropy,
+                                float *top_logp, int64_t *top_ids, void *workspace,
+                                int64_t workspace_bytes, void *stream) {
+  clear_error();
+  CePlan p;
+  int32_t rc = lp_plan(m, v, d, top_k, p);
+  if (rc != NF4S_OK || m == 0) return rc;
+  rc = ce_operands(x, w, targets, m, workspace, workspace_bytes,
+                   lp_forward_bytes(p, m, v, d, top_k));
+  if (rc != NF4S_OK) return rc;
+  if (logp == nullptr || lse == nullptr || entropy == nullptr ||
+      (top_k > 0 && (top_logp == nullptr || top_ids == nullptr)))
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "an output is NULL");
+  if (!aligned(logp, 4) || !aligned(lse, 4) || !aligned(entropy, 4) || !aligned(top_logp, 4) ||
+      !aligned(top_ids, 8))
+    return fail(NF4S_ERR_MISALIGNED, "outputs must be aligned to their elements");
+  const hipStream_t s = as_stream(stream);
+  char *base = static_cast<char *>(workspace);
+  for (int64_t m0 = 0; m0 < m; m0 += p.tokens) {
+    LpLogits a{};
+    a.M = m - m0 < p.tokens ? m - m0 : p.tokens;
+    const LpLayout l = lp_layout(a.M, v, d, top_k);
+    uint64_t *best = reinterpret_cast<uint64_t *>(base + l.best);
+    a.x = x + m0 * d;
+    a.targets = targets + m0;
+    a.d = d;
+    a.V = v;
+    a.ignore = ignore_index;
+    a.k = (int32_t)top_k;
+    a.part = reinterpret_cast<floatx2 *>(base);
+    a.ent = reinterpret_cast<float *>(base + l.ent);
+    a.zt = reinterpret_cast<float *>(base + l.zt);
+    a.z = top_k > 0 ? reinterpret_cast<float *>(base + l.z) : nullptr;
+    for (int64_t v0 = 0; v0 < v; v0 += l.piece) {
+      a.w = w + v0 * d;
+      a.v0 = v0;
+      a.vn = (int32_t)(v - v0 < l.piece ? v - v0 : l.piece);
+      a.best = v0 > 0 && top_k > 0 ? best : nullptr;
+      int64_t slices = 0;
+      LpSelect sel{};
+      rc = lp_logits<false>(a, &slices, sel.seg, s);
+      if (rc != NF4S_OK) return rc;
+      if (top_k > 0) {
+        sel.M = a.M;
+        sel.k = (int32_t)top_k;
+        sel.slices = (int32_t)slices;
+        sel.first = v0 == 0;
+        sel.best = best;
+        const int64_t lds = 4 * ((slices + 63) / 64 * 64 + top_k * (kLpWidth + 1));
+        const int64_t fit = kLpSelectLds / lds, waves = fit < 4 ? (fit < 1 ? 1 : fit) : 4;
+        hipLaunchKernelGGL(lp_select_kernel, dim3((uint32_t)ceil_to(a.M, waves)),
+                           dim3((uint32_t)(64 * waves)), (uint32_t)(waves * lds), s, sel);
+        rc = check_launch("lp_select_kernel");
+        if (rc != NF4S_OK) return rc;
+      }
+      a.part += slices * a.M;
+      a.ent += slices * a.M;
+    }
+    LpJoin j{};
+    j.part = reinterpret_cast<floatx2 *>(base);
+    j.ent = reinterpret_cast<float *>(base + l.ent);
+    j.zt = a.zt;
+    j.best = best;
+    j.targets = a.targets;
+    j.M = a.M;
+    j.slices = (int32_t)l.slices;
+    j.k = (int32_t)top_k;
+    j.V = v;
+    j.ignore = ignore_index;
+    j.logp = logp + m0;
+    j.lse = lse + m0;
+    j.entropy = entropy + m0;
+    j.top_logp = top_k > 0 ? top_logp + m0 * top_k : nullptr;
+    j.top_ids = top_k > 0 ? top_ids + m0 * top_k : nullptr;
+    const bool few = a.M < 512;
+    hipLaunchKernelGGL(few ? lp_join_kernel<1> : lp_join_kernel<8>,
+                       dim3((uint32_t)(few ? a.M : (a.M + 7) / 8)), dim3(256), 0, s, j);
+    rc = check_launch("lp_join_kernel");
+    if (rc != NF4S_OK) return rc;
+  }
+  return NF4S_OK;
+}
+
+int32_t nf4s_linear_logprob_bwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
+                                const float *lse, const float *entropy, const float *dlogp,
+                                const float *dentropy, int64_t m, int64_t v, int64_t d,
+                                int64_t ignore_index, uint16_t *dx, void *dw, int32_t dw_is_f32,
+                                int32_t accumulate, void *workspace, int64_t workspace_bytes,
+                                void *stream) {
+  clear_error();
+  CePlan p;
+  int32_t rc = lp_plan(m, v, d, 0, p);
+  if (rc != NF4S_OK) return rc;
+  rc = ce_operands(x, w, targets, m, workspace, workspace_bytes, p.bwd_bytes);
+  if (rc != NF4S_OK) return rc;
+  if (accumulate && !dw_is_f32)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "dw accumulates in fp32 only");
+  if (dw == nullptr || (m > 0 && (lse == nullptr || dlogp == nullptr || dx == nullptr)))
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "lse, dlogp, dx or dw is NULL");
+  if (m > 0 && dentropy != nullptr && entropy == nullptr)
+    return fail(NF4S_ERR_INVALID_ARGUMENT, "dentropy needs entropy");
+  if (!aligned(dw, 16) || (m > 0 && (!aligned(dx, 16) || !aligned(lse, 4) || !aligned(dlogp, 4) ||
+                                     !aligned(entropy, 4) || !aligned(dentropy, 4))))
+    return fail(NF4S_ERR_MISALIGNED,
+                "dx and dw must be 16-byte aligned, the tokens' values 4-byte");
+  const hipStream_t s = as_stream(stream);
+  if (m == 0) return accumulate ? NF4S_OK : head_zero_dw(dw, dw_is_f32 != 0, v * d, s);
+  const HeadGrad h{x, w, m, v, d, dx, dw, dw_is_f32 != 0, accumulate != 0, workspace};
+  hipLaunchKernelGGL(lp_common_kernel, dim3(1), dim3(1024), 0, s, dlogp, dentropy, targets,
+                     ignore_index, m, head_common(h, p));
+  rc = check_launch("lp_common_kernel");
+  if (rc != NF4S_OK) return rc;
+  LpLogits a{};
+  a.x = x;
+  a.w = w;
+  a.targets = targets;
+  a.M = m;
+  a.d = d;
+  a.V = v;
+  a.ignore = ignore_index;
+  a.lse = lse;
+  a.entropy = entropy;
+  a.dlogp = dlogp;
+  a.dentropy = dentropy;
+  return head_gradients(h, p, lp_grad_logits, &a, s);
+}
+
+}  // extern "C"

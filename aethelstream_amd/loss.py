@@ -2,6 +2,9 @@
 
 ``linear_cross_entropy``      loss and log-sum-exp of each token of x . W^T
 ``linear_cross_entropy_bwd``  dX and dW for given gradients of the losses
+``linear_log_probs``          log probability of each given token, the entropy of its
+                              distribution and the most likely alternatives
+``linear_log_probs_bwd``      dX and dW for gradients of the first two
 
 They take the place of the reference's two passes over vocabulary tiles
 (doublepass/src/loss.rs, doublepass/kernels/fused_ce.cu:71-207): the logits live
@@ -15,13 +18,14 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from .gemm import _workspace_for
-from .nf4 import _require_cuda, _stream_ptr
+from .nf4 import _ptr, _require_cuda, _stream_ptr
 
 IGNORE_INDEX = -100
 
@@ -50,6 +54,21 @@ def _check_head(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor) -> None
         raise ValueError(f"targets must be int64 [{x.shape[0]}]")
     if w.device != x.device or targets.device != x.device:
         raise ValueError("x, w and targets must be on one device")
+
+
+def _check_dw(dw: Optional[torch.Tensor], accumulate: bool, w: torch.Tensor,
+              x: torch.Tensor) -> torch.Tensor:
+    """The gradient of w: what the caller gave, if it can be that, or new memory."""
+    if dw is None:
+        if accumulate:
+            raise ValueError("accumulate needs an existing float32 dw")
+        dw = torch.empty_like(w)
+    if dw.dtype not in (torch.bfloat16, torch.float32) or dw.shape != w.shape \
+            or dw.device != x.device:
+        raise ValueError(f"dw must be bfloat16 or float32 {list(w.shape)} on x's device")
+    if accumulate and dw.dtype != torch.float32:
+        raise ValueError("accumulate needs a float32 dw")
+    return dw
 
 
 def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
@@ -93,15 +112,7 @@ def linear_cross_entropy_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Te
     for t, name in ((lse, "lse"), (dloss, "dloss")):
         if t.dtype != torch.float32 or list(t.shape) != [m] or t.device != x.device:
             raise ValueError(f"{name} must be float32 [{m}] on x's device")
-    if dw is None:
-        if accumulate:
-            raise ValueError("accumulate needs an existing float32 dw")
-        dw = torch.empty_like(w)
-    if dw.dtype not in (torch.bfloat16, torch.float32) or list(dw.shape) != [v, d] \
-            or dw.device != x.device:
-        raise ValueError(f"dw must be bfloat16 or float32 [{v}, {d}] on x's device")
-    if accumulate and dw.dtype != torch.float32:
-        raise ValueError("accumulate needs a float32 dw")
+    dw = _check_dw(dw, accumulate, w, x)
     dx = torch.empty_like(x)
     workspace = _workspace_for(_workspace_bytes(m, v, d, True, x.get_device()), workspace, x)
     _lib.check(_lib.load().nf4s_linear_ce_bwd(
@@ -109,4 +120,95 @@ def linear_cross_entropy_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Te
         ignore_index, dx.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32),
         int(accumulate), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
         _stream_ptr(x)))
+    return dx, dw
+
+
+TOP = 32  # alternatives of a token at most
+
+
+@dataclass
+class LogProbs:
+    """Outputs of :func:`linear_log_probs`."""
+
+    logp: torch.Tensor                # float32 [M], of the given tokens
+    entropy: torch.Tensor             # float32 [M]
+    lse: torch.Tensor                 # float32 [M]
+    top_logp: Optional[torch.Tensor]  # float32 [M, top_k], with top_k > 0
+    top_ids: Optional[torch.Tensor]   # int64 [M, top_k]
+
+
+def log_probs_workspace_bytes(m: int, v: int, d: int, top_k: int = 0,
+                              backward: bool = False) -> int:
+    """Workspace of :func:`linear_log_probs`, or of its gradients, for M tokens and a
+    [V, d] head."""
+    return _log_probs_workspace_bytes(m, v, d, top_k, backward, torch.cuda.current_device())
+
+
+@functools.lru_cache(maxsize=256)
+def _log_probs_workspace_bytes(m: int, v: int, d: int, top_k: int, backward: bool,
+                               device: int) -> int:
+    out = ctypes.c_int64(0)
+    _lib.check(_lib.load().nf4s_linear_logprob_workspace_size(m, v, d, top_k, int(backward),
+                                                              ctypes.byref(out)))
+    return int(out.value)
+
+
+def linear_log_probs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
+                     ignore_index: int = IGNORE_INDEX,
+                     workspace: Optional[torch.Tensor] = None) -> LogProbs:
+    """Log probability of ``targets`` under softmax(x . W^T), the entropy and the
+    log-sum-exp of every token, and with ``top_k`` (up to 32) the tokens of largest
+    logit in order, equal ones by their index, with their log probabilities.  A target
+    equal to ``ignore_index`` (no token is given) has logp 0, and the rest as any
+    other; a target outside [0, V) has NaN (it is only seen on the device).  A row with
+    a NaN logit, or an infinite largest one, is NaN in everything but ``top_ids``."""
+    _check_head(x, w, targets)
+    m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(TOP, v):
+        raise ValueError(f"top_k must be 0 to {TOP} and at most {v}, got {top_k}")
+    logp = torch.empty(m, dtype=torch.float32, device=x.device)
+    lse, entropy = torch.empty_like(logp), torch.empty_like(logp)
+    top_logp = top_ids = None
+    if top_k > 0:
+        top_logp = torch.empty(m, top_k, dtype=torch.float32, device=x.device)
+        top_ids = torch.empty(m, top_k, dtype=torch.int64, device=x.device)
+    workspace = _workspace_for(
+        _log_probs_workspace_bytes(m, v, d, top_k, False, x.get_device()), workspace, x)
+    _lib.check(_lib.load().nf4s_linear_logprob_fwd(
+        x.data_ptr(), w.data_ptr(), targets.data_ptr(), m, v, d, top_k, ignore_index,
+        logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids),
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_ptr(x)))
+    return LogProbs(logp, entropy, lse, top_logp, top_ids)
+
+
+def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, out: LogProbs,
+                         dlogp: torch.Tensor, dentropy: Optional[torch.Tensor] = None,
+                         ignore_index: int = IGNORE_INDEX, dw: Optional[torch.Tensor] = None,
+                         accumulate: bool = False, workspace: Optional[torch.Tensor] = None
+                         ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dx bf16 [M, d], dw [V, d]) for the gradients ``dlogp`` and ``dentropy`` (fp32
+    [M]; None: zero) of :func:`linear_log_probs`' result ``out``.  An ignored target's
+    dlogp does not count, its dentropy does.  dw is bf16 unless a float32 ``dw`` is
+    given, which the micro-batches of a step may ``accumulate`` into; the gradients of
+    the logits enter both products rounded to bf16, as in
+    :func:`linear_cross_entropy_bwd`, divided by the largest ``|dlogp|``.  Tokens with
+    both gradients zero count as zeros times their row of x, which has to be finite."""
+    _check_head(x, w, targets)
+    _require_cuda(out.lse, out.entropy, dlogp, dentropy, dw)
+    m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
+    for t, name in ((out.lse, "lse"), (out.entropy, "entropy"), (dlogp, "dlogp"),
+                    (dentropy, "dentropy")):
+        if t is not None and (t.dtype != torch.float32 or list(t.shape) != [m]
+                              or t.device != x.device):
+            raise ValueError(f"{name} must be float32 [{m}] on x's device")
+    dw = _check_dw(dw, accumulate, w, x)
+    dx = torch.empty_like(x)
+    workspace = _workspace_for(
+        _log_probs_workspace_bytes(m, v, d, 0, True, x.get_device()), workspace, x)
+    _lib.check(_lib.load().nf4s_linear_logprob_bwd(
+        x.data_ptr(), w.data_ptr(), targets.data_ptr(), out.lse.data_ptr(),
+        out.entropy.data_ptr(), dlogp.data_ptr(), _ptr(dentropy), m, v, d, ignore_index,
+        dx.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32), int(accumulate),
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_ptr(x)))
     return dx, dw

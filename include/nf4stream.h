@@ -514,6 +514,45 @@ int32_t nf4s_linear_ce_workspace_size(int64_t m, int64_t v, int64_t d, int32_t b
                                       int64_t *bytes);
 
 /* ---------------------------------------------------------------------------
+ * Log probabilities under a linear head, without keeping the logits z = x . w^T:
+ *   lse[i] = log sum_c exp z[i, c],  logp[i] = z[i, targets[i]] - lse[i]
+ *   entropy[i] = -sum_c p log p,  p = exp(z[i, c] - lse[i])
+ *   top_ids[i, 0 .. top_k - 1]: the columns of the largest logits, equal ones by
+ *   their index, and their log probabilities top_logp
+ * x, w and targets as for the cross entropy; logp, lse and entropy fp32 [m],
+ * top_logp fp32 and top_ids int64 [m, top_k] (top_k = 0: NULL).  A target equal to
+ * ignore_index has logp 0 (the rest of its token is as any other's), any other
+ * outside [0, v) has NaN.  A token with a NaN logit, or an infinite largest one,
+ * has NaN everywhere but in top_ids.
+ * Limits and alignment of the cross entropy; top_k <= 32 and <= v.
+ * ------------------------------------------------------------------------- */
+int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
+                                int64_t m, int64_t v, int64_t d, int64_t top_k,
+                                int64_t ignore_index, float *logp, float *lse, float *entropy,
+                                float *top_logp, int64_t *top_ids, void *workspace,
+                                int64_t workspace_bytes, void *stream);
+/*
+ * Gradients for given dlogp and dentropy (fp32 [m]; dentropy NULL: zero) and the
+ * forward's lse and entropy (NULL without dentropy):
+ *   G[i, c] = [c = targets[i]] dlogp[i] - p (dlogp[i] + dentropy[i] (log p + entropy[i]))
+ *   dx = G . w,  dw = G^T . x
+ * with dlogp 0 where the target is ignored; dx, dw, dw_is_f32, accumulate and the
+ * rounding of G as for the cross entropy, G divided by the largest |dlogp| (by the
+ * largest |dentropy| if there is none).  A token whose gradients are both zero adds
+ * zeros times its row of x, which has to be finite.
+ */
+int32_t nf4s_linear_logprob_bwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
+                                const float *lse, const float *entropy, const float *dlogp,
+                                const float *dentropy, int64_t m, int64_t v, int64_t d,
+                                int64_t ignore_index, uint16_t *dx, void *dw, int32_t dw_is_f32,
+                                int32_t accumulate, void *workspace, int64_t workspace_bytes,
+                                void *stream);
+/* Workspace bytes of the forward (backward = 0) or of the gradients (whatever
+ * top_k).  Calls that share a workspace must not overlap. */
+int32_t nf4s_linear_logprob_workspace_size(int64_t m, int64_t v, int64_t d, int64_t top_k,
+                                           int32_t backward, int64_t *bytes);
+
+/* ---------------------------------------------------------------------------
  * Streamed layer stack (one GPU).  Layers wait in pinned host memory and are
  * copied into a two-slot device double buffer on a dedicated copy stream.
  * ------------------------------------------------------------------------- */
