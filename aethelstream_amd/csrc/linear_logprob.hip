@@ -33,7 +33,6 @@ constexpr int64_t kLpPieceBytes = (int64_t)256 << 20;
 // Columns of a piece, whose maxima (of 64 at least) a wave holds in LDS: 16 KB.
 constexpr int64_t kLpPieceCols = 1 << 18;
 constexpr int64_t kLpSelectLds = 64 << 10;
-constexpr int kLpWidth = 128;  // columns of a half tile at most
 
 struct LpLogits {
   const uint16_t *x, *w;  // w at the launch's first row
@@ -230,7 +229,8 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 // Half tiles of one launch of a piece.
 struct LpSegment {
   int32_t slices, width;
-  int64_t column, columns;  // first one, and how many there are
+  uint32_t column;   // the first one
+  int32_t columns;   // how many there are
   const floatx2 *part;      // [slices][M]
   const float *z;           // [slices][M][width]
 };
@@ -243,101 +243,195 @@ struct LpSelect {
   uint64_t *best;     // [M][k]
 };
 
-// One wave a token: k half tiles by their maxima, then the k best of their logits
-// and of the pieces before.  LDS: the maxima, the chosen ones' logits, both as
-// ordered integers, a lane's own every 64th.
-__global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
-  extern __shared__ uint32_t lp_lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
-  if (row >= a.M) return;
-  const int rounds = (a.slices + 63) / 64;
-  uint32_t *maxima = lp_lds + wave * (64 * rounds + a.k * (kLpWidth + 1));
-  uint32_t *logits = maxima + 64 * rounds;
-  int32_t *chosen = reinterpret_cast<int32_t *>(logits + a.k * kLpWidth);
-  uint64_t *best = a.best + row * a.k;
-  const uint32_t least = a.first ? 0 : (uint32_t)(best[a.k - 1] >> 32);
+// Keys a wave ranks at once: two a lane.
+constexpr int kLpList = 128;
+// Half tiles whose logits are looked at; the lanes name them.
+constexpr int kLpHeld = 64;
 
-  // A half tile is a candidate if its maximum exceeds the k-th best.
-  uint64_t own = 0;
-  for (int i = 0; i < rounds; ++i) {
-    const int s = 64 * i + lane;
-    uint32_t o = 0;
-    if (s < a.slices) {
-      const bool second = s >= a.seg[0].slices;
-      const floatx2 *p = second ? a.seg[1].part + (int64_t)(s - a.seg[0].slices) * a.M
-                                : a.seg[0].part + (int64_t)s * a.M;
-      o = lp_order(p[row].x);
-      if (o <= least) o = 0;
-    }
-    maxima[s] = o;
-    const uint64_t key = lp_key(o, (uint32_t)s);
-    own = key > own ? key : own;
+// The k-th largest of the lanes' values (0 if it has none): below it are none of the
+// k largest of all values whose maxima the lanes hold.
+__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k, int lane) {
+  int ahead = 0;
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)v, i);
+    ahead += o > v || (o == v && i < lane) ? 1 : 0;
   }
-  int count = 0;
-  for (; count < a.k; ++count) {
-    const uint64_t top = wave_max64(own);
-    if (top == 0) break;
-    const int s = (int)~(uint32_t)top;
-    if (lane == 0) chosen[count] = s;
-    if (own == top) {
-      maxima[s] = 0;
-      own = 0;
-      for (int i = 0; i < rounds; ++i) {
-        const uint64_t key = lp_key(maxima[64 * i + lane], (uint32_t)(64 * i + lane));
-        own = key > own ? key : own;
-      }
-    }
-  }
-  if (count == 0) return;  // the pieces before had all
+  const uint64_t at = __ballot(ahead == k - 1);
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, __builtin_ctzll(at));
+}
 
-  // Two logits a lane of every chosen half tile.
+// Writes visible to the wave's other lanes.
+__device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  auto column = [&](int j, int h, bool &in) {
-    const int s = chosen[j];
-    const LpSegment &g = s >= a.seg[0].slices ? a.seg[1] : a.seg[0];
-    const int at = s >= a.seg[0].slices ? s - a.seg[0].slices : s;
-    const int64_t c = (int64_t)at * g.width + 64 * h + lane;
-    in = 64 * h + lane < g.width && c < g.columns;
-    return (uint32_t)(g.column + c);
-  };
-  own = 0;
-  for (int j = 0; j < count; ++j) {
-    const int s = chosen[j];
-    const bool second = s >= a.seg[0].slices;
-    const int width = second ? a.seg[1].width : a.seg[0].width;
-    const float *z = second ? a.seg[1].z + ((int64_t)(s - a.seg[0].slices) * a.M + row) * width
-                            : a.seg[0].z + ((int64_t)s * a.M + row) * width;
+}
+
+// One wave a token.  Twice the same step, over the half tiles' maxima and over the
+// logits of those that are left: the k-th largest of the 64 lanes' own maxima is
+// reached by k values at least, so what lies below is out; of those equal to it the
+// first k are enough.  What remains, about k, is ranked by counting, together with
+// the k best of the pieces before.  The maxima (ordered integers) and the list are in
+// LDS.  Should more than kLpHeld half tiles or kLpList values remain, which takes
+// logits sorted against the lanes, k rounds over all of them find the k best.
+__global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
+  extern __shared__ uint64_t lp_lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
+  if (row >= a.M) return;
+  const int rounds = (a.slices + 63) / 64;
+  uint64_t *list = lp_lds + wave * (kLpList + kLpHeld / 2 + 32 * rounds);
+  int32_t *chosen = reinterpret_cast<int32_t *>(list + kLpList);
+  uint32_t *maxima = reinterpret_cast<uint32_t *>(chosen + kLpHeld);
+  uint64_t *best = a.best + row * a.k;
+  const uint64_t before = !a.first && lane < a.k ? best[lane] : 0;
+  const uint32_t least = a.first ? 0 : (uint32_t)(best[a.k - 1] >> 32);
+  const uint64_t below = (1ull << lane) - 1;
+  const LpSegment g0 = a.seg[0], g1 = a.seg[1];
+
+  uint32_t top = 0;
+  for (int i0 = 0; i0 < rounds; i0 += 8) {
+    float v[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bool in;
-      const uint32_t c = column(j, h, in);
-      const uint32_t o = in ? lp_order(z[64 * h + lane]) : 0;
-      logits[(2 * j + h) * 64 + lane] = o;
-      const uint64_t key = lp_key(o, c);
-      own = key > own ? key : own;
+    for (int i = 0; i < 8; ++i) {
+      const int s = 64 * (i0 + i) + lane;
+      const bool second = s >= g0.slices;
+      const floatx2 *p = second ? g1.part + (int64_t)(s - g0.slices) * a.M
+                                : g0.part + (int64_t)s * a.M;
+      v[i] = s < a.slices ? p[row].x : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = 64 * (i0 + i) + lane;
+      uint32_t o = s < a.slices ? lp_order(v[i]) : 0;
+      // A half tile counts only if its maximum exceeds the k-th best.
+      if (o <= least) o = 0;
+      if (i0 + i < rounds) maxima[s] = o;
+      top = o > top ? o : top;
     }
   }
-  uint64_t before = !a.first && lane < a.k ? best[lane] : 0;
-  for (int t = 0; t < a.k; ++t) {
-    const uint64_t top = wave_max64(own > before ? own : before);
-    if (lane == 0) best[t] = top;
-    if (top == 0) continue;
-    if (before == top) {
-      before = 0;
-    } else if (own == top) {
-      own = 0;
-      for (int j = 0; j < 2 * count; ++j) {
-        bool in;
-        const uint32_t c = column(j / 2, j % 2, in);
-        uint32_t o = logits[j * 64 + lane];
-        if (lp_key(o, c) == top) logits[j * 64 + lane] = o = 0;
-        const uint64_t key = lp_key(o, c);
-        own = key > own ? key : own;
+  if (__ballot(top != 0) == 0) return;  // the pieces before had all
+  uint32_t floor = kth_of_lanes(top, a.k, lane);
+  if (floor == 0) floor = 1;
+
+  // The half tiles that are left, by their index.
+  int count = 0, equal = 0;
+  for (int i = 0; i < rounds; ++i) {
+    const uint32_t o = maxima[64 * i + lane];
+    const uint64_t same = __ballot(o == floor);
+    const bool in = o > floor || (o == floor && equal + __popcll(same & below) < a.k);
+    const uint64_t all = __ballot(in);
+    const int at = count + __popcll(all & below);
+    if (in && at < kLpHeld) chosen[at] = 64 * i + lane;
+    count += __popcll(all);
+    equal += __popcll(same);
+  }
+  wave_lds_fence();
+
+  int n = 0;
+  if (count <= kLpHeld) {
+    const int32_t mine = lane < count ? chosen[lane & (kLpHeld - 1)] : 0;
+    // The logits of eight half tiles from j on, ordered, and their first columns; all
+    // loads before the first use.
+    struct Eight {
+      uint32_t order[16], column[8];
+    };
+    auto eight = [&](int j) {
+      Eight e;
+      float v[16];
+      int wide[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int s = __builtin_amdgcn_readlane(mine, j + i);  // of lanes past `count`: 0
+        const bool second = s >= g0.slices;
+        const int at = second ? s - g0.slices : s, width = second ? g1.width : g0.width;
+        const int left = (second ? g1.columns : g0.columns) - at * width;
+        wide[i] = j + i >= count ? 0 : left < width ? left : width;
+        e.column[i] = (second ? g1.column : g0.column) + (uint32_t)(at * width);
+        const float *z = (second ? g1.z : g0.z) + ((int64_t)at * a.M + row) * width;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[2 * i + h] = 64 * h + lane < wide[i] ? z[64 * h + lane] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        e.order[i] = 64 * (i % 2) + lane < wide[i / 2] ? lp_order(v[i]) : 0;
+      return e;
+    };
+    top = 0;
+#pragma unroll 1
+    for (int j = 0; j < count; j += 8) {
+      const Eight e = eight(j);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = e.order[i] > top ? e.order[i] : top;
+    }
+    const uint32_t kth = kth_of_lanes(top, a.k, lane);
+    floor = kth > floor ? kth : floor;
+    // Later columns lose a tie with the pieces before.
+    if (floor <= least) floor = least + 1;
+    equal = 0;
+#pragma unroll 1
+    for (int j = 0; j < count; j += 8) {
+      const Eight e = eight(j);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t o = e.order[i];
+        if (__ballot(o >= floor) == 0) continue;
+        const uint64_t same = __ballot(o == floor);
+        const bool in = o > floor || (o == floor && equal + __popcll(same & below) < a.k);
+        const uint64_t all = __ballot(in);
+        const int to = n + __popcll(all & below);
+        if (in && to < kLpList)
+          list[to] = lp_key(o, e.column[i / 2] + 64 * (uint32_t)(i % 2) + (uint32_t)lane);
+        n += __popcll(all);
+        equal += __popcll(same);
       }
     }
+    // The pieces before.
+    const uint64_t had = __ballot(before != 0);
+    const int to = n + __popcll(had & below);
+    if (before != 0 && to < kLpList) list[to] = before;
+    n += __popcll(had);
+    wave_lds_fence();
+    if (n <= kLpList) {
+      const uint64_t key[2] = {lane < n ? list[lane] : 0, 64 + lane < n ? list[64 + lane] : 0};
+      int ahead[2] = {0, 0};
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const uint64_t o = list[i];
+        ahead[0] += o > key[0] ? 1 : 0;
+        ahead[1] += o > key[1] ? 1 : 0;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (64 * h + lane < n && ahead[h] < a.k) best[ahead[h]] = key[h];
+      // (Fewer than k only where the vocabulary's first piece has fewer.)
+      if (lane >= n && lane < a.k) best[lane] = 0;
+      return;
+    }
+  }
+
+  uint64_t last = ~0ull;
+  for (int t = 0; t < a.k; ++t) {
+    uint64_t own = before < last ? before : 0;
+    for (int s = 0; s < a.slices; ++s) {
+      const uint32_t o = maxima[s];
+      if (o == 0 || o < floor) continue;
+      const bool second = s >= g0.slices;
+      const int at = second ? s - g0.slices : s, width = second ? g1.width : g0.width;
+      const int c = at * width, columns = second ? g1.columns : g0.columns;
+      const uint32_t column = (second ? g1.column : g0.column) + (uint32_t)c;
+      const float *z = (second ? g1.z : g0.z) + ((int64_t)at * a.M + row) * width;
+      for (int e = lane; e < width && c + e < columns; e += 64) {
+        const uint32_t order = lp_order(z[e]);
+        const uint64_t key = order <= least ? 0 : lp_key(order, column + e);
+        if (key < last && key > own) own = key;
+      }
+    }
+    last = wave_max64(own);
+    if (lane == 0) best[t] = last;
+    if (last == 0) last = 1;
   }
 }
 
@@ -531,7 +625,7 @@ static int32_t lp_logits(LpLogits a, int64_t *slices, LpSegment *seg, hipStream_
     const int32_t rc = check_launch("lp_logits_kernel");
     if (rc != NF4S_OK) return rc;
     if (seg != nullptr)
-      seg[i] = LpSegment{2 * a.tiles_r, 32 * l[i].nt, a.v0, a.vn, a.part, a.z};
+      seg[i] = LpSegment{2 * a.tiles_r, 32 * l[i].nt, (uint32_t)a.v0, a.vn, a.part, a.z};
     a.w += a.vn * a.d;
     a.v0 += a.vn;
     if (kGrad) {
@@ -627,7 +721,7 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
         sel.slices = (int32_t)slices;
         sel.first = v0 == 0;
         sel.best = best;
-        const int64_t lds = 4 * ((slices + 63) / 64 * 64 + top_k * (kLpWidth + 1));
+        const int64_t lds = 8 * kLpList + 4 * kLpHeld + 4 * ((slices + 63) / 64 * 64);
         const int64_t fit = kLpSelectLds / lds, waves = fit < 4 ? (fit < 1 ? 1 : fit) : 4;
         hipLaunchKernelGGL(lp_select_kernel, dim3((uint32_t)ceil_to(a.M, waves)),
                            dim3((uint32_t)(64 * waves)), (uint32_t)(waves * lds), s, sel);
