@@ -34,9 +34,9 @@ namespace nf4s {
 
 constexpr int kAdamThreads = 256;
 constexpr int kAdamBlock = 128;
-constexpr int kAdamEach = 8;   // elements of a lane at once
-constexpr int kAdamIter = 2;   // times that in a chunk
-constexpr int kAdamChunk = kAdamThreads * kAdamEach * kAdamIter;
+// Elements of a lane at once: a block's codes are 16 lanes, fp32 rows of 16 bytes.
+constexpr int kAdamEach8 = 8, kAdamEach32 = 4;
+constexpr int kAdamChunk = 4096;  // elements of a workgroup
 constexpr uint32_t kAdamOffset = 0x38000000u;  // 2^-15
 
 enum { kBeta1, kRest1, kBeta2, kRest2, kKeep, kSize, kInvRoot, kEps, kHyper };
@@ -73,58 +73,65 @@ __device__ __forceinline__ uint32_t dpp_max16(uint32_t v) {
   return with(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
 }
 
-// Eight values of either type from p, or those of them below n, one by one.
+// kN values of either type from p, or `left` of them, one by one.
+template <int kN>
 __device__ __forceinline__ void adam_load(const uint16_t *p, bool whole, uint32_t left,
-                                          float (&x)[kAdamEach]) {
+                                          float (&x)[kN]) {
+  typedef uint32_t words __attribute__((ext_vector_type(kN / 2)));
   if (whole) {
-    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+    const words w = __builtin_nontemporal_load(reinterpret_cast<const words *>(p));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kN / 2; ++i) {
       x[2 * i] = bf16_low(w[i]);
       x[2 * i + 1] = bf16_high(w[i]);
     }
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < kAdamEach; ++i) x[i] = i < left ? bf16_low(p[i]) : 0.0f;
+    for (uint32_t i = 0; i < kN; ++i) x[i] = i < left ? bf16_low(p[i]) : 0.0f;
   }
 }
+template <int kN>
 __device__ __forceinline__ void adam_load(const float *p, bool whole, uint32_t left,
-                                          float (&x)[kAdamEach]) {
+                                          float (&x)[kN]) {
   if (whole) {
-    const floatx4 a = __builtin_nontemporal_load(reinterpret_cast<const floatx4 *>(p));
-    const floatx4 b = __builtin_nontemporal_load(reinterpret_cast<const floatx4 *>(p) + 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = a[i];
-      x[4 + i] = b[i];
+    for (int j = 0; j < kN / 4; ++j) {
+      const floatx4 a = __builtin_nontemporal_load(reinterpret_cast<const floatx4 *>(p) + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * j + i] = a[i];
     }
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < kAdamEach; ++i) x[i] = i < left ? p[i] : 0.0f;
+    for (uint32_t i = 0; i < kN; ++i) x[i] = i < left ? p[i] : 0.0f;
   }
 }
+template <int kN>
 __device__ __forceinline__ void adam_store(uint16_t *p, bool whole, uint32_t left,
-                                           const float (&x)[kAdamEach]) {
+                                           const float (&x)[kN]) {
+  typedef uint32_t words __attribute__((ext_vector_type(kN / 2)));
   if (whole) {
-    u32x4 w;
+    words w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-    __builtin_nontemporal_store(w, reinterpret_cast<u32x4 *>(p));
+    for (int i = 0; i < kN / 2; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    __builtin_nontemporal_store(w, reinterpret_cast<words *>(p));
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < kAdamEach; ++i)
+    for (uint32_t i = 0; i < kN; ++i)
       if (i < left) p[i] = (uint16_t)pack_bf16x2(x[i], 0.0f);
   }
 }
+template <int kN>
 __device__ __forceinline__ void adam_store(float *p, bool whole, uint32_t left,
-                                           const float (&x)[kAdamEach]) {
+                                           const float (&x)[kN]) {
   if (whole) {
-    __builtin_nontemporal_store((floatx4){x[0], x[1], x[2], x[3]}, reinterpret_cast<floatx4 *>(p));
-    __builtin_nontemporal_store((floatx4){x[4], x[5], x[6], x[7]},
-                                reinterpret_cast<floatx4 *>(p) + 1);
+#pragma unroll
+    for (int j = 0; j < kN / 4; ++j)
+      __builtin_nontemporal_store(
+          (floatx4){x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]},
+          reinterpret_cast<floatx4 *>(p) + j);
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < kAdamEach; ++i)
+    for (uint32_t i = 0; i < kN; ++i)
       if (i < left) p[i] = x[i];
   }
 }
@@ -137,39 +144,50 @@ __device__ __forceinline__ float adam_value(uint32_t mag) {
 }
 template <int kShift>
 __device__ __forceinline__ uint32_t adam_code(float y) {
-  const uint32_t u =
-      __builtin_bit_cast(uint32_t, y + __builtin_bit_cast(float, kAdamOffset)) - kAdamOffset;
-  return (u + ((1u << (kShift - 1)) - 1) + ((u >> kShift) & 1)) >> kShift;
+  // (The offset's own bits end above the shift: the tie's bit may be taken before it
+  // is subtracted.)
+  static_assert((kAdamOffset & ((2u << kShift) - 1)) == 0, "offset");
+  const uint32_t u = __builtin_bit_cast(uint32_t, y + __builtin_bit_cast(float, kAdamOffset));
+  return (u + ((u >> kShift) & 1) + (((1u << (kShift - 1)) - 1) - kAdamOffset)) >> kShift;
 }
 // A block's scale from its largest absolute value's bits; NaN if that is no number.
 __device__ __forceinline__ float adam_scale(uint32_t top) {
   const float t = __builtin_bit_cast(float, top);
   return top >= 0x7f800000u ? __builtin_nanf("") : fmaxf(t, 0x1p-126f);
 }
+// m of the code in byte i of w, and sqrt(v).
+template <int kI>
+__device__ __forceinline__ float adam_m(uint32_t w, float scale) {
+  const int32_t q = (int32_t)(w << (24 - 8 * kI)) >> 24;
+  const int32_t n = -q;
+  const float a = adam_value<20>((uint32_t)(q > n ? q : n)) * scale;
+  // The sign of q.
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, a) & 0x7fffffffu) |
+                                       ((uint32_t)q & 0x80000000u));
+}
+template <int kI>
+__device__ __forceinline__ float adam_r(uint32_t w, float scale) {
+  return adam_value<19>((w >> (8 * kI)) & 0xff) * scale;
+}
+// Four codes' low bytes as one word.
+__device__ __forceinline__ uint32_t adam_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return perm(perm(d, c, 0x0c0c0400u), perm(b, a, 0x0c0c0400u), 0x05040100u);
+}
 
-// Moments of the 8 elements from `at`; the moments' buffers are whole blocks long.
-__device__ __forceinline__ void adam_moments(const AdamCommon &c, int64_t at, float (&m)[kAdamEach],
-                                             float (&v)[kAdamEach], bool bits8) {
-  if (bits8) {
-    const u32x2 mc = *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(c.m) + at);
-    const u32x2 vc = *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(c.v) + at);
-    const float ms = c.m_scale[at / kAdamBlock], vs = c.v_scale[at / kAdamBlock];
-#pragma unroll
-    for (int i = 0; i < kAdamEach; ++i) {
-      const int32_t q = (int32_t)(mc[i / 4] << (24 - 8 * (i % 4))) >> 24;
-      const float a = adam_value<20>((uint32_t)(q < 0 ? -q : q)) * ms;
-      m[i] = q < 0 ? -a : a;
-      const float r = adam_value<19>((vc[i / 4] >> (8 * (i % 4))) & 0xff) * vs;
-      v[i] = r * r;
-    }
-  } else {
-    adam_load(static_cast<const float *>(c.m) + at, true, 0, m);
-    adam_load(static_cast<const float *>(c.v) + at, true, 0, v);
-  }
+// The correctly rounded square root of 0 or of a number in [2^-100, 2^120], in six
+// instructions instead of sixteen: v y with y = rsqrt(v), and half y times what its
+// square leaves.  (Every fp32 number of that range was compared with the correctly
+// rounded root.)
+__device__ __forceinline__ float adam_root(float v) {
+  const float y = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-100f));
+  const float s = v * y;
+  return __builtin_fmaf(__builtin_fmaf(-s, s, v), 0.5f * y, s);
 }
 
 template <typename P, typename G, bool kBits8, bool kCopy>
 __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const AdamTable<kCopy> t) {
+  constexpr int kEach = kBits8 ? kAdamEach8 : kAdamEach32;
+  constexpr int kIter = kAdamChunk / kAdamThreads / kEach;
   // The tensor whose chunks hold this one.
   int lo = 0, hi = t.c.count;
   while (hi - lo > 1) {
@@ -179,6 +197,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const AdamTable<kCo
   }
   const uint32_t n = t.n[lo];
   const uint32_t first = (blockIdx.x - t.chunk[lo]) * kAdamChunk;
+  const int64_t base = (int64_t)t.block[lo] * kAdamBlock;  // of the tensor's moments
   P *p = static_cast<P *>(t.p[lo]);
   const G *g = static_cast<const G *>(t.g[lo]);
   uint16_t *copy = kCopy ? t.copy[lo] : nullptr;
@@ -190,83 +209,135 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const AdamTable<kCo
   for (int i = 0; i < kHyper; ++i) h[i] = hyper != nullptr ? hyper[i] : t.c.value[i];
   const float gs = t.c.grad_scale != nullptr ? *t.c.grad_scale : 1.0f;
 
-  float pv[kAdamIter][kAdamEach], gv[kAdamIter][kAdamEach];
-  float m[kAdamIter][kAdamEach], v[kAdamIter][kAdamEach];
+  // All loads, then all else.
+  float pv[kIter][kEach], gv[kIter][kEach], mv[kIter][kEach], vv[kIter][kEach];
+  u32x2 mc[kIter], vc[kIter];
+  float ms[kIter], vs[kIter];
 #pragma unroll
-  for (int k = 0; k < kAdamIter; ++k) {
-    const uint32_t e = first + (k * kAdamThreads + threadIdx.x) * kAdamEach;
+  for (int k = 0; k < kIter; ++k) {
+    const uint32_t e = first + (k * kAdamThreads + threadIdx.x) * kEach;
     const uint32_t left = e < n ? n - e : 0;
     if (left == 0) continue;
-    const bool whole = vec && left >= kAdamEach;
+    const bool whole = vec && left >= kEach;
     adam_load(p + e, whole, left, pv[k]);
     adam_load(g + e, whole, left, gv[k]);
-    adam_moments(t.c, (int64_t)t.block[lo] * kAdamBlock + e, m[k], v[k], kBits8);
+    const int64_t at = base + e;
+    if constexpr (kBits8) {
+      mc[k] = *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(t.c.m) + at);
+      vc[k] = *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(t.c.v) + at);
+      ms[k] = t.c.m_scale[at / kAdamBlock];
+      vs[k] = t.c.v_scale[at / kAdamBlock];
+    } else {
+      adam_load(static_cast<const float *>(t.c.m) + at, true, 0, mv[k]);
+      adam_load(static_cast<const float *>(t.c.v) + at, true, 0, vv[k]);
+    }
   }
 #pragma unroll
-  for (int k = 0; k < kAdamIter; ++k) {
-    const uint32_t e = first + (k * kAdamThreads + threadIdx.x) * kAdamEach;
+  for (int k = 0; k < kIter; ++k) {
+    const uint32_t e = first + (k * kAdamThreads + threadIdx.x) * kEach;
     const uint32_t left = e < n ? n - e : 0;
     if (!kBits8 && left == 0) continue;
-    uint32_t m_top = 0, r_top = 0;
-    float r[kAdamEach];
+    float (&m)[kEach] = mv[k], (&v)[kEach] = vv[k], (&x)[kEach] = pv[k];
+    if constexpr (kBits8) {
+      static_for<0, kEach>([&](auto I) {
+        constexpr int i = decltype(I)::value;
+        m[i] = adam_m<i % 4>(mc[k][i / 4], ms[k]);
+        const float q = adam_r<i % 4>(vc[k][i / 4], vs[k]);
+        v[i] = q * q;
+      });
+    }
 #pragma unroll
-    for (uint32_t i = 0; i < kAdamEach; ++i) {
-      const float x = gv[k][i] * gs;
-      m[k][i] = m[k][i] * h[kBeta1] + x * h[kRest1];
-      v[k][i] = v[k][i] * h[kBeta2] + x * x * h[kRest2];
-      if (i >= left) m[k][i] = v[k][i] = 0.0f;  // past the tensor's end
-      r[i] = __builtin_sqrtf(v[k][i]);
-      pv[k][i] = pv[k][i] * h[kKeep] - m[k][i] / (r[i] * h[kInvRoot] + h[kEps]) * h[kSize];
-      if (kBits8) {
-        const uint32_t a = __builtin_bit_cast(uint32_t, m[k][i]) & 0x7fffffffu;
-        const uint32_t b = __builtin_bit_cast(uint32_t, r[i]) & 0x7fffffffu;
-        m_top = a > m_top ? a : m_top;
-        r_top = b > r_top ? b : r_top;
+    for (int i = 0; i < kEach; ++i) {
+      const float d = gv[k][i] * gs;
+      m[i] = m[i] * h[kBeta1] + d * h[kRest1];
+      v[i] = v[i] * h[kBeta2] + d * d * h[kRest2];
+    }
+    if (left < kEach) {  // zeros past the tensor's end
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i)
+        if (i >= left) m[i] = v[i] = 0.0f;
+    }
+    float r[kEach];
+    uint32_t m_top = 0, r_top = 0, v_least = ~0u;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      r[i] = adam_root(v[i]);
+      // Zero as the largest.
+      const uint32_t b = __builtin_bit_cast(uint32_t, v[i]) - 1;
+      v_least = b < v_least ? b : v_least;
+      const uint32_t rb = __builtin_bit_cast(uint32_t, r[i]);
+      r_top = rb > r_top ? rb : r_top;
+      const uint32_t mb = __builtin_bit_cast(uint32_t, m[i]) & 0x7fffffffu;
+      m_top = mb > m_top ? mb : m_top;
+    }
+    // Outside the quick root's range (2^-100 to 2^120; NaN), for the whole wave.
+    if (__ballot(v_least < 0x0d800000u - 1 || r_top >= 0x5d800000u) != 0) {
+      r_top = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        r[i] = __builtin_sqrtf(v[i]);
+        const uint32_t rb = __builtin_bit_cast(uint32_t, r[i]) & 0x7fffffffu;
+        r_top = rb > r_top ? rb : r_top;
       }
     }
-    const int64_t at = (int64_t)t.block[lo] * kAdamBlock + e;
+    // The quotient by the reciprocal, one step (2^-23) of the update at most.
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      x[i] = x[i] * h[kKeep] -
+             m[i] * __builtin_amdgcn_rcpf(r[i] * h[kInvRoot] + h[kEps]) * h[kSize];
+    const int64_t at = base + e;
     if constexpr (kBits8) {
       // All lanes of a block, those past the end with zeros.
-      const float ms = adam_scale(dpp_max16(m_top)), rs = adam_scale(dpp_max16(r_top));
+      const float scale_m = adam_scale(dpp_max16(m_top)), scale_r = adam_scale(dpp_max16(r_top));
       // The last block's lanes past the tensor's end write its codes' rest.
       if (e / kAdamBlock * kAdamBlock >= n) continue;
-      const float mi = 1.0f / ms, ri = 1.0f / rs;
-      u32x2 mc = {0u, 0u}, vc = {0u, 0u};
+      const float mi = 1.0f / scale_m, ri = 1.0f / scale_r;
+      uint32_t a[kEach], b[kEach];
 #pragma unroll
-      for (int i = 0; i < kAdamEach; ++i) {
-        const uint32_t a = adam_code<20>(fabsf(m[k][i]) * mi);
-        mc[i / 4] |= ((m[k][i] < 0.0f ? 0u - a : a) & 0xff) << (8 * (i % 4));
-        uint32_t b = adam_code<19>(r[i] * ri);
-        b = r[i] > 0.0f && b == 0 ? 1 : b;
-        vc[i / 4] |= (b & 0xff) << (8 * (i % 4));
+      for (int i = 0; i < kEach; ++i) {
+        const uint32_t sign = (uint32_t)(__builtin_bit_cast(int32_t, m[i]) >> 31);
+        a[i] = (adam_code<20>(fabsf(m[i]) * mi) ^ sign) - sign;
+        // At least 1 where r is not zero.
+        const uint32_t some = __builtin_bit_cast(uint32_t, r[i]);
+        const uint32_t least = some < 1u ? some : 1u, c = adam_code<19>(r[i] * ri);
+        b[i] = c > least ? c : least;
       }
-      *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(t.c.m) + at) = mc;
-      *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(t.c.v) + at) = vc;
+      const u32x2 mo = {adam_bytes(a[0], a[1], a[2], a[3]), adam_bytes(a[4], a[5], a[6], a[7])};
+      const u32x2 vo = {adam_bytes(b[0], b[1], b[2], b[3]), adam_bytes(b[4], b[5], b[6], b[7])};
+      *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(t.c.m) + at) = mo;
+      *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(t.c.v) + at) = vo;
       if ((threadIdx.x & 15) == 0) {
-        t.c.m_scale[at / kAdamBlock] = ms;
-        t.c.v_scale[at / kAdamBlock] = rs;
+        t.c.m_scale[at / kAdamBlock] = scale_m;
+        t.c.v_scale[at / kAdamBlock] = scale_r;
       }
     } else {
-      adam_store(static_cast<float *>(t.c.m) + at, true, 0, m[k]);
-      adam_store(static_cast<float *>(t.c.v) + at, true, 0, v[k]);
+      adam_store(static_cast<float *>(t.c.m) + at, true, 0, m);
+      adam_store(static_cast<float *>(t.c.v) + at, true, 0, v);
     }
     if (left == 0) continue;
-    const bool whole = vec && left >= kAdamEach;
-    adam_store(p + e, whole, left, pv[k]);
-    if (kCopy) adam_store(copy + e, whole, left, pv[k]);
+    const bool whole = vec && left >= kEach;
+    adam_store(p + e, whole, left, x);
+    if (kCopy) adam_store(copy + e, whole, left, x);
   }
 }
 
-// What 8-bit moments stand for.
-__global__ void __launch_bounds__(kAdamThreads) adamw_moments_kernel(AdamCommon c, int64_t blocks,
-                                                                     float *m, float *v) {
-  const int64_t groups = blocks * (kAdamBlock / kAdamEach);
-  for (int64_t i = (int64_t)blockIdx.x * kAdamThreads + threadIdx.x; i < groups;
+// What 8-bit moments stand for, four of each a lane.
+__global__ void __launch_bounds__(kAdamThreads) adamw_moments_kernel(
+    const uint32_t *m, const uint32_t *v, const float *m_scale, const float *v_scale,
+    int64_t words, floatx4 *m_out, floatx4 *v_out) {
+  for (int64_t i = (int64_t)blockIdx.x * kAdamThreads + threadIdx.x; i < words;
        i += (int64_t)gridDim.x * kAdamThreads) {
-    float a[kAdamEach], b[kAdamEach];
-    adam_moments(c, i * kAdamEach, a, b, true);
-    adam_store(m + i * kAdamEach, true, 0, a);
-    adam_store(v + i * kAdamEach, true, 0, b);
+    const uint32_t a = m[i], b = v[i];
+    const float ms = m_scale[i / (kAdamBlock / 4)], vs = v_scale[i / (kAdamBlock / 4)];
+    floatx4 x, y;
+    static_for<0, 4>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      x[j] = adam_m<j>(a, ms);
+      const float r = adam_r<j>(b, vs);
+      y[j] = r * r;
+    });
+    __builtin_nontemporal_store(x, m_out + i);
+    __builtin_nontemporal_store(y, v_out + i);
   }
 }
 
@@ -453,15 +524,13 @@ int32_t nf4s_adamw_moments(const uint8_t *m, const uint8_t *v, const float *m_sc
       !aligned(m_scale, 4) || !aligned(v_scale, 4))
     return fail(NF4S_ERR_MISALIGNED,
                 "codes must be 8-byte aligned, moments 16-byte and scales 4-byte");
-  AdamCommon c{};
-  c.m = const_cast<uint8_t *>(m);
-  c.v = const_cast<uint8_t *>(v);
-  c.m_scale = const_cast<float *>(m_scale);
-  c.v_scale = const_cast<float *>(v_scale);
-  const int64_t wgs = ceil_div(blocks * (kAdamBlock / kAdamEach), kAdamThreads);
-  const int64_t most = (int64_t)cu_slots() * 32;
+  const int64_t words = blocks * (kAdamBlock / 4), wgs = ceil_div(words, kAdamThreads);
+  const int64_t most = (int64_t)cu_slots() * 64;
   hipLaunchKernelGGL(adamw_moments_kernel, dim3((uint32_t)(wgs < most ? wgs : most)),
-                     dim3(kAdamThreads), 0, as_stream(stream), c, blocks, m_out, v_out);
+                     dim3(kAdamThreads), 0, as_stream(stream),
+                     reinterpret_cast<const uint32_t *>(m), reinterpret_cast<const uint32_t *>(v),
+                     m_scale, v_scale, words, reinterpret_cast<floatx4 *>(m_out),
+                     reinterpret_cast<floatx4 *>(v_out));
   return check_launch("adamw_moments_kernel");
 }
 
