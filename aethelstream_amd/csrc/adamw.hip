@@ -321,23 +321,39 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const AdamTable<kCo
   }
 }
 
-// What 8-bit moments stand for, four of each a lane.
+// What 8-bit moments stand for: a lane four of each at once, four times.
+constexpr int kAdamWords = 4;
 __global__ void __launch_bounds__(kAdamThreads) adamw_moments_kernel(
     const uint32_t *m, const uint32_t *v, const float *m_scale, const float *v_scale,
     int64_t words, floatx4 *m_out, floatx4 *v_out) {
-  for (int64_t i = (int64_t)blockIdx.x * kAdamThreads + threadIdx.x; i < words;
-       i += (int64_t)gridDim.x * kAdamThreads) {
-    const uint32_t a = m[i], b = v[i];
-    const float ms = m_scale[i / (kAdamBlock / 4)], vs = v_scale[i / (kAdamBlock / 4)];
-    floatx4 x, y;
-    static_for<0, 4>([&](auto J) {
-      constexpr int j = decltype(J)::value;
-      x[j] = adam_m<j>(a, ms);
-      const float r = adam_r<j>(b, vs);
-      y[j] = r * r;
-    });
-    __builtin_nontemporal_store(x, m_out + i);
-    __builtin_nontemporal_store(y, v_out + i);
+  for (int64_t first = (int64_t)blockIdx.x * kAdamThreads * kAdamWords + threadIdx.x;
+       first < words; first += (int64_t)gridDim.x * kAdamThreads * kAdamWords) {
+    uint32_t a[kAdamWords], b[kAdamWords];
+    float ms[kAdamWords], vs[kAdamWords];
+#pragma unroll
+    for (int k = 0; k < kAdamWords; ++k) {
+      const int64_t i = first + k * kAdamThreads;
+      if (i < words) {
+        a[k] = m[i];
+        b[k] = v[i];
+        ms[k] = m_scale[i / (kAdamBlock / 4)];
+        vs[k] = v_scale[i / (kAdamBlock / 4)];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAdamWords; ++k) {
+      const int64_t i = first + k * kAdamThreads;
+      if (i >= words) break;
+      floatx4 x, y;
+      static_for<0, 4>([&](auto J) {
+        constexpr int j = decltype(J)::value;
+        x[j] = adam_m<j>(a[k], ms[k]);
+        const float r = adam_r<j>(b[k], vs[k]);
+        y[j] = r * r;
+      });
+      __builtin_nontemporal_store(x, m_out + i);
+      __builtin_nontemporal_store(y, v_out + i);
+    }
   }
 }
 
@@ -524,8 +540,9 @@ int32_t nf4s_adamw_moments(const uint8_t *m, const uint8_t *v, const float *m_sc
       !aligned(m_scale, 4) || !aligned(v_scale, 4))
     return fail(NF4S_ERR_MISALIGNED,
                 "codes must be 8-byte aligned, moments 16-byte and scales 4-byte");
-  const int64_t words = blocks * (kAdamBlock / 4), wgs = ceil_div(words, kAdamThreads);
-  const int64_t most = (int64_t)cu_slots() * 64;
+  const int64_t words = blocks * (kAdamBlock / 4);
+  const int64_t wgs = ceil_div(words, kAdamThreads * kAdamWords);
+  const int64_t most = (int64_t)cu_slots() * 4096;
   hipLaunchKernelGGL(adamw_moments_kernel, dim3((uint32_t)(wgs < most ? wgs : most)),
                      dim3(kAdamThreads), 0, as_stream(stream),
                      reinterpret_cast<const uint32_t *>(m), reinterpret_cast<const uint32_t *>(v),

@@ -22,7 +22,9 @@
 // A lane holds kNP pairs of a row, both halves of the head, so a rotation needs no
 // exchange; 1 to 64 lanes hold a row and sum its squares with DPP adds.  Both
 // directions are bound by memory: 4 bytes an element forward in bf16, 6 backward
-// with norms.
+// with norms.  What is read and written once leaves the caches to others (non-temporal
+// accesses: 68 -> 62 us forward of 8192 x 72 heads of 128 in bf16, 4.9 TB/s; backward
+// 126 -> 115, as the loads of the next tile run ahead and with the shape above 102).
 #include "row_common.hpp"
 
 namespace nf4s {
@@ -30,8 +32,11 @@ namespace nf4s {
 constexpr int kRotaryThreads = 256;
 constexpr int64_t kMaxHeadSize = 1024;
 constexpr int64_t kMaxHeads = 4096;
-// Rows of a lane in flight.
-constexpr int kRotaryRows = 4;
+// Rows of a lane in flight.  The norms' backward holds two tensors and its sums: with
+// two rows of 4 + 4 elements a lane four workgroups fit a CU, which together are its
+// whole grid.  8192 x 72 heads of 128: 102 us, 108 to 112 with rows of 8 + 8, 133 with
+// five workgroups a CU, of which one waits.
+constexpr int kRotaryRows = 4, kRotaryBwdRows = 2, kRotaryBwdWgs = 4;
 // LDS for the angles of a workgroup's tokens that costs no occupancy.
 constexpr int64_t kRotaryAngleBytes = 20 << 10;
 
@@ -55,6 +60,7 @@ struct RotaryArgs {
   int32_t d, rot;
   int32_t lanes_shift;  // log2 of the lanes of a row
   int32_t iters;        // rows of a lane in a tile, up to kRotaryRows
+  int32_t angles;       // of a tile's tokens, at most
   float scale, scale_sin, eps;  // scale_sin: negative where the rotation is taken back
 };
 
@@ -119,13 +125,17 @@ struct RotaryLane {
         if constexpr (kHalf % 4 == 0) {
 #pragma unroll
           for (int i = 0; i < kHalf; i += 4) {
-            *reinterpret_cast<u32x4 *>(r.v + i) = *reinterpret_cast<const u32x4 *>(a + i);
-            *reinterpret_cast<u32x4 *>(r.v + kHalf + i) = *reinterpret_cast<const u32x4 *>(b + i);
+            *reinterpret_cast<u32x4 *>(r.v + i) =
+                __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(a + i));
+            *reinterpret_cast<u32x4 *>(r.v + kHalf + i) =
+                __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(b + i));
           }
         } else {
           static_assert(kHalf == 2, "four bf16 values");
-          *reinterpret_cast<u32x2 *>(r.v) = *reinterpret_cast<const u32x2 *>(a);
-          *reinterpret_cast<u32x2 *>(r.v + 2) = *reinterpret_cast<const u32x2 *>(b);
+          *reinterpret_cast<u32x2 *>(r.v) =
+              __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(a));
+          *reinterpret_cast<u32x2 *>(r.v + 2) =
+              __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(b));
         }
       } else {
 #pragma unroll
@@ -189,12 +199,16 @@ struct RotaryLane {
       if constexpr (kHalf % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < kHalf; i += 4) {
-          *reinterpret_cast<u32x4 *>(p + i) = *reinterpret_cast<const u32x4 *>(r.v + i);
-          *reinterpret_cast<u32x4 *>(q + i) = *reinterpret_cast<const u32x4 *>(r.v + kHalf + i);
+          __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(r.v + i),
+                                      reinterpret_cast<u32x4 *>(p + i));
+          __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(r.v + kHalf + i),
+                                      reinterpret_cast<u32x4 *>(q + i));
         }
       } else {
-        *reinterpret_cast<u32x2 *>(p) = *reinterpret_cast<const u32x2 *>(r.v);
-        *reinterpret_cast<u32x2 *>(q) = *reinterpret_cast<const u32x2 *>(r.v + 2);
+        __builtin_nontemporal_store(*reinterpret_cast<const u32x2 *>(r.v),
+                                    reinterpret_cast<u32x2 *>(p));
+        __builtin_nontemporal_store(*reinterpret_cast<const u32x2 *>(r.v + 2),
+                                    reinterpret_cast<u32x2 *>(q));
       }
     } else {
 #pragma unroll
@@ -216,6 +230,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
   using Lane = RotaryLane<T, kNP, kVec, kAdj>;
   using Raw = typename Lane::Raw;
   constexpr bool kNorm = kMode != kTurn, kBwd = kMode == kNormTurnBwd;
+  constexpr int kRows = kBwd ? kRotaryBwdRows : kRotaryRows;
   extern __shared__ __attribute__((aligned(16))) f32x2 angles[];  // cos, sin; then dw's sums
   const bool is_k = (int)blockIdx.x >= a.side[0].wgs;
   const RotarySide s = is_k ? a.side[1] : a.side[0];
@@ -240,103 +255,143 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
     }
   }
   const float inv_d = 1.0f / (float)a.d;
-
   const int tile_rows = groups * a.iters;
-#pragma unroll 1
-  for (int64_t row0 = (int64_t)wg * tile_rows; row0 < s.rows; row0 += (int64_t)s.wgs * tile_rows) {
-    const int64_t t0 = row0 / s.heads;
-    const uint32_t h0 = (uint32_t)(row0 - t0 * s.heads);
-    const int rows = s.rows - row0 < tile_rows ? (int)(s.rows - row0) : tile_rows;
-    int64_t token[kRotaryRows];
-    int head[kRotaryRows], at[kRotaryRows];
-    Raw x[kRotaryRows], dy[kRotaryRows];
-#pragma unroll
-    for (int i = 0; i < kRotaryRows; ++i) {
-      const int r = group + i * groups;
-      const uint32_t local = h0 + (uint32_t)r;
-      const uint32_t t = (uint32_t)(((uint64_t)local * s.magic) >> 31);
-      at[i] = i < a.iters && r < rows ? (int)t : -1;
-      head[i] = (int)(local - t * (uint32_t)s.heads);
-      token[i] = t0 + t;
-      if (at[i] >= 0) {
-        x[i] = lane.load(static_cast<const T *>(s.x) + token[i] * s.x_token + head[i] * s.x_head);
-        if (kBwd)
-          dy[i] = lane.load(static_cast<const T *>(s.dy) + token[i] * s.dy_token +
-                            head[i] * s.dy_head);
-      }
-    }
-    // The angles of the tile's tokens.
-    const int tokens = (int)(((uint64_t)(h0 + (uint32_t)rows - 1) * s.magic) >> 31) + 1;
-    __syncthreads();  // the last tile's are no longer read
-    for (int i = (int)threadIdx.x; i < tokens * half; i += kRotaryThreads) {
-      const int t = i / half, p = i - t * half;
-      const uint64_t turn = (uint64_t)a.positions[t0 + t] * (uint64_t)a.turns[p];
-      float sn, cs;
-      sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &sn, &cs);
-      angles[i] = (f32x2){cs * a.scale, sn * a.scale_sin};
-    }
-    __syncthreads();
+  const int64_t stride = (int64_t)s.wgs * tile_rows;
 
+  // Rows of a tile, `group` and every `groups`-th behind it.
+  struct Tile {
+    Raw x[kRows], dy[kBwd ? kRows : 1];
+  };
+  struct Place {
+    int64_t token;  // of the tile's first row
+    uint32_t head;
+    int rows;
+  };
+  auto place = [&](int64_t row0) {
+    Place p;
+    p.token = row0 / s.heads;
+    p.head = (uint32_t)(row0 - p.token * s.heads);
+    p.rows = s.rows - row0 < tile_rows ? (int)(s.rows - row0) : tile_rows;
+    return p;
+  };
+  // Token (from the tile's first) and head of its row r.
+  auto find = [&](const Place &p, int r, int &head) {
+    const uint32_t local = p.head + (uint32_t)r;
+    const uint32_t t = (uint32_t)(((uint64_t)local * s.magic) >> 31);
+    head = (int)(local - t * (uint32_t)s.heads);
+    return (int)t;
+  };
+  auto load = [&](Tile &v, const Place &p) {
 #pragma unroll
-    for (int i = 0; i < kRotaryRows; ++i) {
-      if (at[i] < 0) continue;
+    for (int i = 0; i < kRows; ++i) {
+      const int r = group + i * groups;
+      if (i >= a.iters || r >= p.rows) continue;
+      int head;
+      const int64_t token = p.token + find(p, r, head);
+      v.x[i] = lane.load(static_cast<const T *>(s.x) + token * s.x_token + head * s.x_head);
+      if constexpr (kBwd)
+        v.dy[i] = lane.load(static_cast<const T *>(s.dy) + token * s.dy_token + head * s.dy_head);
+    }
+  };
+  // The angles of its tokens.
+  auto turn = [&](const Place &p, f32x2 *to) {
+    int head;
+    const int tokens = find(p, p.rows - 1, head) + 1;
+    for (int i = (int)threadIdx.x; i < tokens * half; i += kRotaryThreads) {
+      const int t = i / half, c = i - t * half;
+      const uint64_t at = (uint64_t)a.positions[p.token + t] * (uint64_t)a.turns[c];
+      float sn, cs;
+      sincospif((float)(int32_t)(at >> 32) * 0x1p-31f, &sn, &cs);
+      to[i] = (f32x2){cs * a.scale, sn * a.scale_sin};
+    }
+  };
+  auto work = [&](const Tile &v, const Place &p, const f32x2 *angles) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int r = group + i * groups;
+      if (i >= a.iters || r >= p.rows) continue;
+      int head;
+      const int t = find(p, r, head);
       float va[kNP], vb[kNP], ya[kNP], yb[kNP];
-      const f32x2 *turned = angles + at[i] * half;
-      if constexpr (!kBwd) {
-        Lane::values(x[i], va, vb);
-        if constexpr (kNorm) {
-          float sum = 0.0f;
+      const f32x2 *turned = angles + t * half;
+      if constexpr (kBwd)
+        Lane::values(v.dy[i], va, vb);
+      else
+        Lane::values(v.x[i], va, vb);
+      if constexpr (kMode == kNormTurn) {
+        float sum = 0.0f;
 #pragma unroll
-          for (int j = 0; j < kNP; ++j) sum += va[j] * va[j] + vb[j] * vb[j];
-          const float inv = 1.0f / __builtin_sqrtf(lanes_sum(sum, a.lanes_shift) * inv_d + a.eps);
-#pragma unroll
-          for (int j = 0; j < kNP; ++j) {
-            va[j] *= inv * wa[j];
-            vb[j] *= inv * wb[j];
-          }
-        }
+        for (int j = 0; j < kNP; ++j)
+          sum = __builtin_fmaf(va[j], va[j], __builtin_fmaf(vb[j], vb[j], sum));
+        const float inv = 1.0f / __builtin_sqrtf(lanes_sum(sum, a.lanes_shift) * inv_d + a.eps);
 #pragma unroll
         for (int j = 0; j < kNP; ++j) {
-          ya[j] = va[j];
-          yb[j] = vb[j];
-          if (lane.turns(j)) {
-            const f32x2 c = turned[lane.pair(j)];
-            ya[j] = va[j] * c.x - vb[j] * c.y;
-            yb[j] = vb[j] * c.x + va[j] * c.y;
-          }
+          va[j] *= inv * wa[j];
+          vb[j] *= inv * wb[j];
         }
-      } else {
-        Lane::values(dy[i], va, vb);
+      }
 #pragma unroll
-        for (int j = 0; j < kNP; ++j) {
-          ya[j] = va[j];
-          yb[j] = vb[j];
-          if (lane.turns(j)) {
-            const f32x2 c = turned[lane.pair(j)];
-            ya[j] = va[j] * c.x - vb[j] * c.y;
-            yb[j] = vb[j] * c.x + va[j] * c.y;
-          }
+      for (int j = 0; j < kNP; ++j) {
+        ya[j] = va[j];
+        yb[j] = vb[j];
+        if (lane.turns(j)) {
+          const f32x2 c = turned[lane.pair(j)];
+          ya[j] = __builtin_fmaf(va[j], c.x, -(vb[j] * c.y));
+          yb[j] = __builtin_fmaf(vb[j], c.x, va[j] * c.y);
         }
-        Lane::values(x[i], va, vb);
+      }
+      if constexpr (kBwd) {
+        Lane::values(v.x[i], va, vb);
         float sum = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int j = 0; j < kNP; ++j) {
-          sum += va[j] * va[j] + vb[j] * vb[j];
-          dot += ya[j] * wa[j] * va[j] + yb[j] * wb[j] * vb[j];
+          sum = __builtin_fmaf(va[j], va[j], __builtin_fmaf(vb[j], vb[j], sum));
+          dot = __builtin_fmaf(ya[j] * wa[j], va[j], __builtin_fmaf(yb[j] * wb[j], vb[j], dot));
         }
         const float inv = 1.0f / __builtin_sqrtf(lanes_sum(sum, a.lanes_shift) * inv_d + a.eps);
-        const float mean = lanes_sum(dot, a.lanes_shift) * inv * inv_d;
+        // dx = (e - x (e x) / (d rms^2)) / rms
+        const float back = lanes_sum(dot, a.lanes_shift) * inv * inv * inv_d;
 #pragma unroll
         for (int j = 0; j < kNP; ++j) {
-          const float xa = va[j] * inv, xb = vb[j] * inv;
-          sa[j] += ya[j] * xa;
-          sb[j] += yb[j] * xb;
-          ya[j] = (ya[j] * wa[j] - xa * mean) * inv;
-          yb[j] = (yb[j] * wb[j] - xb * mean) * inv;
+          const float na = ya[j] * inv, nb = yb[j] * inv;
+          sa[j] = __builtin_fmaf(na, va[j], sa[j]);
+          sb[j] = __builtin_fmaf(nb, vb[j], sb[j]);
+          ya[j] = __builtin_fmaf(va[j], -back * inv, na * wa[j]);
+          yb[j] = __builtin_fmaf(vb[j], -back * inv, nb * wb[j]);
         }
       }
-      lane.store(static_cast<T *>(s.out) + token[i] * s.out_token + head[i] * s.out_head, ya, yb);
+      lane.store(static_cast<T *>(s.out) + (p.token + t) * s.out_token + head * s.out_head, ya, yb);
     }
+  };
+
+  // The next tile's rows and angles are on their way while one is worked on.
+  f32x2 *second = angles + a.angles;
+  int64_t row = (int64_t)wg * tile_rows;
+  Tile v0, v1;
+  Place p0, p1;
+  if (row < s.rows) {
+    p0 = place(row);
+    load(v0, p0);
+    turn(p0, angles);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (; row < s.rows; row += 2 * stride) {
+    if (row + stride < s.rows) {
+      p1 = place(row + stride);
+      load(v1, p1);
+      turn(p1, second);
+    }
+    work(v0, p0, angles);
+    __syncthreads();
+    if (row + stride >= s.rows) break;
+    if (row + 2 * stride < s.rows) {
+      p0 = place(row + 2 * stride);
+      load(v0, p0);
+      turn(p0, angles);
+    }
+    work(v1, p1, second);
+    __syncthreads();
   }
 
   if constexpr (kBwd) {
@@ -393,12 +448,15 @@ struct RotaryPlan {
   bool vec;
   int lanes_shift, iters;
   int32_t wgs[2];
+  int32_t angles;
   int64_t lds;
 };
 
-// Workgroups of the norms' backward, which each write d sums: four a CU.
+// Workgroups of a launch.  The norms' backward, whose workgroups each write d sums:
+// as many as run at once.  The others: one for each tile (8192 x 72 heads of 128: 61
+// us; 69 to 82 with fewer that go on to further tiles).
 static int64_t rotary_most(bool sums) {
-  return sums ? (int64_t)cu_slots() * 4 : kMaxThreadsPerLaunch / kRotaryThreads / 2;
+  return sums ? (int64_t)cu_slots() * kRotaryBwdWgs : kMaxThreadsPerLaunch / kRotaryThreads / 2;
 }
 
 static RotaryPlan rotary_plan(int64_t m, int64_t d, int64_t rot, const int64_t (&heads)[2],
@@ -407,7 +465,7 @@ static RotaryPlan rotary_plan(int64_t m, int64_t d, int64_t rot, const int64_t (
   const int64_t pairs = d / 2;
   // Vector loads of 8 or 4 pairs where rows, halves and what is not turned are
   // whole ones.
-  int np = aligned_pairs;
+  int np = sums && aligned_pairs > 4 && pairs <= 256 ? 4 : aligned_pairs;
   while (np > 1 && (rot % (2 * np) != 0 || d % (2 * np) != 0 || pairs / np > 64)) np /= 2;
   p.vec = np >= 4;
   int64_t lanes;
@@ -426,11 +484,12 @@ static RotaryPlan rotary_plan(int64_t m, int64_t d, int64_t rot, const int64_t (
   };
   const int64_t least = heads[1] > 0 && heads[1] < heads[0] ? heads[1] : heads[0];
   const int64_t rows = m * (heads[0] + heads[1]);
-  p.iters = kRotaryRows;
+  p.iters = sums ? kRotaryBwdRows : kRotaryRows;
   while (p.iters > 1 && (tokens(least, p.iters) * (rot / 2) * 8 > kRotaryAngleBytes ||
                          rows < groups * p.iters * 2 * cu_slots()))
     p.iters /= 2;
-  p.lds = tokens(least, p.iters) * (rot / 2) * 8;
+  p.angles = (int32_t)(tokens(least, p.iters) * (rot / 2));
+  p.lds = 2 * (int64_t)p.angles * 8;
   if (sums && p.lds < 16 * d) p.lds = 16 * d;
   const int64_t tile = groups * p.iters, most = rotary_most(sums);
   for (int i = 0; i < 2; ++i) {
@@ -512,6 +571,7 @@ static RotaryArgs rotary_args(const RotaryPlan &p, int64_t m, int64_t d, int64_t
   a.rot = (int32_t)rot;
   a.lanes_shift = p.lanes_shift;
   a.iters = p.iters;
+  a.angles = p.angles;
   a.scale = scale;
   a.scale_sin = scale_sin;
   a.eps = eps;
