@@ -245,21 +245,8 @@ struct LpSelect {
 
 // Keys a wave ranks at once: two a lane.
 constexpr int kLpList = 128;
-// Half tiles whose logits are looked at; the lanes name them.
-constexpr int kLpHeld = 64;
-
-// The k-th largest of the lanes' values (0 if it has none): below it are none of the
-// k largest of all values whose maxima the lanes hold.
-__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k, int lane) {
-  int ahead = 0;
-#pragma unroll 8
-  for (int i = 0; i < 64; ++i) {
-    const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)v, i);
-    ahead += o > v || (o == v && i < lane) ? 1 : 0;
-  }
-  const uint64_t at = __ballot(ahead == k - 1);
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, __builtin_ctzll(at));
-}
+// Half tiles whose logits are looked at, and those of them at once.
+constexpr int kLpHeld = 64, kLpAt = 32;
 
 // Writes visible to the wave's other lanes.
 __device__ __forceinline__ void wave_lds_fence() {
@@ -268,28 +255,58 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// A wave's LDS, in front of the half tiles' maxima.
+struct LpWave {
+  uint64_t list[kLpList];
+  u32x4 lanes[16];  // a value of every lane
+  int32_t chosen[kLpHeld];
+  uint32_t count[4];
+};
+
+// The k-th largest of the lanes' values (0 if fewer have one): below it are none of
+// the k largest of all values whose maxima the lanes hold.
+__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k, int lane, LpWave &w) {
+  reinterpret_cast<uint32_t *>(w.lanes)[lane] = v;
+  wave_lds_fence();
+  int ahead = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const u32x4 o = w.lanes[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ahead += o[j] > v ? 1 : 0;
+  }
+  // The least of those with fewer than k ahead, as the largest complement.
+  uint32_t c = ahead < k ? ~v : 0;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)c, off, 64);
+    c = o > c ? o : c;
+  }
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)~c);
+}
+
 // One wave a token.  Twice the same step, over the half tiles' maxima and over the
 // logits of those that are left: the k-th largest of the 64 lanes' own maxima is
-// reached by k values at least, so what lies below is out; of those equal to it the
-// first k are enough.  What remains, about k, is ranked by counting, together with
-// the k best of the pieces before.  The maxima (ordered integers) and the list are in
-// LDS.  Should more than kLpHeld half tiles or kLpList values remain, which takes
-// logits sorted against the lanes, k rounds over all of them find the k best.
+// reached by k values at least, so what lies below is out.  What remains, about k, is
+// ranked by counting, together with the k best of the pieces before.  Where too many
+// are left because they are equal, the first k by their index are enough and are
+// taken in that order; where they are not equal (which takes logits sorted against
+// the lanes), k rounds over all of them find the k best.
 __global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
-  extern __shared__ uint64_t lp_lds[];
+  extern __shared__ __attribute__((aligned(16))) char lp_lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
   if (row >= a.M) return;
   const int rounds = (a.slices + 63) / 64;
-  uint64_t *list = lp_lds + wave * (kLpList + kLpHeld / 2 + 32 * rounds);
-  int32_t *chosen = reinterpret_cast<int32_t *>(list + kLpList);
-  uint32_t *maxima = reinterpret_cast<uint32_t *>(chosen + kLpHeld);
+  LpWave &w = *reinterpret_cast<LpWave *>(lp_lds + wave * (sizeof(LpWave) + 256 * rounds));
+  uint32_t *maxima = reinterpret_cast<uint32_t *>(&w + 1);
   uint64_t *best = a.best + row * a.k;
   const uint64_t before = !a.first && lane < a.k ? best[lane] : 0;
   const uint32_t least = a.first ? 0 : (uint32_t)(best[a.k - 1] >> 32);
   const uint64_t below = (1ull << lane) - 1;
   const LpSegment g0 = a.seg[0], g1 = a.seg[1];
+  if (lane < 4) w.count[lane] = 0;
 
   uint32_t top = 0;
   for (int i0 = 0; i0 < rounds; i0 += 8) {
@@ -313,93 +330,158 @@ __global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
     }
   }
   if (__ballot(top != 0) == 0) return;  // the pieces before had all
-  uint32_t floor = kth_of_lanes(top, a.k, lane);
+  uint32_t floor = kth_of_lanes(top, a.k, lane, w);
   if (floor == 0) floor = 1;
 
-  // The half tiles that are left, by their index.
-  int count = 0, equal = 0;
-  for (int i = 0; i < rounds; ++i) {
-    const uint32_t o = maxima[64 * i + lane];
-    const uint64_t same = __ballot(o == floor);
-    const bool in = o > floor || (o == floor && equal + __popcll(same & below) < a.k);
-    const uint64_t all = __ballot(in);
-    const int at = count + __popcll(all & below);
-    if (in && at < kLpHeld) chosen[at] = 64 * i + lane;
-    count += __popcll(all);
-    equal += __popcll(same);
+  // The half tiles that are left.
+  int mine = 0;
+  for (int i = 0; i < rounds; ++i) mine += maxima[64 * i + lane] >= floor ? 1 : 0;
+  if (mine > 0) {
+    int at = (int)atomicAdd(&w.count[0], (uint32_t)mine);
+    for (int i = 0; i < rounds; ++i)
+      if (maxima[64 * i + lane] >= floor) {
+        if (at < kLpHeld) w.chosen[at] = 64 * i + lane;
+        ++at;
+      }
   }
   wave_lds_fence();
+  int count = __builtin_amdgcn_readfirstlane((int)w.count[0]);
+  // The same by their index, and of those equal to the bound the first k.
+  auto pick_in_order = [&] {
+    int equal = 0;
+    count = 0;
+    for (int i = 0; i < rounds; ++i) {
+      const uint32_t o = maxima[64 * i + lane];
+      const uint64_t same = __ballot(o == floor);
+      const bool in = o > floor || (o == floor && equal + __popcll(same & below) < a.k);
+      const uint64_t all = __ballot(in);
+      const int at = count + __popcll(all & below);
+      if (in && at < kLpHeld) w.chosen[at] = 64 * i + lane;
+      count += __popcll(all);
+      equal += __popcll(same);
+    }
+    wave_lds_fence();
+  };
+  const uint32_t bound = floor;  // of the half tiles
+  if (count > kLpHeld) pick_in_order();
 
-  int n = 0;
+  // Half tile s: its first column, how many it has, its first logit.
+  auto half_tile = [&](int s, uint32_t &column, int &wide, const float *&z) {
+    const bool second = s >= g0.slices;
+    const int at = second ? s - g0.slices : s, width = second ? g1.width : g0.width;
+    const int left = (second ? g1.columns : g0.columns) - at * width;
+    column = (second ? g1.column : g0.column) + (uint32_t)(at * width);
+    wide = left < width ? left : width;
+    z = (second ? g1.z : g0.z) + ((int64_t)at * a.M + row) * width;
+  };
   if (count <= kLpHeld) {
-    const int32_t mine = lane < count ? chosen[lane & (kLpHeld - 1)] : 0;
-    // The logits of eight half tiles from j on, ordered, and their first columns; all
-    // loads before the first use.
-    struct Eight {
-      uint32_t order[16], column[8];
+    // 32 chosen half tiles from j on, two at a time: a lane has four columns of one.
+    struct Logits {
+      uint32_t order[kLpAt / 2][4], column[kLpAt / 2];
     };
-    auto eight = [&](int j) {
-      Eight e;
-      float v[16];
-      int wide[8];
+    auto read = [&](int j, Logits &e) {
+      floatx4 v[kLpAt / 2];
+      int left[kLpAt / 2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int s = __builtin_amdgcn_readlane(mine, j + i);  // of lanes past `count`: 0
-        const bool second = s >= g0.slices;
-        const int at = second ? s - g0.slices : s, width = second ? g1.width : g0.width;
-        const int left = (second ? g1.columns : g0.columns) - at * width;
-        wide[i] = j + i >= count ? 0 : left < width ? left : width;
-        e.column[i] = (second ? g1.column : g0.column) + (uint32_t)(at * width);
-        const float *z = (second ? g1.z : g0.z) + ((int64_t)at * a.M + row) * width;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v[2 * i + h] = 64 * h + lane < wide[i] ? z[64 * h + lane] : 0.0f;
+      for (int i = 0; i < kLpAt / 2; ++i) {
+        left[i] = 0;
+        if (j + 2 * i >= count) continue;
+        const int c = j + 2 * i + (lane >> 5);
+        const float *z;
+        int wide;
+        half_tile(w.chosen[c < count ? c : 0], e.column[i], wide, z);
+        e.column[i] += 4 * (uint32_t)(lane & 31);
+        left[i] = c < count ? wide - 4 * (lane & 31) : 0;
+        // (The rows of a half tile are whole, past the last column with -inf.)
+        if (left[i] > 0) v[i] = *reinterpret_cast<const floatx4 *>(z + 4 * (lane & 31));
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        e.order[i] = 64 * (i % 2) + lane < wide[i / 2] ? lp_order(v[i]) : 0;
-      return e;
-    };
-    top = 0;
-#pragma unroll 1
-    for (int j = 0; j < count; j += 8) {
-      const Eight e = eight(j);
+      for (int i = 0; i < kLpAt / 2; ++i)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = e.order[i] > top ? e.order[i] : top;
+        for (int q = 0; q < 4; ++q) e.order[i][q] = q < left[i] ? lp_order(v[i][q]) : 0;
+    };
+    auto most = [&](const Logits &e) {
+#pragma unroll
+      for (int i = 0; i < kLpAt / 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) top = e.order[i][q] > top ? e.order[i][q] : top;
+    };
+    Logits e;
+    top = 0;
+    if (count > kLpAt) {
+      read(kLpAt, e);
+      most(e);
     }
-    const uint32_t kth = kth_of_lanes(top, a.k, lane);
+    read(0, e);
+    most(e);
+    const uint32_t kth = kth_of_lanes(top, a.k, lane, w);
     floor = kth > floor ? kth : floor;
     // Later columns lose a tie with the pieces before.
     if (floor <= least) floor = least + 1;
-    equal = 0;
-#pragma unroll 1
-    for (int j = 0; j < count; j += 8) {
-      const Eight e = eight(j);
+    auto gather = [&](const Logits &e) {
+      mine = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t o = e.order[i];
-        if (__ballot(o >= floor) == 0) continue;
-        const uint64_t same = __ballot(o == floor);
-        const bool in = o > floor || (o == floor && equal + __popcll(same & below) < a.k);
-        const uint64_t all = __ballot(in);
-        const int to = n + __popcll(all & below);
-        if (in && to < kLpList)
-          list[to] = lp_key(o, e.column[i / 2] + 64 * (uint32_t)(i % 2) + (uint32_t)lane);
-        n += __popcll(all);
-        equal += __popcll(same);
+      for (int i = 0; i < kLpAt / 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mine += e.order[i][q] >= floor ? 1 : 0;
+      int at = 0;
+      if (mine > 0) at = (int)atomicAdd(&w.count[1], (uint32_t)mine);
+#pragma unroll
+      for (int i = 0; i < kLpAt / 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const bool in = e.order[i][q] >= floor;
+          if (__ballot(in) == 0) continue;
+          if (in && at < kLpList) w.list[at] = lp_key(e.order[i][q], e.column[i] + (uint32_t)q);
+          at += in ? 1 : 0;
+        }
+    };
+    gather(e);
+    if (count > kLpAt) {
+      read(kLpAt, e);
+      gather(e);
+    }
+    wave_lds_fence();
+    int n = __builtin_amdgcn_readfirstlane((int)w.count[1]);
+    const uint64_t had = __ballot(before != 0);
+    if (n + __popcll(had) > kLpList) {
+      // In the order of the columns, of those equal to the bound the first k.
+      const uint32_t f = floor;
+      floor = bound;
+      pick_in_order();
+      floor = f;
+      n = 0;
+      int equal = 0;
+      for (int j = 0; j < count && j < kLpHeld; ++j) {
+        uint32_t column;
+        int wide;
+        const float *z;
+        half_tile(__builtin_amdgcn_readfirstlane(w.chosen[j]), column, wide, z);
+        for (int c = lane; c < (wide + 63) / 64 * 64; c += 64) {
+          const uint32_t o = c < wide ? lp_order(z[c]) : 0;
+          const uint64_t same = __ballot(o == floor);
+          const bool in = o > floor || (o == floor && equal + __popcll(same & below) < a.k);
+          const uint64_t all = __ballot(in);
+          const int at = n + __popcll(all & below);
+          if (in && at < kLpList) w.list[at] = lp_key(o, column + (uint32_t)c);
+          n += __popcll(all);
+          equal += __popcll(same);
+        }
       }
+      if (count > kLpHeld) n = kLpList + 1;
     }
     // The pieces before.
-    const uint64_t had = __ballot(before != 0);
-    const int to = n + __popcll(had & below);
-    if (before != 0 && to < kLpList) list[to] = before;
+    const int at = n + __popcll(had & below);
+    if (before != 0 && at < kLpList) w.list[at] = before;
     n += __popcll(had);
     wave_lds_fence();
     if (n <= kLpList) {
-      const uint64_t key[2] = {lane < n ? list[lane] : 0, 64 + lane < n ? list[64 + lane] : 0};
+      const uint64_t key[2] = {lane < n ? w.list[lane] : 0,
+                               64 + lane < n ? w.list[64 + lane] : 0};
       int ahead[2] = {0, 0};
 #pragma unroll 8
       for (int i = 0; i < n; ++i) {
-        const uint64_t o = list[i];
+        const uint64_t o = w.list[i];
         ahead[0] += o > key[0] ? 1 : 0;
         ahead[1] += o > key[1] ? 1 : 0;
       }
@@ -418,14 +500,13 @@ __global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
     for (int s = 0; s < a.slices; ++s) {
       const uint32_t o = maxima[s];
       if (o == 0 || o < floor) continue;
-      const bool second = s >= g0.slices;
-      const int at = second ? s - g0.slices : s, width = second ? g1.width : g0.width;
-      const int c = at * width, columns = second ? g1.columns : g0.columns;
-      const uint32_t column = (second ? g1.column : g0.column) + (uint32_t)c;
-      const float *z = (second ? g1.z : g0.z) + ((int64_t)at * a.M + row) * width;
-      for (int e = lane; e < width && c + e < columns; e += 64) {
-        const uint32_t order = lp_order(z[e]);
-        const uint64_t key = order <= least ? 0 : lp_key(order, column + e);
+      uint32_t column;
+      int wide;
+      const float *z;
+      half_tile(s, column, wide, z);
+      for (int c = lane; c < wide; c += 64) {
+        const uint32_t order = lp_order(z[c]);
+        const uint64_t key = order <= least ? 0 : lp_key(order, column + (uint32_t)c);
         if (key < last && key > own) own = key;
       }
     }
@@ -721,7 +802,7 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
         sel.slices = (int32_t)slices;
         sel.first = v0 == 0;
         sel.best = best;
-        const int64_t lds = 8 * kLpList + 4 * kLpHeld + 4 * ((slices + 63) / 64 * 64);
+        const int64_t lds = (int64_t)sizeof(LpWave) + (slices + 63) / 64 * 256;
         const int64_t fit = kLpSelectLds / lds, waves = fit < 4 ? (fit < 1 ? 1 : fit) : 4;
         hipLaunchKernelGGL(lp_select_kernel, dim3((uint32_t)ceil_to(a.M, waves)),
                            dim3((uint32_t)(64 * waves)), (uint32_t)(waves * lds), s, sel);
