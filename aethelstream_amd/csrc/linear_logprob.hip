@@ -285,21 +285,15 @@ __device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k, int lane, Lp
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)~c);
 }
 
-// One wave a token.  Twice the same step, over the half tiles' maxima and over the
+// The alternatives of a token, by one wave.  Twice the same step, over the half tiles' maxima and over the
 // logits of those that are left: the k-th largest of the 64 lanes' own maxima is
 // reached by k values at least, so what lies below is out.  What remains, about k, is
 // ranked by counting, together with the k best of the pieces before.  Where too many
 // are left because they are equal, the first k by their index are enough and are
 // taken in that order; where they are not equal (which takes logits sorted against
 // the lanes), k rounds over all of them find the k best.
-__global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
-  extern __shared__ __attribute__((aligned(16))) char lp_lds[];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
-  if (row >= a.M) return;
+__device__ __forceinline__ void lp_select(const LpSelect &a, int64_t row, int lane, LpWave &w) {
   const int rounds = (a.slices + 63) / 64;
-  LpWave &w = *reinterpret_cast<LpWave *>(lp_lds + wave * (sizeof(LpWave) + 256 * rounds));
   uint32_t *maxima = reinterpret_cast<uint32_t *>(&w + 1);
   uint64_t *best = a.best + row * a.k;
   const uint64_t before = !a.first && lane < a.k ? best[lane] : 0;
@@ -516,6 +510,16 @@ __global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
   }
 }
 
+// One wave a token.
+__global__ void __launch_bounds__(256) lp_select_kernel(const LpSelect a) {
+  extern __shared__ __attribute__((aligned(16))) char lp_lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
+  if (row >= a.M) return;
+  const int bytes = (int)sizeof(LpWave) + (a.slices + 63) / 64 * 256;
+  lp_select(a, row, threadIdx.x & 63, *reinterpret_cast<LpWave *>(lp_lds + wave * bytes));
+}
+
 struct LpJoin {
   const floatx2 *part;
   const float *ent, *zt;
@@ -528,58 +532,43 @@ struct LpJoin {
   int64_t *top_ids;
 };
 
-// Joins a token's partial sums, as ce_join_kernel: 256 / kTokens threads a token take
-// every so many slices, then meet in a fixed order.
-template <int kTokens>
-__global__ void __launch_bounds__(256) lp_join_kernel(const LpJoin a) {
-  constexpr int kGroups = 256 / kTokens;
-  __shared__ float lds[3][kGroups][kTokens];
-  struct Sums {
-    float top, sum, ent;
-  };
-  const int tok = threadIdx.x % kTokens, grp = threadIdx.x / kTokens;
-  const int64_t row = (int64_t)blockIdx.x * kTokens + tok;
-  auto join = [](const Sums &x, const Sums &y) {
-    const float top = fmaxf(x.top, y.top);
-    const float ref = top == -__builtin_inff() ? 0.0f : top;
-    const float dx = lp_floor((x.top - ref) * kLog2e), dy = lp_floor((y.top - ref) * kLog2e);
-    const float ex = __builtin_amdgcn_exp2f(dx), ey = __builtin_amdgcn_exp2f(dy);
-    return Sums{top, x.sum * ex + y.sum * ey,
+// Maximum, sum of exponentials and sum of e y of some of a token's logits.
+struct LpSums {
+  float top, sum, ent;
+};
+__device__ __forceinline__ LpSums lp_none() { return LpSums{-__builtin_inff(), 0.0f, 0.0f}; }
+__device__ __forceinline__ LpSums lp_joined(const LpSums &x, const LpSums &y) {
+  const float top = fmaxf(x.top, y.top);
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  const float dx = lp_floor((x.top - ref) * kLog2e), dy = lp_floor((y.top - ref) * kLog2e);
+  const float ex = __builtin_amdgcn_exp2f(dx), ey = __builtin_amdgcn_exp2f(dy);
+  return LpSums{top, x.sum * ex + y.sum * ey,
                 (x.ent + dx * x.sum) * ex + (y.ent + dy * y.sum) * ey};
-  };
-  const Sums none{-__builtin_inff(), 0.0f, 0.0f};
-  Sums s = none;
-  if (row < a.M)
-    for (int i = grp; i < a.slices; i += 4 * kGroups) {
-      Sums v[4];
+}
+// Half tiles first, first + step, .. of a token, four loads ahead.
+__device__ __forceinline__ LpSums lp_column(const LpJoin &a, int64_t row, int first, int step) {
+  LpSums s = lp_none();
+  for (int i = first; i < a.slices; i += 4 * step) {
+    LpSums v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = i + j * kGroups;
-        v[j] = none;
-        if (n < a.slices) {
-          const floatx2 p = a.part[(int64_t)n * a.M + row];
-          v[j] = Sums{p.x, p.y, a.ent[(int64_t)n * a.M + row]};
-        }
+    for (int j = 0; j < 4; ++j) {
+      const int n = i + j * step;
+      v[j] = lp_none();
+      if (n < a.slices) {
+        const floatx2 p = a.part[(int64_t)n * a.M + row];
+        v[j] = LpSums{p.x, p.y, a.ent[(int64_t)n * a.M + row]};
       }
-      s = join(s, join(join(v[0], v[1]), join(v[2], v[3])));
     }
-  auto put = [&](const Sums &v) {
-    lds[0][grp][tok] = v.top;
-    lds[1][grp][tok] = v.sum;
-    lds[2][grp][tok] = v.ent;
-  };
-  auto get = [&](int g) { return Sums{lds[0][g][tok], lds[1][g][tok], lds[2][g][tok]}; };
-  put(s);
-#pragma unroll
-  for (int half = kGroups / 2; half >= 1; half /= 2) {
-    __syncthreads();
-    if (grp < half) put(join(get(grp), get(grp + half)));
+    s = lp_joined(s, lp_joined(lp_joined(v[0], v[1]), lp_joined(v[2], v[3])));
   }
-  __syncthreads();
-  if (row >= a.M) return;
-  s = get(0);
+  return s;
+}
+// A token's results by threads `first`, first + step, .. of the alternatives, the
+// first one of which has the rest.
+__device__ __forceinline__ void lp_results(const LpJoin &a, int64_t row, const LpSums &s, int first,
+                                           int step) {
   const float log_sum = __builtin_amdgcn_logf(s.sum) * kLn2;
-  if (grp == 0) {
+  if (first == 0) {
     a.lse[row] = s.top + log_sum;
     a.entropy[row] = log_sum - s.ent / s.sum * kLn2;
     const int64_t t = a.targets[row];
@@ -588,11 +577,51 @@ __global__ void __launch_bounds__(256) lp_join_kernel(const LpJoin a) {
       v = t < 0 || t >= a.V ? __builtin_nanf("") : (a.zt[row] - s.top) - log_sum;
     a.logp[row] = v;
   }
-  for (int i = grp; i < a.k; i += kGroups) {
+  for (int i = first; i < a.k; i += step) {
     const uint64_t key = a.best[row * a.k + i];
     a.top_ids[row * a.k + i] = (int64_t)(uint32_t)~(uint32_t)key;
     a.top_logp[row * a.k + i] = (lp_value((uint32_t)(key >> 32)) - s.top) - log_sum;
   }
+}
+
+// Joins a token's partial sums: 32 threads a token take every 32nd half tile, then
+// meet in a fixed order.
+constexpr int kLpTokens = 8;
+__global__ void __launch_bounds__(256) lp_join_kernel(const LpJoin a) {
+  constexpr int kGroups = 256 / kLpTokens;
+  __shared__ LpSums lds[kGroups][kLpTokens];
+  const int tok = threadIdx.x % kLpTokens, grp = threadIdx.x / kLpTokens;
+  const int64_t row = (int64_t)blockIdx.x * kLpTokens + tok;
+  lds[grp][tok] = row < a.M ? lp_column(a, row, grp, kGroups) : lp_none();
+#pragma unroll
+  for (int half = kGroups / 2; half >= 1; half /= 2) {
+    __syncthreads();
+    if (grp < half) lds[grp][tok] = lp_joined(lds[grp][tok], lds[grp + half][tok]);
+  }
+  __syncthreads();
+  if (row < a.M) lp_results(a, row, lds[0][tok], grp, kGroups);
+}
+
+// Few tokens: a workgroup a token, whose first wave finds the alternatives of the last
+// piece while the others join the sums.
+__global__ void __launch_bounds__(256) lp_finish_kernel(const LpSelect c, const LpJoin a) {
+  extern __shared__ __attribute__((aligned(16))) char lp_lds[];
+  __shared__ LpSums lds[3];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int64_t row = blockIdx.x;
+  if (wave == 0) {
+    if (a.k > 0) lp_select(c, row, lane, *reinterpret_cast<LpWave *>(lp_lds));
+  } else {
+    LpSums s = lp_column(a, row, threadIdx.x - 64, 192);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1)
+      s = lp_joined(s, LpSums{__shfl_xor(s.top, off, 64), __shfl_xor(s.sum, off, 64),
+                              __shfl_xor(s.ent, off, 64)});
+    if (lane == 0) lds[wave - 1] = s;
+  }
+  __syncthreads();
+  if (wave == 0) lp_results(a, row, lp_joined(lp_joined(lds[0], lds[1]), lds[2]), lane, 64);
 }
 
 // C = max |dlogp| over the tokens that have one, or max |dentropy|, or 1.
@@ -787,13 +816,15 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
     a.ent = reinterpret_cast<float *>(base + l.ent);
     a.zt = reinterpret_cast<float *>(base + l.zt);
     a.z = top_k > 0 ? reinterpret_cast<float *>(base + l.z) : nullptr;
+    const bool few = a.M < 512;
+    LpSelect sel{};
+    int64_t lds = 0;
     for (int64_t v0 = 0; v0 < v; v0 += l.piece) {
       a.w = w + v0 * d;
       a.v0 = v0;
       a.vn = (int32_t)(v - v0 < l.piece ? v - v0 : l.piece);
       a.best = v0 > 0 && top_k > 0 ? best : nullptr;
       int64_t slices = 0;
-      LpSelect sel{};
       rc = lp_logits<false>(a, &slices, sel.seg, s);
       if (rc != NF4S_OK) return rc;
       if (top_k > 0) {
@@ -802,12 +833,14 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
         sel.slices = (int32_t)slices;
         sel.first = v0 == 0;
         sel.best = best;
-        const int64_t lds = (int64_t)sizeof(LpWave) + (slices + 63) / 64 * 256;
-        const int64_t fit = kLpSelectLds / lds, waves = fit < 4 ? (fit < 1 ? 1 : fit) : 4;
-        hipLaunchKernelGGL(lp_select_kernel, dim3((uint32_t)ceil_to(a.M, waves)),
-                           dim3((uint32_t)(64 * waves)), (uint32_t)(waves * lds), s, sel);
-        rc = check_launch("lp_select_kernel");
-        if (rc != NF4S_OK) return rc;
+        lds = (int64_t)sizeof(LpWave) + (slices + 63) / 64 * 256;
+        if (!few || v0 + l.piece < v) {
+          const int64_t fit = kLpSelectLds / lds, waves = fit < 4 ? fit : 4;
+          hipLaunchKernelGGL(lp_select_kernel, dim3((uint32_t)ceil_to(a.M, waves)),
+                             dim3((uint32_t)(64 * waves)), (uint32_t)(waves * lds), s, sel);
+          rc = check_launch("lp_select_kernel");
+          if (rc != NF4S_OK) return rc;
+        }
       }
       a.part += slices * a.M;
       a.ent += slices * a.M;
@@ -828,9 +861,12 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
     j.entropy = entropy + m0;
     j.top_logp = top_k > 0 ? top_logp + m0 * top_k : nullptr;
     j.top_ids = top_k > 0 ? top_ids + m0 * top_k : nullptr;
-    const bool few = a.M < 512;
-    hipLaunchKernelGGL(few ? lp_join_kernel<1> : lp_join_kernel<8>,
-                       dim3((uint32_t)(few ? a.M : (a.M + 7) / 8)), dim3(256), 0, s, j);
+    if (few)
+      hipLaunchKernelGGL(lp_finish_kernel, dim3((uint32_t)a.M), dim3(256), (uint32_t)lds, s, sel,
+                         j);
+    else
+      hipLaunchKernelGGL(lp_join_kernel, dim3((uint32_t)ceil_to(a.M, kLpTokens)), dim3(256), 0, s,
+                         j);
     rc = check_launch("lp_join_kernel");
     if (rc != NF4S_OK) return rc;
   }
