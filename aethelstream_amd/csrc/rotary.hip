@@ -91,8 +91,8 @@ __device__ __forceinline__ void rotary_put(uint16_t *p, float v) {
 __device__ __forceinline__ void rotary_put(float *p, float v) { *p = v; }
 
 // Places of a lane's pairs in a row and the moves between memory and registers.
-// kVec: pairs kNP l to kNP l + kNP - 1 of lane l, by vector loads; all of them are
-// turned, or none.  Otherwise pairs l + 64 j, element by element.
+// kVec: pairs kNP l to kNP l + kNP - 1 of lane l, by vector loads; of pairs that are
+// not adjacent all are turned, or none.  Otherwise pairs l + 64 j, element by element.
 template <typename T, int kNP, bool kVec, bool kAdj>
 struct RotaryLane {
   static constexpr int kWords = kVec ? 2 * kNP * (int)sizeof(T) / 4 : 2 * kNP;
@@ -104,7 +104,10 @@ struct RotaryLane {
 
   __device__ __forceinline__ int pair(int j) const { return kVec ? first + j : first + 64 * j; }
   __device__ __forceinline__ bool has(int j) const { return pair(kVec ? 0 : j) < pairs; }
-  __device__ __forceinline__ bool turns(int j) const { return pair(kVec ? 0 : j) < half; }
+  // (Of adjacent pairs a lane may have some that turn.)
+  __device__ __forceinline__ bool turns(int j) const {
+    return pair(kVec && !kAdj ? 0 : j) < half;
+  }
   // Element of pair j's first value, and the distance of its second one.
   __device__ __forceinline__ int place(int j) const {
     const int p = pair(j);
@@ -130,8 +133,11 @@ struct RotaryLane {
             *reinterpret_cast<u32x4 *>(r.v + kHalf + i) =
                 __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(b + i));
           }
+        } else if constexpr (kHalf == 1) {
+          r.v[0] = __builtin_nontemporal_load(a);
+          r.v[1] = __builtin_nontemporal_load(b);
         } else {
-          static_assert(kHalf == 2, "four bf16 values");
+          static_assert(kHalf == 2, "two fp32 or four bf16 values");
           *reinterpret_cast<u32x2 *>(r.v) =
               __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(a));
           *reinterpret_cast<u32x2 *>(r.v + 2) =
@@ -204,6 +210,9 @@ struct RotaryLane {
           __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(r.v + kHalf + i),
                                       reinterpret_cast<u32x4 *>(q + i));
         }
+      } else if constexpr (kHalf == 1) {
+        __builtin_nontemporal_store(r.v[0], p);
+        __builtin_nontemporal_store(r.v[1], q);
       } else {
         __builtin_nontemporal_store(*reinterpret_cast<const u32x2 *>(r.v),
                                     reinterpret_cast<u32x2 *>(p));
@@ -460,14 +469,15 @@ static int64_t rotary_most(bool sums) {
 }
 
 static RotaryPlan rotary_plan(int64_t m, int64_t d, int64_t rot, const int64_t (&heads)[2],
-                              int aligned_pairs, bool sums) {
+                              int aligned_pairs, bool adjacent, bool sums) {
   RotaryPlan p{};
   const int64_t pairs = d / 2;
-  // Vector loads of 8 or 4 pairs where rows, halves and what is not turned are
-  // whole ones.
+  // Vector accesses of 8, 4 or 2 pairs where rows are whole ones, and of pairs that are
+  // not adjacent the halves and what is not turned too.
   int np = sums && aligned_pairs > 4 && pairs <= 256 ? 4 : aligned_pairs;
-  while (np > 1 && (rot % (2 * np) != 0 || d % (2 * np) != 0 || pairs / np > 64)) np /= 2;
-  p.vec = np >= 4;
+  while (np > 1 && (d % (2 * np) != 0 || (!adjacent && rot % (2 * np) != 0) || pairs / np > 64))
+    np /= 2;
+  p.vec = np >= 2;
   int64_t lanes;
   if (p.vec) {
     p.np = np;
@@ -506,7 +516,8 @@ static void rotary_launch(const RotaryPlan &p, const RotaryArgs &a, hipStream_t 
   auto *kernel = !p.vec ? (p.np == 2 ? rotary_kernel<T, 2, false, kAdj, kMode>
                                      : rotary_kernel<T, 8, false, kAdj, kMode>)
                  : p.np == 8 ? rotary_kernel<T, 8, true, kAdj, kMode>
-                             : rotary_kernel<T, 4, true, kAdj, kMode>;
+                 : p.np == 4 ? rotary_kernel<T, 4, true, kAdj, kMode>
+                             : rotary_kernel<T, 2, true, kAdj, kMode>;
   hipLaunchKernelGGL(kernel, dim3((uint32_t)(p.wgs[0] + p.wgs[1])), dim3(kRotaryThreads),
                      (uint32_t)p.lds, s, a);
 }
@@ -540,14 +551,13 @@ static int32_t rotary_shape(int64_t m, int64_t hq, int64_t hk, int64_t d, int64_
   return NF4S_OK;
 }
 
-// Pairs that vector accesses may take at once: 8, 4, or 1 where a pointer or a
-// stride is not a multiple of 16 (8) bytes.
+// Pairs that vector accesses may take at once, by the alignment of a pointer and its
+// strides: 8 of them in accesses of 16 bytes, 4 of 16 or 8, 2 of 8 or 4; else 1.
 static int aligned_pairs(const void *p, int64_t token, int64_t head, int size, int most) {
-  while (most > 1) {
-    const int64_t bytes = size == 2 && most == 4 ? 8 : 16;
+  for (; most > 1; most /= 2) {
+    const int64_t bytes = most * size < 16 ? most * size : 16;
     if (aligned(p, (uintptr_t)bytes) && token * size % bytes == 0 && head * size % bytes == 0)
       break;
-    most = most == 8 ? 4 : 1;
   }
   return most;
 }
@@ -608,7 +618,7 @@ int32_t nf4s_rotary_fwd(const void *q, const void *k, int32_t is_bf16, int64_t m
     np = aligned_pairs(k_out, strides[6], strides[7], size, np);
   }
   const int64_t heads[2] = {hq, hk};
-  const RotaryPlan p = rotary_plan(m, d, rot, heads, np, false);
+  const RotaryPlan p = rotary_plan(m, d, rot, heads, np, interleaved != 0, false);
   const void *in[2] = {q, k};
   void *out[2] = {q_out, k_out};
   const float *w[2] = {w_q, w_k};
@@ -674,7 +684,7 @@ int32_t nf4s_rotary_bwd(const void *dq, const void *dk, const void *q, const voi
       if (ptrs[i] != nullptr && (hk > 0 || i % 2 == 0))
         np = aligned_pairs(ptrs[i], strides[2 * i], strides[2 * i + 1], size, np);
     const int64_t heads[2] = {hq, hk};
-    p = rotary_plan(m, d, rot, heads, np, norm);
+    p = rotary_plan(m, d, rot, heads, np, interleaved != 0, norm);
     const int64_t need = norm ? (int64_t)(p.wgs[0] + p.wgs[1]) * d * 4 : 0;
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
       return fail(NF4S_ERR_INVALID_ARGUMENT, "rotary backward needs %lld workspace bytes",

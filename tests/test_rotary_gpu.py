@@ -113,7 +113,9 @@ SHAPES = [(1, 1, 1, 128, 128), (1, 32, 8, 128, 128), (37, 6, 2, 64, 64), (5, 3, 
           (130, 5, 1, 96, 96), (9, 4, 2, 256, 64), (3, 2, 1, 1024, 1024), (7, 3, 2, 512, 256),
           (11, 2, 2, 192, 128), (64, 1, 1, 16, 16), (21, 7, 3, 34, 18), (13, 2, 1, 30, 30),
           (6, 2, 2, 2, 2), (5, 2, 1, 258, 6), (4, 1, 1, 1022, 1020), (300, 9, 4, 128, 32),
-          (17, 65, 33, 64, 32), (2, 4096, 1, 8, 8), (700, 1, 1, 32, 16), (50, 2, 2, 112, 56)]
+          (17, 65, 33, 64, 32), (2, 4096, 1, 8, 8), (700, 1, 1, 32, 16), (50, 2, 2, 112, 56),
+          (9, 5, 2, 128, 84), (8, 3, 1, 256, 68), (7, 2, 2, 36, 12), (2, 2, 1, 1000, 500),
+          (40, 3, 1, 256, 60), (6, 2, 1, 768, 768)]
 
 
 @pytest.mark.parametrize("m,hq,hk,d,rot", SHAPES)
