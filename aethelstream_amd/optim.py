@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import operator
+from array import array
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
@@ -155,7 +156,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
     # Whole lists at a time: of 241 tensors 0.1 ms, of which each is looked at alone
     # (0.16) only to say what is wrong.
     kinds = [list(map(_dtype, params)), list(map(_dtype, grads))]
-    found = [_TYPES.get(t) for t in kinds[0]], [_TYPES.get(t) for t in kinds[1]]
+    found = [list(map(_TYPES.get, k)) for k in kinds]
     if None in found[0] or None in found[1] or list(map(_numel, params)) != state.sizes \
             or not all(map(_same_size, params, grads)) \
             or set(map(_device, params)) | set(map(_device, grads)) != {index} \
@@ -177,13 +178,14 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
     host = None
     if hyper is None:
         host = (ctypes.c_float * 8)(*coefficients(step, lr, betas, eps, weight_decay))
-    pointers = ctypes.c_void_p * count
-    copied = None if copies is None else pointers(*[_ptr(c) for c in copies])
+    lists = [array("Q", map(_data_ptr, params)), array("Q", map(_data_ptr, grads)),
+             None if copies is None else array("Q", [0 if c is None else c.data_ptr()
+                                                     for c in copies]),
+             array("q", state.sizes), array("i", types)]
+    at = [None if a is None else a.buffer_info()[0] for a in lists]
     _lib.check(_lib.load().nf4s_adamw_step(
-        pointers(*map(_data_ptr, params)), pointers(*map(_data_ptr, grads)),
-        copied, (ctypes.c_int64 * count)(*state.sizes), (ctypes.c_int32 * count)(*types), count,
-        state.m.data_ptr(), state.v.data_ptr(), _ptr(state.m_scale), _ptr(state.v_scale), host,
-        _ptr(hyper), _ptr(grad_scale), _stream_ptr(state.m)))
+        *at, count, state.m.data_ptr(), state.v.data_ptr(), _ptr(state.m_scale),
+        _ptr(state.v_scale), host, _ptr(hyper), _ptr(grad_scale), _stream_ptr(state.m)))
 
 
 def moments(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:
