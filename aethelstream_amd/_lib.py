@@ -146,9 +146,10 @@ SIGNATURES = {
                                   _P, _I64, _P]),
     "nf4s_linear_ce_workspace_size": (_I32, [_I64, _I64, _I64, _I32, ctypes.POINTER(_I64)]),
     "nf4s_linear_logprob_fwd": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P,
-                                       _P, _P, _I64, _P]),
-    "nf4s_linear_logprob_bwd": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P,
-                                       _I32, _I32, _P, _I64, _P]),
+                                       _P, _P, _P, _I64, _P]),
+    "nf4s_linear_logprob_bwd": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P,
+                                       _P, _I32, _I32, _P, _I64, _P]),
+    "nf4s_linear_logprob_logits_size": (_I32, [_I64, _I64, _I64, ctypes.POINTER(_I64)]),
     "nf4s_linear_logprob_workspace_size": (_I32, [_I64, _I64, _I64, _I64, _I32,
                                                   ctypes.POINTER(_I64)]),
     "nf4s_host_alloc": (_I32, [_I64, ctypes.POINTER(_P)]),

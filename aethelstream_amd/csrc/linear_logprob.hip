@@ -72,6 +72,29 @@ __device__ __forceinline__ uint64_t lp_key(uint32_t order, uint32_t column) {
 // At least -1e4, where exp2 is 0; NaN stays.
 __device__ __forceinline__ float lp_floor(float y) { return y < -1e4f ? -1e4f : y; }
 
+// What a token's gradients of the logits need, divided by C.
+struct LpToken {
+  float lse, da, dh, base;  // base: dlogp + dentropy * entropy
+  bool none;                // both gradients are zero
+};
+__device__ __forceinline__ LpToken lp_token(const LpLogits &a, int64_t row, bool here, int64_t t) {
+  LpToken k;
+  k.lse = here ? a.lse[row] : 0.0f;
+  const bool given = t != a.ignore;
+  k.da = here && given ? a.dlogp[row] / *a.common : 0.0f;
+  k.dh = here && a.dentropy != nullptr ? a.dentropy[row] / *a.common : 0.0f;
+  k.none = k.da == 0.0f && k.dh == 0.0f;
+  if (given && (t < 0 || t >= a.V)) k.da = __builtin_nanf("");
+  k.base = k.dh == 0.0f ? k.da : k.da + k.dh * a.entropy[row];
+  return k;
+}
+// G of a logit that is not the given token's.
+__device__ __forceinline__ float lp_grad(const LpToken &k, float z) {
+  // Past -1e4 the exponential is zero whatever is behind it.
+  const float l = lp_floor(z - k.lse);
+  return -exp_of(l) * (k.base + k.dh * l);
+}
+
 template <int kMT, int kNT, bool kGrad>
 __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) lp_logits_kernel(const LpLogits a) {
   using Core = GcCore<kMT, kNT, false, false>;
@@ -160,32 +183,22 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) lp_logits_kernel
         a.ent[slice] = ent;
       }
     } else {
-      const float lse = here ? a.lse[row] : 0.0f;
-      const bool given = t != a.ignore;
-      float da = here && given ? a.dlogp[row] / *a.common : 0.0f;
-      const float dh = here && a.dentropy != nullptr ? a.dentropy[row] / *a.common : 0.0f;
-      const bool none = da == 0.0f && dh == 0.0f;
-      if (given && (t < 0 || t >= a.V)) da = __builtin_nanf("");
-      const float base = dh == 0.0f ? da : da + dh * a.entropy[row];
+      const LpToken k = lp_token(a, row, here, t);
 #pragma unroll
       for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // Past -1e4 the exponential is zero whatever is behind it.
-          const float l = lp_floor(z[nt][i] - lse);
-          z[nt][i] = -exp_of(l) * (base + dh * l);
-        }
+        for (int i = 0; i < 4; ++i) z[nt][i] = lp_grad(k, z[nt][i]);
       if (__ballot(mine) != 0) {
 #pragma unroll
         for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) z[nt][i] += at == 4 * nt + i ? da : 0.0f;
+          for (int i = 0; i < 4; ++i) z[nt][i] += at == 4 * nt + i ? k.da : 0.0f;
       }
       // A token without a gradient has none, whatever its logits are.
 #pragma unroll
       for (int nt = 0; nt < 2 * kNT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z[nt][i] = none ? 0.0f : fp32_rounded(z[nt][i]);
+        for (int i = 0; i < 4; ++i) z[nt][i] = k.none ? 0.0f : fp32_rounded(z[nt][i]);
       // Columns of the piece's last, partial 64 hold zeros: G is read in steps of 64.
       if (mt % 2 == 1) {
         const int64_t first = row0 + 16 * (mt - 1);
@@ -195,6 +208,57 @@ __global__ void __launch_bounds__(kGcThreads, kMT == 1 ? 2 : 1) lp_logits_kernel
             a.gcols - (r0 + c0), lane);
       }
     }
+  }
+}
+
+// Half tiles of one launch: their logits as they are stored.
+struct LpSegment {
+  int32_t slices, width;
+  uint32_t column;   // the first one
+  int32_t columns;   // how many there are
+  const floatx2 *part;      // [slices][M]
+  const float *z;           // [slices][M][width]
+};
+
+// G of a piece from kept logits, for half tiles s0 .. of one segment: eight columns a
+// lane, kLpKept rows one after the other.  Bound by memory: 6 bytes a logit.
+constexpr int kLpKept = 4;
+__global__ void __launch_bounds__(256) lp_kept_kernel(const LpLogits a, const LpSegment g,
+                                                      int32_t s0, int32_t row_blocks) {
+  const int s = s0 + (int)(blockIdx.x / (uint32_t)row_blocks);
+  const int eights = g.width / 8, rows = 256 / eights;
+  const int o = (int)threadIdx.x % eights;
+  const int64_t row0 = (int64_t)(blockIdx.x % (uint32_t)row_blocks) * (rows * kLpKept) +
+                       (int)threadIdx.x / eights;
+  const int64_t column = (int64_t)g.column + (int64_t)s * g.width + 8 * o;
+  if (column - a.v0 >= a.gcols) return;  // G's rows are whole 64s
+  floatx4 v[kLpKept][2];
+#pragma unroll
+  for (int i = 0; i < kLpKept; ++i) {
+    const int64_t row = row0 + i * rows;
+    if (row >= a.M) break;
+    const floatx4 *z =
+        reinterpret_cast<const floatx4 *>(g.z + ((int64_t)s * a.M + row) * g.width + 8 * o);
+    v[i][0] = __builtin_nontemporal_load(z);
+    v[i][1] = __builtin_nontemporal_load(z + 1);
+  }
+#pragma unroll
+  for (int i = 0; i < kLpKept; ++i) {
+    const int64_t row = row0 + i * rows;
+    if (row >= a.M) break;
+    const int64_t t = a.targets[row];
+    const LpToken k = lp_token(a, row, true, t);
+    const int64_t rel = t - column;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = lp_grad(k, v[i][j / 4][j % 4]);
+      if (t != a.ignore && rel == j && t < a.V) x[j] += k.da;
+      x[j] = k.none ? 0.0f : fp32_rounded(x[j]);
+    }
+    *reinterpret_cast<u32x4 *>(a.g + row * a.ldg + (column - a.v0)) =
+        (u32x4){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                pack_bf16x2(x[6], x[7])};
   }
 }
 
@@ -225,15 +289,6 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
   b = (uint64_t)h32[1] << 32 | l32[1];
   return a > b ? a : b;
 }
-
-// Half tiles of one launch of a piece.
-struct LpSegment {
-  int32_t slices, width;
-  uint32_t column;   // the first one
-  int32_t columns;   // how many there are
-  const floatx2 *part;      // [slices][M]
-  const float *z;           // [slices][M][width]
-};
 
 struct LpSelect {
   LpSegment seg[2];
@@ -752,15 +807,53 @@ static int32_t lp_logits(LpLogits a, int64_t *slices, LpSegment *seg, hipStream_
   return NF4S_OK;
 }
 
+// Where kept logits lie: the half tiles of the launches over all columns.
+static int64_t lp_kept(int64_t m, int64_t v, int64_t d, const float *z, LpSegment (&seg)[2]) {
+  CeLaunch l[2];
+  const int n = ce_tiles(m, v, d, l);
+  int64_t at = 0, column = 0;
+  seg[1] = LpSegment{};
+  for (int i = 0; i < n; ++i) {
+    const int64_t slices = 2 * ceil_to(l[i].cols, 64 * l[i].nt), width = 32 * l[i].nt;
+    seg[i] = LpSegment{(int32_t)slices, (int32_t)width, (uint32_t)column, (int32_t)l[i].cols,
+                       nullptr, z != nullptr ? z + at * m : nullptr};
+    at += slices * width;
+    column += l[i].cols;
+  }
+  return at * m * 4;
+}
+
+struct LpGrad {
+  LpLogits a;
+  bool kept;
+  LpSegment seg[2];
+};
+
 static int32_t lp_grad_logits(const void *ctx, const HeadPiece &p) {
-  LpLogits a = *static_cast<const LpLogits *>(ctx);
+  const LpGrad &c = *static_cast<const LpGrad *>(ctx);
+  LpLogits a = c.a;
   a.w += p.v0 * a.d;
   a.v0 = p.v0;
   a.vn = (int32_t)p.vn;
   a.common = p.common;
   a.g = p.g;
   a.ldg = a.gcols = p.ldg;
-  return lp_logits<true>(a, nullptr, nullptr, p.stream);
+  if (!c.kept) return lp_logits<true>(a, nullptr, nullptr, p.stream);
+  // Pieces begin at multiples of 256 columns and launches too, so at half tiles.
+  for (int i = 0; i < 2; ++i) {
+    const LpSegment &g = c.seg[i];
+    const int64_t end = (int64_t)g.column + g.columns;
+    const int64_t from = p.v0 > g.column ? p.v0 : g.column;
+    const int64_t to = p.v0 + p.vn < end ? p.v0 + p.vn : end;
+    if (g.slices == 0 || from >= to) continue;
+    const int64_t s0 = (from - g.column) / g.width, s1 = ceil_to(to - g.column, g.width);
+    const int64_t blocks = ceil_to(a.M, 256 / (g.width / 8) * kLpKept);
+    hipLaunchKernelGGL(lp_kept_kernel, dim3((uint32_t)((s1 - s0) * blocks)), dim3(256), 0,
+                       p.stream, a, g, (int32_t)s0, (int32_t)blocks);
+    const int32_t rc = check_launch("lp_kept_kernel");
+    if (rc != NF4S_OK) return rc;
+  }
+  return NF4S_OK;
 }
 
 }  // namespace nf4s
@@ -781,10 +874,21 @@ int32_t nf4s_linear_logprob_workspace_size(int64_t m, int64_t v, int64_t d, int6
   return rc;
 }
 
+int32_t nf4s_linear_logprob_logits_size(int64_t m, int64_t v, int64_t d, int64_t *bytes) {
+  clear_error();
+  if (bytes == nullptr) return fail(NF4S_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  *bytes = 0;
+  CePlan p;
+  const int32_t rc = lp_plan(m, v, d, 0, p);
+  LpSegment seg[2];
+  if (rc == NF4S_OK && m > 0 && m == p.tokens) *bytes = lp_kept(m, v, d, nullptr, seg);
+  return rc;
+}
+
 int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
                                 int64_t m, int64_t v, int64_t d, int64_t top_k,
                                 int64_t ignore_index, float *logp, float *lse, float *entropy,
-                                float *top_logp, int64_t *top_ids, void *workspace,
+                                float *top_logp, int64_t *top_ids, float *logits, void *workspace,
                                 int64_t workspace_bytes, void *stream) {
   clear_error();
   CePlan p;
@@ -797,8 +901,13 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
       (top_k > 0 && (top_logp == nullptr || top_ids == nullptr)))
     return fail(NF4S_ERR_INVALID_ARGUMENT, "an output is NULL");
   if (!aligned(logp, 4) || !aligned(lse, 4) || !aligned(entropy, 4) || !aligned(top_logp, 4) ||
-      !aligned(top_ids, 8))
-    return fail(NF4S_ERR_MISALIGNED, "outputs must be aligned to their elements");
+      !aligned(top_ids, 8) || !aligned(logits, 16))
+    return fail(NF4S_ERR_MISALIGNED,
+                "outputs must be aligned to their elements, logits 16-byte");
+  if (logits != nullptr && (top_k > 0 || m != p.tokens))
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE,
+                "logits are kept of up to %lld tokens, without alternatives",
+                (long long)kCeTokens);
   const hipStream_t s = as_stream(stream);
   char *base = static_cast<char *>(workspace);
   for (int64_t m0 = 0; m0 < m; m0 += p.tokens) {
@@ -815,7 +924,7 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
     a.part = reinterpret_cast<floatx2 *>(base);
     a.ent = reinterpret_cast<float *>(base + l.ent);
     a.zt = reinterpret_cast<float *>(base + l.zt);
-    a.z = top_k > 0 ? reinterpret_cast<float *>(base + l.z) : nullptr;
+    a.z = top_k > 0 ? reinterpret_cast<float *>(base + l.z) : logits;
     const bool few = a.M < 512;
     LpSelect sel{};
     int64_t lds = 0;
@@ -874,11 +983,11 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
 }
 
 int32_t nf4s_linear_logprob_bwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
-                                const float *lse, const float *entropy, const float *dlogp,
-                                const float *dentropy, int64_t m, int64_t v, int64_t d,
-                                int64_t ignore_index, uint16_t *dx, void *dw, int32_t dw_is_f32,
-                                int32_t accumulate, void *workspace, int64_t workspace_bytes,
-                                void *stream) {
+                                const float *lse, const float *entropy, const float *logits,
+                                const float *dlogp, const float *dentropy, int64_t m, int64_t v,
+                                int64_t d, int64_t ignore_index, uint16_t *dx, void *dw,
+                                int32_t dw_is_f32, int32_t accumulate, void *workspace,
+                                int64_t workspace_bytes, void *stream) {
   clear_error();
   CePlan p;
   int32_t rc = lp_plan(m, v, d, 0, p);
@@ -891,10 +1000,14 @@ int32_t nf4s_linear_logprob_bwd(const uint16_t *x, const uint16_t *w, const int6
     return fail(NF4S_ERR_INVALID_ARGUMENT, "lse, dlogp, dx or dw is NULL");
   if (m > 0 && dentropy != nullptr && entropy == nullptr)
     return fail(NF4S_ERR_INVALID_ARGUMENT, "dentropy needs entropy");
+  if (logits != nullptr && m > 0 && m != p.tokens)
+    return fail(NF4S_ERR_UNSUPPORTED_SHAPE, "logits are kept of up to %lld tokens",
+                (long long)kCeTokens);
   if (!aligned(dw, 16) || (m > 0 && (!aligned(dx, 16) || !aligned(lse, 4) || !aligned(dlogp, 4) ||
-                                     !aligned(entropy, 4) || !aligned(dentropy, 4))))
+                                     !aligned(entropy, 4) || !aligned(dentropy, 4) ||
+                                     !aligned(logits, 16))))
     return fail(NF4S_ERR_MISALIGNED,
-                "dx and dw must be 16-byte aligned, the tokens' values 4-byte");
+                "dx, dw and logits must be 16-byte aligned, the tokens' values 4-byte");
   const hipStream_t s = as_stream(stream);
   if (m == 0) return accumulate ? NF4S_OK : head_zero_dw(dw, dw_is_f32 != 0, v * d, s);
   const HeadGrad h{x, w, m, v, d, dx, dw, dw_is_f32 != 0, accumulate != 0, workspace};
@@ -902,7 +1015,8 @@ int32_t nf4s_linear_logprob_bwd(const uint16_t *x, const uint16_t *w, const int6
                      ignore_index, m, head_common(h, p));
   rc = check_launch("lp_common_kernel");
   if (rc != NF4S_OK) return rc;
-  LpLogits a{};
+  LpGrad c{};
+  LpLogits &a = c.a;
   a.x = x;
   a.w = w;
   a.targets = targets;
@@ -914,7 +1028,9 @@ int32_t nf4s_linear_logprob_bwd(const uint16_t *x, const uint16_t *w, const int6
   a.entropy = entropy;
   a.dlogp = dlogp;
   a.dentropy = dentropy;
-  return head_gradients(h, p, lp_grad_logits, &a, s);
+  c.kept = logits != nullptr;
+  if (c.kept) lp_kept(m, v, d, logits, c.seg);
+  return head_gradients(h, p, lp_grad_logits, &c, s);
 }
 
 }  // extern "C"

@@ -135,6 +135,7 @@ class LogProbs:
     lse: torch.Tensor                 # float32 [M]
     top_logp: Optional[torch.Tensor]  # float32 [M, top_k], with top_k > 0
     top_ids: Optional[torch.Tensor]   # int64 [M, top_k]
+    logits: Optional[torch.Tensor] = None  # float32, in the kernels' order, if kept
 
 
 def log_probs_workspace_bytes(m: int, v: int, d: int, top_k: int = 0,
@@ -153,15 +154,29 @@ def _log_probs_workspace_bytes(m: int, v: int, d: int, top_k: int, backward: boo
     return int(out.value)
 
 
+@functools.lru_cache(maxsize=256)
+def _logits_bytes(m: int, v: int, d: int, device: int) -> int:
+    out = ctypes.c_int64(0)
+    _lib.check(_lib.load().nf4s_linear_logprob_logits_size(m, v, d, ctypes.byref(out)))
+    return int(out.value)
+
+
 def linear_log_probs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
                      ignore_index: int = IGNORE_INDEX,
-                     workspace: Optional[torch.Tensor] = None) -> LogProbs:
+                     workspace: Optional[torch.Tensor] = None,
+                     keep_logits: Optional[bool] = None) -> LogProbs:
     """Log probability of ``targets`` under softmax(x . W^T), the entropy and the
     log-sum-exp of every token, and with ``top_k`` (up to 32) the tokens of largest
     logit in order, equal ones by their index, with their log probabilities.  A target
     equal to ``ignore_index`` (no token is given) has logp 0, and the rest as any
     other; a target outside [0, V) has NaN (it is only seen on the device).  A row with
-    a NaN logit, or an infinite largest one, is NaN in everything but ``top_ids``."""
+    a NaN logit, or an infinite largest one, is NaN in everything but ``top_ids``.
+
+    ``keep_logits``: the result holds the logits in fp32, and the gradients need not
+    multiply x . W^T again (a quarter of a training pass' products).  By default
+    (None) where no alternatives are asked for and they take no more memory than W,
+    which is up to d / 2 tokens, 16384 at most; a pass that only scores saves 4 M V
+    bytes and up to a seventh of its time with False."""
     _check_head(x, w, targets)
     m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
     top_k = int(top_k)
@@ -173,13 +188,20 @@ def linear_log_probs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, to
     if top_k > 0:
         top_logp = torch.empty(m, top_k, dtype=torch.float32, device=x.device)
         top_ids = torch.empty(m, top_k, dtype=torch.int64, device=x.device)
+    logits = None
+    if keep_logits or (keep_logits is None and top_k == 0 and 2 * m <= d):
+        need = _logits_bytes(m, v, d, x.get_device())
+        if keep_logits and m > 0 and (top_k > 0 or need == 0):
+            raise ValueError("logits are kept without alternatives, of up to 16384 tokens")
+        if need > 0:
+            logits = torch.empty(need // 4, dtype=torch.float32, device=x.device)
     workspace = _workspace_for(
         _log_probs_workspace_bytes(m, v, d, top_k, False, x.get_device()), workspace, x)
     _lib.check(_lib.load().nf4s_linear_logprob_fwd(
         x.data_ptr(), w.data_ptr(), targets.data_ptr(), m, v, d, top_k, ignore_index,
         logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids),
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_ptr(x)))
-    return LogProbs(logp, entropy, lse, top_logp, top_ids)
+        _ptr(logits), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_ptr(x)))
+    return LogProbs(logp, entropy, lse, top_logp, top_ids, logits)
 
 
 def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, out: LogProbs,
@@ -202,13 +224,20 @@ def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
         if t is not None and (t.dtype != torch.float32 or list(t.shape) != [m]
                               or t.device != x.device):
             raise ValueError(f"{name} must be float32 [{m}] on x's device")
+    logits = out.logits
+    if logits is not None:
+        _require_cuda(logits)
+        if logits.dtype != torch.float32 or logits.device != x.device \
+                or logits.numel() * 4 != _logits_bytes(m, v, d, x.get_device()):
+            raise ValueError("out's logits are of another head, or of other tokens")
     dw = _check_dw(dw, accumulate, w, x)
     dx = torch.empty_like(x)
     workspace = _workspace_for(
         _log_probs_workspace_bytes(m, v, d, 0, True, x.get_device()), workspace, x)
     _lib.check(_lib.load().nf4s_linear_logprob_bwd(
         x.data_ptr(), w.data_ptr(), targets.data_ptr(), out.lse.data_ptr(),
-        out.entropy.data_ptr(), dlogp.data_ptr(), _ptr(dentropy), m, v, d, ignore_index,
-        dx.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32), int(accumulate),
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_ptr(x)))
+        out.entropy.data_ptr(), _ptr(logits), dlogp.data_ptr(), _ptr(dentropy), m, v, d,
+        ignore_index, dx.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32),
+        int(accumulate), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        _stream_ptr(x)))
     return dx, dw

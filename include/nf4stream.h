@@ -514,7 +514,7 @@ int32_t nf4s_linear_ce_workspace_size(int64_t m, int64_t v, int64_t d, int32_t b
                                       int64_t *bytes);
 
 /* ---------------------------------------------------------------------------
- * Log probabilities under a linear head, without keeping the logits z = x . w^T:
+ * Log probabilities under a linear head, of logits z = x . w^T:
  *   lse[i] = log sum_c exp z[i, c],  logp[i] = z[i, targets[i]] - lse[i]
  *   entropy[i] = -sum_c p log p,  p = exp(z[i, c] - lse[i])
  *   top_ids[i, 0 .. top_k - 1]: the columns of the largest logits, equal ones by
@@ -529,11 +529,15 @@ int32_t nf4s_linear_ce_workspace_size(int64_t m, int64_t v, int64_t d, int32_t b
 int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
                                 int64_t m, int64_t v, int64_t d, int64_t top_k,
                                 int64_t ignore_index, float *logp, float *lse, float *entropy,
-                                float *top_logp, int64_t *top_ids, void *workspace,
+                                float *top_logp, int64_t *top_ids, float *logits, void *workspace,
                                 int64_t workspace_bytes, void *stream);
+/* Bytes of the logits that the forward keeps for the gradients where `logits` is not
+ * NULL (fp32, in the order of its tiles; of up to 16384 tokens, without alternatives;
+ * 0: not kept).  The gradients, given them, do not multiply x . w^T again. */
+int32_t nf4s_linear_logprob_logits_size(int64_t m, int64_t v, int64_t d, int64_t *bytes);
 /*
  * Gradients for given dlogp and dentropy (fp32 [m]; dentropy NULL: zero) and the
- * forward's lse and entropy (NULL without dentropy):
+ * forward's lse, entropy (NULL without dentropy) and kept logits (NULL: made again):
  *   G[i, c] = [c = targets[i]] dlogp[i] - p (dlogp[i] + dentropy[i] (log p + entropy[i]))
  *   dx = G . w,  dw = G^T . x
  * with dlogp 0 where the target is ignored; dx, dw, dw_is_f32, accumulate and the
@@ -542,11 +546,11 @@ int32_t nf4s_linear_logprob_fwd(const uint16_t *x, const uint16_t *w, const int6
  * zeros times its row of x, which has to be finite.
  */
 int32_t nf4s_linear_logprob_bwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,
-                                const float *lse, const float *entropy, const float *dlogp,
-                                const float *dentropy, int64_t m, int64_t v, int64_t d,
-                                int64_t ignore_index, uint16_t *dx, void *dw, int32_t dw_is_f32,
-                                int32_t accumulate, void *workspace, int64_t workspace_bytes,
-                                void *stream);
+                                const float *lse, const float *entropy, const float *logits,
+                                const float *dlogp, const float *dentropy, int64_t m, int64_t v,
+                                int64_t d, int64_t ignore_index, uint16_t *dx, void *dw,
+                                int32_t dw_is_f32, int32_t accumulate, void *workspace,
+                                int64_t workspace_bytes, void *stream);
 /* Workspace bytes of the forward (backward = 0) or of the gradients (whatever
  * top_k).  Calls that share a workspace must not overlap. */
 int32_t nf4s_linear_logprob_workspace_size(int64_t m, int64_t v, int64_t d, int64_t top_k,

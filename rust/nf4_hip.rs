@@ -232,15 +232,16 @@ extern "C" {
     pub fn nf4s_linear_logprob_fwd(x: *const u16, w: *const u16, targets: *const i64, m: i64,
                                    v: i64, d: i64, top_k: i64, ignore_index: i64,
                                    logp: *mut f32, lse: *mut f32, entropy: *mut f32,
-                                   top_logp: *mut f32, top_ids: *mut i64,
+                                   top_logp: *mut f32, top_ids: *mut i64, logits: *mut f32,
                                    workspace: *mut c_void, workspace_bytes: i64,
                                    stream: *mut c_void) -> i32;
     pub fn nf4s_linear_logprob_bwd(x: *const u16, w: *const u16, targets: *const i64,
-                                   lse: *const f32, entropy: *const f32, dlogp: *const f32,
-                                   dentropy: *const f32, m: i64, v: i64, d: i64,
+                                   lse: *const f32, entropy: *const f32, logits: *const f32,
+                                   dlogp: *const f32, dentropy: *const f32, m: i64, v: i64, d: i64,
                                    ignore_index: i64, dx: *mut u16, dw: *mut c_void,
                                    dw_is_f32: i32, accumulate: i32, workspace: *mut c_void,
                                    workspace_bytes: i64, stream: *mut c_void) -> i32;
+    pub fn nf4s_linear_logprob_logits_size(m: i64, v: i64, d: i64, bytes: *mut i64) -> i32;
     pub fn nf4s_linear_logprob_workspace_size(m: i64, v: i64, d: i64, top_k: i64, backward: i32,
                                               bytes: *mut i64) -> i32;
 

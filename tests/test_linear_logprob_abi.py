@@ -18,16 +18,16 @@ P = 0x1000
 BIG = 1 << 42
 
 
-def _fwd(x=P, w=P, t=P, m=4, v=32, d=64, k=3, logp=P, lse=P, ent=P, top=P, ids=P, work=P,
-         size=BIG):
-    return _lib.load().nf4s_linear_logprob_fwd(x, w, t, m, v, d, k, -100, logp, lse, ent, top, ids,
-                                               work, size, None)
-
-
-def _bwd(x=P, w=P, t=P, lse=P, ent=P, da=P, dh=P, m=4, v=32, d=64, dx=P, dw=P, f32=0, acc=0,
+def _fwd(x=P, w=P, t=P, m=4, v=32, d=64, k=3, logp=P, lse=P, ent=P, top=P, ids=P, logits=None,
          work=P, size=BIG):
-    return _lib.load().nf4s_linear_logprob_bwd(x, w, t, lse, ent, da, dh, m, v, d, -100, dx, dw,
-                                               f32, acc, work, size, None)
+    return _lib.load().nf4s_linear_logprob_fwd(x, w, t, m, v, d, k, -100, logp, lse, ent, top, ids,
+                                               logits, work, size, None)
+
+
+def _bwd(x=P, w=P, t=P, lse=P, ent=P, logits=None, da=P, dh=P, m=4, v=32, d=64, dx=P, dw=P, f32=0,
+         acc=0, work=P, size=BIG):
+    return _lib.load().nf4s_linear_logprob_bwd(x, w, t, lse, ent, logits, da, dh, m, v, d, -100,
+                                               dx, dw, f32, acc, work, size, None)
 
 
 def test_refusals():
@@ -46,6 +46,10 @@ def test_refusals():
     assert _bwd(dx=None) == INVALID and _bwd(dw=None) == INVALID and _bwd(dw=P + 8) == ALIGN
     assert _bwd(ent=None) == INVALID and _bwd(da=None) == INVALID and _bwd(dh=P + 2) == ALIGN
     assert _bwd(acc=1) == INVALID
+    # Logits are kept of up to 16384 tokens, without alternatives.
+    assert _fwd(logits=P) == SHAPE and _fwd(k=0, logits=P, m=16385) == SHAPE
+    assert _fwd(k=0, logits=P + 8) == ALIGN
+    assert _bwd(logits=P, m=16385) == SHAPE and _bwd(logits=P + 4) == ALIGN
     assert _fwd(m=0, x=None, t=None, logp=None, lse=None, ent=None, top=None, ids=None,
                 work=None, size=0) == 0
 
@@ -63,6 +67,13 @@ def test_workspace():
         # Alternatives: a piece of the logits and the best ones so far.
         assert q(m, v, d, 8, 0, ctypes.byref(out)) == 0
         assert without < out.value < without + (270 << 20) + 100 * m
+    f = lib.nf4s_linear_logprob_logits_size
+    assert f(4, 32, 64, None) == INVALID and f(4, 32, 60, ctypes.byref(out)) == SHAPE
+    for m, v, d in ((1, 40, 64), (77, 32000, 4096), (4096, 128000, 8192)):
+        assert f(m, v, d, ctypes.byref(out)) == 0
+        assert 4 * m * v <= out.value <= 4 * m * (v + 256)
+    assert f(0, 32, 64, ctypes.byref(out)) == 0 and out.value == 0
+    assert f(16385, 32, 64, ctypes.byref(out)) == 0 and out.value == 0
     assert q(4096, 128000, 8192, 0, 1, ctypes.byref(out)) == 0
     same = ctypes.c_int64(-1)
     lib.nf4s_linear_ce_workspace_size(4096, 128000, 8192, 1, ctypes.byref(same))
@@ -84,5 +95,5 @@ def test_listing(tmp_path):
         n, found = k.faults()
         tied += n > 0
         assert not found, (name, found[:5])
-    assert tied == 4 and len(kernels) == 10, sorted(kernels)
+    assert tied == 4 and len(kernels) == 11, sorted(kernels)
     assert text.count(".amdhsa_private_segment_fixed_size 0\n") == len(kernels)

@@ -246,6 +246,30 @@ def test_backward(m, v, d, entropy):
         assert torch.equal(other, dx)
 
 
+@pytest.mark.parametrize("m,v,d", [s[:3] for s in SHAPES] + [(3000, 20000, 64), (700, 40007, 256),
+                                                             (16384, 3000, 16)])
+def test_kept_logits(m, v, d):
+    """The gradients from kept logits are those from logits made again, bit for bit, in
+    one piece of the vocabulary and in several, and the forward's results the same."""
+    print(m, v, d, flush=True)
+    x, w, t, da = ce._inputs(m, v, d, seed=m + v)
+    dh = ce._randn((m,), 9, 0.5, torch.float32)
+    dh[: m // 3] = 0
+    da[: m // 4] = 0
+    r = loss.linear_log_probs(x, w, t, keep_logits=True)
+    s = loss.linear_log_probs(x, w, t, keep_logits=False)
+    assert r.logits is not None and s.logits is None
+    for name in ("logp", "entropy", "lse"):
+        assert torch.equal(getattr(r, name), getattr(s, name))
+    kept = loss.linear_log_probs(x, w, t).logits
+    assert (kept is not None) == (2 * m <= d)
+    assert loss.linear_log_probs(x, w, t, top_k=1).logits is None
+    for b in (dh, None):
+        got = loss.linear_log_probs_bwd(x, w, t, r, da, b)
+        want = loss.linear_log_probs_bwd(x, w, t, s, da, b)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_entropy_alone_and_tokens_without_gradients():
     m, v, d = 70, 900, 136
     x, w, t, _ = ce._inputs(m, v, d, seed=21)
@@ -390,6 +414,10 @@ def test_refusals():
         a.update(kw)
         with pytest.raises(ValueError):
             loss.linear_log_probs(a.pop("x"), a.pop("w"), a.pop("t"), **a)
+    big = ce._randn((16385, 64), 1)
+    for kw in (dict(top_k=1), dict(x=big, t=torch.zeros(16385, dtype=torch.int64, device="cuda"))):
+        with pytest.raises(ValueError):
+            loss.linear_log_probs(kw.pop("x", x), w, kw.pop("t", t), keep_logits=True, **kw)
     with pytest.raises(RuntimeError):  # d no multiple of 8
         loss.linear_log_probs(x[:, :60].contiguous(), w[:, :60].contiguous(), t)
     r = loss.linear_log_probs(x, w, t)
@@ -397,7 +425,9 @@ def test_refusals():
                dict(dentropy=da.cpu()), dict(accumulate=True), dict(dw=w.half()),
                dict(dw=torch.empty(4, 64, device="cuda")), dict(dw=w.clone(), accumulate=True),
                dict(out=loss.LogProbs(r.logp, r.entropy, r.lse[:5], None, None)),
-               dict(out=loss.LogProbs(r.logp, r.entropy[:5], r.lse, None, None))):
+               dict(out=loss.LogProbs(r.logp, r.entropy[:5], r.lse, None, None)),
+               dict(out=loss.LogProbs(r.logp, r.entropy, r.lse, None, None, r.logits[:-4])),
+               dict(out=loss.LogProbs(r.logp, r.entropy, r.lse, None, None, r.logits.double()))):
         a = dict(out=r, dlogp=da)
         a.update(kw)
         with pytest.raises(ValueError):
