@@ -450,11 +450,22 @@ static int32_t adam_blocks(const int64_t *sizes, int32_t count, int64_t &blocks)
   return NF4S_OK;
 }
 
-// Every tensor's buffers are there and aligned, and no two of what is written
-// overlap: each element is updated by one lane, once.
-static int32_t adam_buffers(const AdamList &l) {
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
-  written.reserve(2 * (size_t)l.count);
+// Every tensor's buffers are there and aligned, no two of what is written overlap, as
+// each element is updated by one lane, once, and no gradient lies in what is written,
+// but for one that is its own parameter.
+static int32_t adam_buffers(const AdamList &l, const AdamCommon &c, int64_t blocks) {
+  typedef std::pair<uintptr_t, uintptr_t> Range;
+  std::vector<Range> written;
+  written.reserve(2 * (size_t)l.count + 4);
+  auto add = [&](const void *p, int64_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    if (p != nullptr) written.emplace_back(at, at + (uintptr_t)bytes);
+  };
+  const bool bits8 = c.m_scale != nullptr;
+  add(c.m, blocks * kAdamBlock * (bits8 ? 1 : 4));
+  add(c.v, blocks * kAdamBlock * (bits8 ? 1 : 4));
+  add(c.m_scale, blocks * 4);
+  add(c.v_scale, blocks * 4);
   for (int32_t i = 0; i < l.count; ++i) {
     if (l.types[i] < 0 || l.types[i] > 3)
       return fail(NF4S_ERR_INVALID_ARGUMENT, "tensor %d has an unknown type", (int)i);
@@ -468,16 +479,26 @@ static int32_t adam_buffers(const AdamList &l) {
                   (int)i);
     if (!aligned(l.params[i], p) || !aligned(l.grads[i], g) || !aligned(copy, 2))
       return fail(NF4S_ERR_MISALIGNED, "tensor %d is not aligned to its elements", (int)i);
-    const uintptr_t at = reinterpret_cast<uintptr_t>(l.params[i]);
-    written.emplace_back(at, at + (uintptr_t)l.sizes[i] * p);
-    if (copy != nullptr)
-      written.emplace_back(reinterpret_cast<uintptr_t>(copy),
-                           reinterpret_cast<uintptr_t>(copy) + (uintptr_t)l.sizes[i] * 2);
+    add(l.params[i], l.sizes[i] * p);
+    add(copy, l.sizes[i] * 2);
   }
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i)
     if (written[i].first < written[i - 1].second)
-      return fail(NF4S_ERR_INVALID_ARGUMENT, "parameters or copies overlap");
+      return fail(NF4S_ERR_INVALID_ARGUMENT, "parameters, copies or moments overlap");
+  for (int32_t i = 0; i < l.count; ++i) {
+    if (l.sizes[i] == 0) continue;
+    const int p = l.types[i] & 1 ? 2 : 4, g = l.types[i] & 2 ? 2 : 4;
+    if (l.grads[i] == l.params[i] && p == g) continue;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(l.grads[i]);
+    const uintptr_t to = from + (uintptr_t)l.sizes[i] * g;
+    // The first range that ends behind the gradient's begin.
+    const auto at = std::upper_bound(
+        written.begin(), written.end(), from,
+        [](uintptr_t v, const Range &r) { return v < r.second; });
+    if (at != written.end() && at->first < to)
+      return fail(NF4S_ERR_INVALID_ARGUMENT, "gradient %d lies in what is written", (int)i);
+  }
   return NF4S_OK;
 }
 
@@ -507,12 +528,6 @@ int32_t nf4s_adamw_step(void *const *params, const void *const *grads, uint16_t 
       !aligned(device_hyper, 4) || !aligned(grad_scale, 4))
     return fail(NF4S_ERR_MISALIGNED, "m and v must be 16-byte aligned, scales and scalars 4-byte");
   const AdamList l{params, grads, copies, sizes, types, count};
-  try {
-    rc = adam_buffers(l);
-  } catch (const std::exception &e) {
-    rc = fail(NF4S_ERR_INVALID_ARGUMENT, "%d tensors: %s", (int)count, e.what());
-  }
-  if (rc != NF4S_OK) return rc;
   AdamCommon c{};
   c.m = m;
   c.v = v;
@@ -521,6 +536,12 @@ int32_t nf4s_adamw_step(void *const *params, const void *const *grads, uint16_t 
   c.grad_scale = grad_scale;
   c.hyper = device_hyper;
   for (int i = 0; i < kHyper && device_hyper == nullptr; ++i) c.value[i] = hyper[i];
+  try {
+    rc = adam_buffers(l, c, blocks);
+  } catch (const std::exception &e) {
+    rc = fail(NF4S_ERR_INVALID_ARGUMENT, "%d tensors: %s", (int)count, e.what());
+  }
+  if (rc != NF4S_OK) return rc;
   const hipStream_t s = as_stream(stream);
   return m_scale != nullptr ? adam_run<true>(l, c, s) : adam_run<false>(l, c, s);
 }

@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 from .gemm import _workspace_for
-from .nf4 import _ptr, _require_cuda, _stream_ptr
+from .nf4 import _ptr, _require_cuda, _run, _stream_ptr
 
 IGNORE_INDEX = -100
 
@@ -149,15 +149,15 @@ def log_probs_workspace_bytes(m: int, v: int, d: int, top_k: int = 0,
 def _log_probs_workspace_bytes(m: int, v: int, d: int, top_k: int, backward: bool,
                                device: int) -> int:
     out = ctypes.c_int64(0)
-    _lib.check(_lib.load().nf4s_linear_logprob_workspace_size(m, v, d, top_k, int(backward),
-                                                              ctypes.byref(out)))
+    _run(device, _lib.load().nf4s_linear_logprob_workspace_size, m, v, d, top_k, int(backward),
+         ctypes.byref(out))
     return int(out.value)
 
 
 @functools.lru_cache(maxsize=256)
 def _logits_bytes(m: int, v: int, d: int, device: int) -> int:
     out = ctypes.c_int64(0)
-    _lib.check(_lib.load().nf4s_linear_logprob_logits_size(m, v, d, ctypes.byref(out)))
+    _run(device, _lib.load().nf4s_linear_logprob_logits_size, m, v, d, ctypes.byref(out))
     return int(out.value)
 
 
@@ -197,10 +197,11 @@ def linear_log_probs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, to
             logits = torch.empty(need // 4, dtype=torch.float32, device=x.device)
     workspace = _workspace_for(
         _log_probs_workspace_bytes(m, v, d, top_k, False, x.get_device()), workspace, x)
-    _lib.check(_lib.load().nf4s_linear_logprob_fwd(
-        x.data_ptr(), w.data_ptr(), targets.data_ptr(), m, v, d, top_k, ignore_index,
+    _run(
+        x.get_device(), _lib.load().nf4s_linear_logprob_fwd, x.data_ptr(), w.data_ptr(), targets.data_ptr(), m, v, d, top_k, ignore_index,
         logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids),
-        _ptr(logits), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_ptr(x)))
+        _ptr(logits), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        _stream_ptr(x))
     return LogProbs(logp, entropy, lse, top_logp, top_ids, logits)
 
 
@@ -214,8 +215,8 @@ def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     dlogp does not count, its dentropy does.  dw is bf16 unless a float32 ``dw`` is
     given, which the micro-batches of a step may ``accumulate`` into; the gradients of
     the logits enter both products rounded to bf16, as in
-    :func:`linear_cross_entropy_bwd`, divided by the largest ``|dlogp|``.  Tokens with
-    both gradients zero count as zeros times their row of x, which has to be finite."""
+    :func:`linear_cross_entropy_bwd`, divided by the largest ``|dlogp|``.  Kept logits
+    are the forward's: of x and W as they were then.  Tokens with both gradients zero count as zeros times their row of x, which has to be finite."""
     _check_head(x, w, targets)
     _require_cuda(out.lse, out.entropy, dlogp, dentropy, dw)
     m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
@@ -234,10 +235,10 @@ def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     dx = torch.empty_like(x)
     workspace = _workspace_for(
         _log_probs_workspace_bytes(m, v, d, 0, True, x.get_device()), workspace, x)
-    _lib.check(_lib.load().nf4s_linear_logprob_bwd(
-        x.data_ptr(), w.data_ptr(), targets.data_ptr(), out.lse.data_ptr(),
+    _run(
+        x.get_device(), _lib.load().nf4s_linear_logprob_bwd, x.data_ptr(), w.data_ptr(), targets.data_ptr(), out.lse.data_ptr(),
         out.entropy.data_ptr(), _ptr(logits), dlogp.data_ptr(), _ptr(dentropy), m, v, d,
         ignore_index, dx.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32),
         int(accumulate), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        _stream_ptr(x)))
+        _stream_ptr(x))
     return dx, dw

@@ -50,6 +50,16 @@ def _stream_ptr(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+def _run(device: int, fn, *args) -> None:
+    """fn(*args) with ``device`` current: a launch on the default stream goes to the
+    current device, and workgroups are counted there."""
+    if torch._C._cuda_getDevice() == device:
+        _lib.check(fn(*args))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args))
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

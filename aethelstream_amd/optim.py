@@ -21,7 +21,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .nf4 import _ptr, _require_cuda, _stream_ptr
+from .nf4 import _ptr, _require_cuda, _run, _stream_ptr
 
 BLOCK = 128  # elements that share a scale, and what every tensor's moments begin at
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -183,9 +183,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
                                                      for c in copies]),
              array("q", state.sizes), array("i", types)]
     at = [None if a is None else a.buffer_info()[0] for a in lists]
-    _lib.check(_lib.load().nf4s_adamw_step(
-        *at, count, state.m.data_ptr(), state.v.data_ptr(), _ptr(state.m_scale),
-        _ptr(state.v_scale), host, _ptr(hyper), _ptr(grad_scale), _stream_ptr(state.m)))
+    _run(
+        index, _lib.load().nf4s_adamw_step, *at, count, state.m.data_ptr(), state.v.data_ptr(), _ptr(state.m_scale),
+        _ptr(state.v_scale), host, _ptr(hyper), _ptr(grad_scale), _stream_ptr(state.m))
 
 
 def moments(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -196,7 +196,7 @@ def moments(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:
         return state.m, state.v
     m = torch.empty(blocks * BLOCK, dtype=torch.float32, device=state.m.device)
     v = torch.empty_like(m)
-    _lib.check(_lib.load().nf4s_adamw_moments(
-        state.m.data_ptr(), state.v.data_ptr(), state.m_scale.data_ptr(),
-        state.v_scale.data_ptr(), blocks, m.data_ptr(), v.data_ptr(), _stream_ptr(m)))
+    _run(
+        m.get_device(), _lib.load().nf4s_adamw_moments, state.m.data_ptr(), state.v.data_ptr(), state.m_scale.data_ptr(),
+        state.v_scale.data_ptr(), blocks, m.data_ptr(), v.data_ptr(), _stream_ptr(m))
     return m, v

@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from .gemm import _workspace_for
-from .nf4 import _ptr, _stream_ptr
+from .nf4 import _ptr, _run, _stream_ptr
 
 EPS = 1e-6  # of the norms, as the layers' (math.rs:45)
 MAX_HEAD = 1024
@@ -247,18 +247,18 @@ def apply(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, r
     else:
         _heads(out_k, "out_k", q, k.shape)
         _check_out(out_k, "out_k", [k], [q, out_q])
-    _lib.check(_lib.load().nf4s_rotary_fwd(
-        q.data_ptr(), _ptr(k), int(q.dtype == torch.bfloat16), m, hq, hk, d,
+    _run(
+        q.get_device(), _lib.load().nf4s_rotary_fwd, q.data_ptr(), _ptr(k), int(q.dtype == torch.bfloat16), m, hq, hk, d,
         _EIGHT(*q.stride()[:2], *_pair(k), *out_q.stride()[:2], *_pair(out_k)), _ptr(w_q), _ptr(w_k), float(eps), positions.data_ptr(),
         rope.turns.data_ptr(), 2 * rope.turns.shape[0], int(rope.interleaved), float(rope.scale),
-        out_q.data_ptr(), _ptr(out_k), _stream_ptr(q)))
+        out_q.data_ptr(), _ptr(out_k), _stream_ptr(q))
     return out_q, out_k
 
 
 @functools.lru_cache(maxsize=256)
 def _bwd_workspace_bytes(m: int, hq: int, hk: int, d: int, device: int) -> int:
     size = ctypes.c_int64()
-    _lib.check(_lib.load().nf4s_rotary_bwd_workspace_size(m, hq, hk, d, ctypes.byref(size)))
+    _run(device, _lib.load().nf4s_rotary_bwd_workspace_size, m, hq, hk, d, ctypes.byref(size))
     return size.value
 
 
@@ -311,11 +311,11 @@ def apply_bwd(dq: torch.Tensor, dk: Optional[torch.Tensor], positions: torch.Ten
         else:
             workspace = _workspace_for(need, workspace, dq)
         work = workspace.data_ptr()
-    _lib.check(_lib.load().nf4s_rotary_bwd(
-        dq.data_ptr(), _ptr(dk), _ptr(q), _ptr(k), int(dq.dtype == torch.bfloat16), m, hq, hk, d,
+    _run(
+        dq.get_device(), _lib.load().nf4s_rotary_bwd, dq.data_ptr(), _ptr(dk), _ptr(q), _ptr(k), int(dq.dtype == torch.bfloat16), m, hq, hk, d,
         _TWELVE(*dq.stride()[:2], *_pair(dk), *_pair(q), *_pair(k), *out_q.stride()[:2],
                 *_pair(out_k)), _ptr(w_q), _ptr(w_k), float(eps),
         positions.data_ptr(), rope.turns.data_ptr(), 2 * rope.turns.shape[0],
         int(rope.interleaved), float(rope.scale), out_q.data_ptr(), _ptr(out_k), _ptr(dw_q),
-        _ptr(dw_k), work, need, _stream_ptr(dq)))
+        _ptr(dw_k), work, need, _stream_ptr(dq))
     return RotaryGrad(out_q, out_k, dw_q, dw_k)

@@ -467,7 +467,7 @@ int32_t nf4s_rotary_bwd_workspace_size(int64_t m, int64_t hq, int64_t hk, int64_
  * block with an infinity or a NaN has a NaN scale.  The step uses m and v before
  * they are rounded.
  * m and v 16-byte aligned, the tensors to their elements; what is written must not
- * overlap.
+ * overlap, nor hold a gradient other than as its own parameter.
  * ------------------------------------------------------------------------- */
 int32_t nf4s_adamw_step(void *const *params, const void *const *grads, uint16_t *const *copies,
                         const int64_t *sizes, const int32_t *types, int32_t count, void *m,

@@ -277,6 +277,15 @@ def test_past_31_bits():
     assert not p[:-3077].any() and not state.m[:-k].any() and not state.v[:-k].any()
 
 
+def test_gradient_in_its_parameters_place():
+    p, g = _randn((1000,), 1), _randn((1000,), 1)
+    a, b = optim.adamw_state([p]), optim.adamw_state([g])
+    q = g.clone()
+    optim.adamw_step([p], [g], a, 1, LR, BETAS, EPS, WD)
+    optim.adamw_step([q], [q], b, 1, LR, BETAS, EPS, WD)
+    assert torch.equal(p, q) and torch.equal(a.m, b.m)
+
+
 def test_refusals():
     ps, gs, _ = _tensors([256, 100], [(F, F, False)])
     state = optim.adamw_state(ps)
@@ -312,6 +321,8 @@ def test_refusals():
     bad(params=[ps[0], ps[0][100:200]], grads=[gs[0], gs[1]])
     c = torch.zeros(256, dtype=B, device="cuda")
     bad(copies=[c, c[:100]])
+    bad(grads=[gs[0], ps[0][:100]])
+    bad(params=[state.m[:256], ps[1]])
     with pytest.raises(ValueError):
         optim.adamw_state(ps, bits=16)
     with pytest.raises(ValueError):

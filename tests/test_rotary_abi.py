@@ -2,10 +2,13 @@
 (CPU only: the pointers are dummies), and its angles against 64-bit arithmetic."""
 import ctypes
 import math
+import os
+import shutil
+import subprocess
 
 import pytest
 
-from aethelstream_amd import _lib, rotary
+from aethelstream_amd import _lib, build, rotary
 
 INVALID = _lib.NF4S_ERR_INVALID_ARGUMENT
 SHAPE = _lib.NF4S_ERR_UNSUPPORTED_SHAPE
@@ -110,3 +113,17 @@ def test_refuses_host_tensors():
     with pytest.raises(ValueError):
         rotary.apply(q, None, torch.zeros(2, dtype=torch.int64),
                      rotary.Rotary(torch.zeros(4, dtype=torch.int64)))
+
+
+@pytest.mark.skipif(not (os.path.exists(build.HIPCC) or shutil.which(build.HIPCC)),
+                    reason="needs hipcc")
+def test_no_scratch_memory(tmp_path):
+    out = str(tmp_path / "listing.s")
+    subprocess.run([build.HIPCC, *build.HIP_FLAGS, "-S", "--offload-device-only",
+                    os.path.join(build.CSRC, "rotary.hip"), "-o", out], check=True,
+                   capture_output=True)
+    with open(out) as f:
+        text = f.read()
+    kernels = text.count(".amdhsa_kernel ")
+    assert kernels >= 13
+    assert text.count(".amdhsa_private_segment_fixed_size 0\n") == kernels

@@ -339,3 +339,51 @@ def test_refusals():
                dict(w_q=w, w_k=w, q=q, k=k, workspace=torch.empty(1 << 20, dtype=torch.uint8))):
         with pytest.raises(ValueError):
             rotary.apply_bwd(dq, dk, pos, rope, **kw)
+
+
+def test_past_31_bits():
+    """More than 2^31 elements of q, forward and backward: the first and last tokens as a
+    call over them alone, the weights' gradient of a few rows."""
+    m, hq, d = 70000, 240, 128
+    e = torch.cat([torch.arange(5, device="cuda"), torch.arange(m - 5, m, device="cuda")])
+    s = _inputs(5, hq, 2, d, torch.bfloat16, True)
+    q = torch.zeros(m, hq, d, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(m, 2, d, dtype=torch.bfloat16, device="cuda")
+    q[e], k[e] = _randn((10, hq, d), 1, 1.0, q.dtype), _randn((10, 2, d), 2, 1.0, q.dtype)
+    positions = torch.arange(m, device="cuda")
+    rope = _rope(128)
+    print("forward", m, hq, d, flush=True)
+    a, b = rotary.apply(q, k, positions, rope, s["w_q"], s["w_k"])
+    c = rotary.apply(q[e], k[e], positions[e], rope, s["w_q"], s["w_k"])
+    assert torch.equal(a[e], c[0]) and torch.equal(b[e], c[1])
+    assert not a[5:-5].any() and not b[5:-5].any()
+    print("backward", flush=True)
+    g = rotary.apply_bwd(a, b, positions, rope, q, k, s["w_q"], s["w_k"])
+    h = rotary.apply_bwd(a[e], b[e], positions[e], rope, q[e], k[e], s["w_q"], s["w_k"])
+    assert torch.equal(g.dq[e], h.dq) and torch.equal(g.dk[e], h.dk)
+    assert not g.dq[5:-5].any() and not g.dk[5:-5].any()
+    _check_bwd(g.dq[e], g.dw_q, a[e], q[e], s["w_q"], positions[e], rope)
+
+
+def test_runs_on_the_tensors_device(monkeypatch):
+    """With another device current, calls and workspace queries make the tensors' own
+    current (here the one device there is, under a wrong report)."""
+    s = _inputs(9, 4, 2, 64, torch.bfloat16, True)
+    rope = _rope(64)
+    want = rotary.apply_bwd(s["dq"], s["dk"], s["positions"], rope, s["q"], s["k"], s["w_q"],
+                            s["w_k"])
+    seen = []
+    real = torch.cuda.device
+
+    def device(index):
+        seen.append(index)
+        return real(index)
+
+    rotary._bwd_workspace_bytes.cache_clear()
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    got = rotary.apply_bwd(s["dq"], s["dk"], s["positions"], rope, s["q"], s["k"], s["w_q"],
+                           s["w_k"])
+    monkeypatch.undo()
+    assert seen == [0, 0]
+    assert torch.equal(got.dq, want.dq) and torch.equal(got.dw_k, want.dw_k)
