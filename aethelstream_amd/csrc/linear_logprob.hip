@@ -1,6 +1,6 @@
 // linear_logprob.hip - log probabilities of given tokens under a linear head, the
 // entropy of each token's distribution and its most likely alternatives, with the
-// gradients of the first two, without keeping the logits, for gfx950 (MI355X).
+// gradients of the first two, for gfx950 (MI355X).
 //
 // x [M, d] and w [V, d] bf16 (the head of doublepass/src/loss.rs and
 // doublepass/kernels/fused_ce.cu:71-207, whose cross entropy is linear_ce.hip's):
@@ -10,7 +10,9 @@
 //   G_c = ([c = t] a - exp(l_c) (a + h (l_c + H))) / C,  a = dlogp, h = dH,
 //   dx = C G . w,  dw = C G^T . x
 // C is the largest |a| (of |h| if there is none), kept out of the bf16 G as in the
-// cross entropy.  Products accumulate in fp32; maxima, sums and results are fp32.
+// cross entropy.  Products accumulate in fp32; maxima, sums and results are fp32.  The
+// rounding of G leaves dx 0.0017 to 0.0024 (relative) from the exact gradient and dw
+// up to 0.0027, a bf16 result's own rounding being 0.0017.
 //
 // Forward: the tiles of the cross entropy, a lane holding one token's columns.  A
 // half tile leaves its maximum, its sum of exponentials and the sum of e y with y =
@@ -21,8 +23,18 @@
 // maximum (earlier ones first among equals): any other one has k logits before all
 // of its own.  So the logits of the present piece of the vocabulary are stored in
 // fp32, but for half tiles whose maximum does not exceed the k-th best of the pieces
-// before, and one wave a token picks half tiles by their maxima and reads k of
+// before, and one wave a token picks half tiles by their maxima and reads about k of
 // them.  Later columns lose a tie, so what is skipped is never needed.
+// Gradients: G by pieces of the vocabulary, from the logits made again or, where the
+// forward kept them (the caller's memory), from those: a read of 4 M V bytes for a
+// product of 2 M V d.
+//
+// Measured at 4096 tokens, 128000 x 8192: forward 6.2 ms with the logits kept (2 GB;
+// 6.0 without), G of 32000 columns 160 us from them (4.9 TB/s; 1640 made again), dx
+// and dw of a piece 1505 and 1540; all of it 19.2 to 19.8 ms, 25.1 with the logits made
+// again.  77 tokens, 32000 x 4096: 221 us (258).  1000 tokens, 50021 x 5120 with 20
+// alternatives: logits 425 + 44 us (the stores of 200 MB are about 25 of them),
+// alternatives 20, sums 7.
 #include "linear_head.hpp"
 
 namespace nf4s {
