@@ -95,5 +95,5 @@ def test_listing(tmp_path):
         n, found = k.faults()
         tied += n > 0
         assert not found, (name, found[:5])
-    assert tied == 4 and len(kernels) == 11, sorted(kernels)
+    assert tied == 4 and len(kernels) == 13, sorted(kernels)
     assert text.count(".amdhsa_private_segment_fixed_size 0\n") == len(kernels)
