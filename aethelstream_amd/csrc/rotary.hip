@@ -181,7 +181,8 @@ struct RotaryLane {
     }
   }
 
-  __device__ __forceinline__ void store(T *row, const float (&a)[kNP], const float (&b)[kNP]) const {
+  __device__ __forceinline__ void store(T *row, const float (&a)[kNP],
+                                        const float (&b)[kNP]) const {
     if constexpr (kVec) {
       if (!has(0)) return;
       Raw r;

@@ -36,7 +36,8 @@ class AdamWState:
     In 8 bits a value is within 2^-4 (m) or 2^-5 (sqrt(v)) of itself, and values
     below 2^-15 of their block's largest within 2^-19 (2^-20) of that.  A change by less
     than half of such a step is lost, so with beta2 near 1 a block's v follows its
-    gradients up and, while its largest value stays, hardly down."""
+    gradients up and, while its largest value stays, hardly down.  A NaN or an infinity
+    in a block's moments makes its scale, and so all 128 of them, NaN."""
 
     sizes: List[int]
     m: torch.Tensor
@@ -183,9 +184,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
                                                      for c in copies]),
              array("q", state.sizes), array("i", types)]
     at = [None if a is None else a.buffer_info()[0] for a in lists]
-    _run(
-        index, _lib.load().nf4s_adamw_step, *at, count, state.m.data_ptr(), state.v.data_ptr(), _ptr(state.m_scale),
-        _ptr(state.v_scale), host, _ptr(hyper), _ptr(grad_scale), _stream_ptr(state.m))
+    _run(index, _lib.load().nf4s_adamw_step, *at, count, state.m.data_ptr(), state.v.data_ptr(),
+         _ptr(state.m_scale), _ptr(state.v_scale), host, _ptr(hyper), _ptr(grad_scale),
+         _stream_ptr(state.m))
 
 
 def moments(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -196,7 +197,7 @@ def moments(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:
         return state.m, state.v
     m = torch.empty(blocks * BLOCK, dtype=torch.float32, device=state.m.device)
     v = torch.empty_like(m)
-    _run(
-        m.get_device(), _lib.load().nf4s_adamw_moments, state.m.data_ptr(), state.v.data_ptr(), state.m_scale.data_ptr(),
-        state.v_scale.data_ptr(), blocks, m.data_ptr(), v.data_ptr(), _stream_ptr(m))
+    _run(m.get_device(), _lib.load().nf4s_adamw_moments, state.m.data_ptr(), state.v.data_ptr(),
+         state.m_scale.data_ptr(), state.v_scale.data_ptr(), blocks, m.data_ptr(), v.data_ptr(),
+         _stream_ptr(m))
     return m, v

@@ -100,7 +100,7 @@ class RotaryGrad:
 
 def _heads(t: torch.Tensor, name: str, ref: torch.Tensor, shape=None) -> None:
     if t.dim() != 3 or t.dtype != ref.dtype or t.device != ref.device or not t.is_cuda:
-        raise ValueError(f"{name} must be a [M, heads, d] device tensor of one type with the others")
+        raise ValueError(f"{name} must be a [M, heads, d] device tensor of the others' type")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.stride(2) != 1 and t.shape[2] > 1:
@@ -134,8 +134,8 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _check_out(out: torch.Tensor, name: str, own: Sequence[torch.Tensor],
                others: Sequence[torch.Tensor]) -> None:
-    """Raises unless every element of out has a place of its own, and out is one of
-    ``own`` or lies apart from all of them and of ``others``."""
+    """Raises unless every element of out has a place of its own, and out lies apart
+    from each of ``own`` or is it, and apart from all of ``others``."""
     if out.numel() == 0:
         return
     (m, h, d), (st, sh, _) = out.shape, out.stride()
@@ -143,8 +143,8 @@ def _check_out(out: torch.Tensor, name: str, own: Sequence[torch.Tensor],
     heads = (m == 1 or st >= d) and (h == 1 or sh >= (m - 1) * st + d)
     if not (tokens or heads):
         raise ValueError(f"{name} has elements that share a place")
-    mine = any(_same(out, t) for t in own)
-    if not all(_apart(out, t) for t in (others if mine else [*own, *others])):
+    if not all(_same(out, t) or _apart(out, t) for t in own) \
+            or not all(_apart(out, t) for t in others):
         raise ValueError(f"{name} overlaps another tensor that it is not")
 
 
@@ -247,11 +247,12 @@ def apply(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, r
     else:
         _heads(out_k, "out_k", q, k.shape)
         _check_out(out_k, "out_k", [k], [q, out_q])
-    _run(
-        q.get_device(), _lib.load().nf4s_rotary_fwd, q.data_ptr(), _ptr(k), int(q.dtype == torch.bfloat16), m, hq, hk, d,
-        _EIGHT(*q.stride()[:2], *_pair(k), *out_q.stride()[:2], *_pair(out_k)), _ptr(w_q), _ptr(w_k), float(eps), positions.data_ptr(),
-        rope.turns.data_ptr(), 2 * rope.turns.shape[0], int(rope.interleaved), float(rope.scale),
-        out_q.data_ptr(), _ptr(out_k), _stream_ptr(q))
+    _run(q.get_device(), _lib.load().nf4s_rotary_fwd, q.data_ptr(), _ptr(k),
+         int(q.dtype == torch.bfloat16), m, hq, hk, d,
+         _EIGHT(*q.stride()[:2], *_pair(k), *out_q.stride()[:2], *_pair(out_k)), _ptr(w_q),
+         _ptr(w_k), float(eps), positions.data_ptr(), rope.turns.data_ptr(),
+         2 * rope.turns.shape[0], int(rope.interleaved), float(rope.scale), out_q.data_ptr(),
+         _ptr(out_k), _stream_ptr(q))
     return out_q, out_k
 
 
@@ -311,11 +312,11 @@ def apply_bwd(dq: torch.Tensor, dk: Optional[torch.Tensor], positions: torch.Ten
         else:
             workspace = _workspace_for(need, workspace, dq)
         work = workspace.data_ptr()
-    _run(
-        dq.get_device(), _lib.load().nf4s_rotary_bwd, dq.data_ptr(), _ptr(dk), _ptr(q), _ptr(k), int(dq.dtype == torch.bfloat16), m, hq, hk, d,
-        _TWELVE(*dq.stride()[:2], *_pair(dk), *_pair(q), *_pair(k), *out_q.stride()[:2],
-                *_pair(out_k)), _ptr(w_q), _ptr(w_k), float(eps),
-        positions.data_ptr(), rope.turns.data_ptr(), 2 * rope.turns.shape[0],
-        int(rope.interleaved), float(rope.scale), out_q.data_ptr(), _ptr(out_k), _ptr(dw_q),
-        _ptr(dw_k), work, need, _stream_ptr(dq))
+    _run(dq.get_device(), _lib.load().nf4s_rotary_bwd, dq.data_ptr(), _ptr(dk), _ptr(q), _ptr(k),
+         int(dq.dtype == torch.bfloat16), m, hq, hk, d,
+         _TWELVE(*dq.stride()[:2], *_pair(dk), *_pair(q), *_pair(k), *out_q.stride()[:2],
+                 *_pair(out_k)), _ptr(w_q), _ptr(w_k), float(eps), positions.data_ptr(),
+         rope.turns.data_ptr(), 2 * rope.turns.shape[0], int(rope.interleaved),
+         float(rope.scale), out_q.data_ptr(), _ptr(out_k), _ptr(dw_q), _ptr(dw_k), work, need,
+         _stream_ptr(dq))
     return RotaryGrad(out_q, out_k, dw_q, dw_k)

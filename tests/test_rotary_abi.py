@@ -107,6 +107,25 @@ def test_turns():
         rotary.Rotary.from_frequencies([float("nan")], device="cpu")
 
 
+def test_places_of_outputs():
+    """An output is one of its own inputs or lies apart from each of them, and from the
+    others; parts of one row lie apart."""
+    import torch
+    flat = torch.zeros(4 * 6 * 8 + 100)
+    rows = flat[:192].view(4, 6, 8)
+    q, k, rest = rows[:, :3], rows[:, 3:5], rows[:, 5:]
+    rotary._check_out(q, "out", [q], [k, rest])
+    rotary._check_out(k, "out", [], [q, rest])
+    rotary._check_out(q, "out", [q, q], [k])
+    shifted = flat[4:196].view(4, 6, 8)[:, :3]
+    for own, others in (([], [q]), ([shifted], []), ([q, shifted], []), ([shifted, q], []),
+                        ([q], [shifted]), ([rows], [])):
+        with pytest.raises(ValueError):
+            rotary._check_out(q, "out", own, others)
+    with pytest.raises(ValueError):
+        rotary._check_out(flat[:8].expand(4, 3, 8), "out", [], [])
+
+
 def test_refuses_host_tensors():
     import torch
     q = torch.zeros(2, 2, 8, dtype=torch.bfloat16)
