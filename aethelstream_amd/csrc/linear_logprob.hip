@@ -9,8 +9,8 @@
 //   top k: the k largest z_c, equal ones by their index, with their l_c
 //   G_c = ([c = t] a - exp(l_c) (a + h (l_c + H))) / C,  a = dlogp, h = dH,
 //   dx = C G . w,  dw = C G^T . x
-// C is the largest |a| (of |h| if there is none), kept out of the bf16 G as in the
-// cross entropy.  Products accumulate in fp32; maxima, sums and results are fp32.  The
+// C is the largest |a| (of |h| if that is next to nothing), kept out of the bf16 G as in
+// the cross entropy.  Products accumulate in fp32; maxima, sums and results are fp32.  The
 // rounding of G leaves dx 0.0017 to 0.0024 (relative) from the exact gradient and dw
 // up to 0.0027, a bf16 result's own rounding being 0.0017.
 //
@@ -352,12 +352,12 @@ __device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k, int lane, Lp
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)~c);
 }
 
-// The alternatives of a token, by one wave.  Twice the same step, over the half tiles' maxima and over the
-// logits of those that are left: the k-th largest of the 64 lanes' own maxima is
-// reached by k values at least, so what lies below is out.  What remains, about k, is
-// ranked by counting, together with the k best of the pieces before.  Where too many
-// are left because they are equal, the first k by their index are enough and are
-// taken in that order; where they are not equal (which takes logits sorted against
+// The alternatives of a token, by one wave.  Twice the same step, over the half tiles'
+// maxima and over the logits of those that are left: the k-th largest of the 64 lanes'
+// own maxima is reached by k values at least, so what lies below is out.  What remains,
+// about k, is ranked by counting, together with the k best of the pieces before.  Where
+// too many are left because they are equal, the first k by their index are enough and
+// are taken in that order; where they are not equal (which takes logits sorted against
 // the lanes), k rounds over all of them find the k best.
 __device__ __forceinline__ void lp_select(const LpSelect &a, int64_t row, int lane, LpWave &w) {
   const int rounds = (a.slices + 63) / 64;
@@ -691,7 +691,8 @@ __global__ void __launch_bounds__(256) lp_finish_kernel(const LpSelect c, const 
   if (wave == 0) lp_results(a, row, lp_joined(lp_joined(lds[0], lds[1]), lds[2]), lane, 64);
 }
 
-// C = max |dlogp| over the tokens that have one, or max |dentropy|, or 1.
+// C = max |dlogp| over the tokens that have one, or max |dentropy| if that is 2^64 times
+// as large (G would leave fp32's range), or 1.
 __global__ void __launch_bounds__(1024) lp_common_kernel(const float *dlogp, const float *dentropy,
                                                          const int64_t *targets, int64_t ignore,
                                                          int64_t M, float *common) {
@@ -713,7 +714,7 @@ __global__ void __launch_bounds__(1024) lp_common_kernel(const float *dlogp, con
   if (threadIdx.x != 0) return;
   for (int j = 0; j < 2; ++j)
     for (int i = 1; i < 16; ++i) top[j] = fmaxf(top[j], part[j][i]);
-  const float c = top[0] > 0.0f ? top[0] : top[1];
+  const float c = top[0] > 0.0f && top[1] <= top[0] * 0x1p64f ? top[0] : top[1];
   *common = c == 0.0f || c == __builtin_inff() ? 1.0f : c;
 }
 
@@ -872,7 +873,9 @@ static int32_t lp_grad_logits(const void *ctx, const HeadPiece &p) {
     const int64_t from = p.v0 > g.column ? p.v0 : g.column;
     const int64_t to = p.v0 + p.vn < end ? p.v0 + p.vn : end;
     if (g.slices == 0 || from >= to) continue;
-    const int64_t s0 = (from - g.column) / g.width, s1 = ceil_to(to - g.column, g.width);
+    // Whole 64s, as G's rows: of 32 columns the vocabulary's last half tile may be none.
+    const int64_t s0 = (from - g.column) / g.width;
+    const int64_t s1 = ceil_to(up(to - g.column, 64), g.width);
     const int64_t blocks = ceil_to(a.M, 256 / (g.width / 8) * kLpKept);
     hipLaunchKernelGGL(lp_kept_kernel, dim3((uint32_t)((s1 - s0) * blocks)), dim3(256), 0,
                        p.stream, a, g, (int32_t)s0, (int32_t)blocks);

@@ -170,7 +170,8 @@ def linear_log_probs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, to
     logit in order, equal ones by their index, with their log probabilities.  A target
     equal to ``ignore_index`` (no token is given) has logp 0, and the rest as any
     other; a target outside [0, V) has NaN (it is only seen on the device).  A row with
-    a NaN logit, or an infinite largest one, is NaN in everything but ``top_ids``.
+    a NaN logit, or an infinite largest one, is NaN in everything but ``top_ids`` (and
+    the log-sum-exp of -inf alone, -inf).
 
     ``keep_logits``: the result holds the logits in fp32, and the gradients need not
     multiply x . W^T again (a quarter of a training pass' products).  By default
@@ -197,11 +198,10 @@ def linear_log_probs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, to
             logits = torch.empty(need // 4, dtype=torch.float32, device=x.device)
     workspace = _workspace_for(
         _log_probs_workspace_bytes(m, v, d, top_k, False, x.get_device()), workspace, x)
-    _run(
-        x.get_device(), _lib.load().nf4s_linear_logprob_fwd, x.data_ptr(), w.data_ptr(), targets.data_ptr(), m, v, d, top_k, ignore_index,
-        logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids),
-        _ptr(logits), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        _stream_ptr(x))
+    _run(x.get_device(), _lib.load().nf4s_linear_logprob_fwd, x.data_ptr(), w.data_ptr(),
+         targets.data_ptr(), m, v, d, top_k, ignore_index, logp.data_ptr(), lse.data_ptr(),
+         entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids), _ptr(logits), workspace.data_ptr(),
+         workspace.numel() * workspace.element_size(), _stream_ptr(x))
     return LogProbs(logp, entropy, lse, top_logp, top_ids, logits)
 
 
@@ -216,7 +216,8 @@ def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     given, which the micro-batches of a step may ``accumulate`` into; the gradients of
     the logits enter both products rounded to bf16, as in
     :func:`linear_cross_entropy_bwd`, divided by the largest ``|dlogp|``.  Kept logits
-    are the forward's: of x and W as they were then.  Tokens with both gradients zero count as zeros times their row of x, which has to be finite."""
+    are the forward's: of x and W as they were then.  Tokens with both gradients zero
+    count as zeros times their row of x, which has to be finite."""
     _check_head(x, w, targets)
     _require_cuda(out.lse, out.entropy, dlogp, dentropy, dw)
     m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
@@ -235,10 +236,9 @@ def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     dx = torch.empty_like(x)
     workspace = _workspace_for(
         _log_probs_workspace_bytes(m, v, d, 0, True, x.get_device()), workspace, x)
-    _run(
-        x.get_device(), _lib.load().nf4s_linear_logprob_bwd, x.data_ptr(), w.data_ptr(), targets.data_ptr(), out.lse.data_ptr(),
-        out.entropy.data_ptr(), _ptr(logits), dlogp.data_ptr(), _ptr(dentropy), m, v, d,
-        ignore_index, dx.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32),
-        int(accumulate), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        _stream_ptr(x))
+    _run(x.get_device(), _lib.load().nf4s_linear_logprob_bwd, x.data_ptr(), w.data_ptr(),
+         targets.data_ptr(), out.lse.data_ptr(), out.entropy.data_ptr(), _ptr(logits),
+         dlogp.data_ptr(), _ptr(dentropy), m, v, d, ignore_index, dx.data_ptr(), dw.data_ptr(),
+         int(dw.dtype == torch.float32), int(accumulate), workspace.data_ptr(),
+         workspace.numel() * workspace.element_size(), _stream_ptr(x))
     return dx, dw

@@ -542,7 +542,7 @@ int32_t nf4s_linear_logprob_logits_size(int64_t m, int64_t v, int64_t d, int64_t
  *   dx = G . w,  dw = G^T . x
  * with dlogp 0 where the target is ignored; dx, dw, dw_is_f32, accumulate and the
  * rounding of G as for the cross entropy, G divided by the largest |dlogp| (by the
- * largest |dentropy| if there is none).  A token whose gradients are both zero adds
+ * largest |dentropy| if that is 2^64 times as large).  A token whose gradients are both zero adds
  * zeros times its row of x, which has to be finite.
  */
 int32_t nf4s_linear_logprob_bwd(const uint16_t *x, const uint16_t *w, const int64_t *targets,

@@ -270,6 +270,47 @@ def test_kept_logits(m, v, d):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("m,v,d", [(1, 1, 8), (2, 32, 16), (1, 4050, 256), (64, 90, 128),
+                                   (40, 8000, 136), (3, 16401, 64), (100, 4097, 64),
+                                   (300, 2050, 64)])
+def test_workspaces_that_held_something(m, v, d):
+    """Workspaces full of NaN before the calls: all that is read of them is written."""
+    print(m, v, d, flush=True)
+    x, w, t, da = ce._inputs(m, v, d, seed=m + v)
+    dh = ce._randn((m,), 9, 0.5, torch.float32)
+
+    def used(backward, k=0):
+        n = loss.log_probs_workspace_bytes(m, v, d, k, backward)
+        return torch.full((n,), 0xff, dtype=torch.uint8, device="cuda")
+
+    k = min(v, 7)
+    r = loss.linear_log_probs(x, w, t, top_k=k, workspace=used(False, k))
+    _check_forward(x, w, t, r)
+    for keep in (False, True):
+        r = loss.linear_log_probs(x, w, t, workspace=used(False), keep_logits=keep)
+        _check_forward(x, w, t, r)
+        dx, dw = loss.linear_log_probs_bwd(x, w, t, r, da, dh, workspace=used(True))
+        _check_backward(x, w, t, da, dh, r, dx, dw)
+
+
+@pytest.mark.parametrize("size", [1e-36, 1e-20, 1e-9])
+def test_entropy_far_above_log_probabilities(size):
+    """dlogp next to nothing beside dentropy: G stays within its range."""
+    m, v, d = 33, 500, 64
+    x, w, t, da = ce._inputs(m, v, d, seed=41)
+    dh = ce._randn((m,), 9, 1.0, torch.float32)
+    r = loss.linear_log_probs(x, w, t)
+    dx, dw = loss.linear_log_probs_bwd(x, w, t, r, da * size, dh)
+    _check_backward(x, w, t, da * size, dh, r, dx, dw)
+
+
+def test_nothing_but_minus_infinity():
+    x, w, t, _ = ce._inputs(3, 100, 64, seed=5, skip=0.0)
+    x[:, 0], w[:, 0] = 1.0, float("-inf")
+    r = loss.linear_log_probs(x, w, t)
+    assert (r.lse == float("-inf")).all() and r.logp.isnan().all() and r.entropy.isnan().all()
+
+
 def test_entropy_alone_and_tokens_without_gradients():
     m, v, d = 70, 900, 136
     x, w, t, _ = ce._inputs(m, v, d, seed=21)
