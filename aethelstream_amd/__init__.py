@@ -2,7 +2,9 @@
 
 Hand-written HIP kernels behind the C ABI of ``include/nf4stream.h``
 (libnf4stream.so): NF4 quantize / double-quant / dequant and the
-NF4-dequant-fused bf16 MFMA GEMM (forward X.W^T and input-gradient dY.W).
+NF4-dequant-fused bf16 MFMA GEMM (forward X.W^T and input-gradient dY.W).  Around
+it: ``norm``, ``checkpoint``, ``rotary`` (queries and keys), ``loss`` (cross entropy
+and log probabilities of a head) and ``optim`` (AdamW).
 """
 from . import _lib  # noqa: F401
 from .nf4 import (  # noqa: F401
