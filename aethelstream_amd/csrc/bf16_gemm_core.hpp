@@ -161,11 +161,12 @@ struct GcPlace {
 
 // Stages of the rings.  256 x 256 tiles: 3 of L and 2 of R are the 160 KB of a
 // CU.  64 x 256 and 128 x 128 tiles: 2 of each, and two workgroups a CU; 64 x
-// 128: 3 of each and two workgroups.
+// 128: 3 of each and two workgroups; 64 x 64: 5 of each and two workgroups, also the
+// 160 KB.
 template <int kMT, int kNT>
-constexpr int kGcStagesL = kMT * kNT == 4 ? 2 : 3;
+constexpr int kGcStagesL = kMT * kNT == 4 ? 2 : kMT * kNT == 1 ? 5 : 3;
 template <int kMT, int kNT>
-constexpr int kGcStagesR = kMT * kNT == 4 || kMT * kNT == 16 ? 2 : 3;
+constexpr int kGcStagesR = kMT * kNT == 4 || kMT * kNT == 16 ? 2 : kMT * kNT == 1 ? 5 : 3;
 
 template <int kMT, int kNT, bool kLAcross, bool kRAcross>
 struct GcCore {
@@ -174,11 +175,12 @@ struct GcCore {
   using RSide = GcSide<kNT, kRAcross, kWide>;
   static constexpr int kTileL = 64 * kMT, kTileR = 64 * kNT;
   static constexpr int kNL = kGcStagesL<kMT, kNT>, kNR = kGcStagesR<kMT, kNT>;
-  static_assert((kNL == 2 || kNL == 3) && kNR >= 2 && kNR <= kNL, "kInFlight below");
+  static_assert(kNL == kNR || (kNL == 3 && kNR == 2), "kInFlight below");
   static constexpr int kPeriod = kNL == kNR ? kNL : 6;  // steps until both rings are back
-  // DMAs of step t + 2 that may be in flight when step t closes: all, L's, none.
-  static constexpr int kInFlight = kNR == 3 ? LSide::kDmas + RSide::kDmas
-                                            : (kNL == 3 ? LSide::kDmas : 0);
+  // DMAs that may be in flight when step t closes, those of steps t + 2 to t + kNL - 1:
+  // all, or of step t + 2 L's.
+  static constexpr int kInFlight =
+      kNL == kNR ? (kNL - 2) * (LSide::kDmas + RSide::kDmas) : LSide::kDmas;
   static constexpr int kLdsBytes = kNL * LSide::kBytes + kNR * RSide::kBytes;
   static constexpr int kFL = LSide::kFrags, kFR = RSide::kFrags;
   static constexpr int kSub = kFL * kFR;       // MFMAs per sub-step of 32
@@ -295,10 +297,11 @@ struct GcCore {
   }
 
   // The barrier that closes step t: this wave's DMAs of step t + 1 have landed
-  // and its LDS reads of step t have ended.  Those of step t + 2 that are already
-  // issued may be in flight: they were issued after step t + 1's.
+  // and its LDS reads of step t have ended.  Those of the steps from t + 2 on that are
+  // already issued may be in flight: they were issued after step t + 1's.  (Where the
+  // last of them is missing, none may.)
   static __device__ __forceinline__ void close_step(int t, int nsteps) {
-    if (t + 2 < nsteps)
+    if (t + (kNL > 3 ? kNL - 1 : 2) < nsteps)
       step_barrier<kInFlight>();
     else
       step_barrier<0>();
