@@ -721,16 +721,20 @@ __global__ void __launch_bounds__(1024) lp_common_kernel(const float *dlogp, con
 // Launches over the logits: those of the cross entropy, but tiles of 64 x 64, which have
 // more loads in flight, in two cases.  Where each is alone on a CU, a CU's share being
 // half of what it is in tiles of 64 x 128: whole calls of one token, 8000 columns of 8192
-// 66 -> 39 us, of 2048 20.5 -> 18.5, 16000 of 4096 40 -> 30; of 64 tokens 43 -> 33.  And
+// 66 -> 39 us, of 2048 20.5 -> 18.5, 16000 of 4096 40 -> 30; of 64 tokens 43 -> 33; what
+// whole rounds leave of 1000 tokens, 50021 of 5120, 470 -> 456 (with alternatives).  And
 // where two of them fill at least three quarters of the CUs' places, and few tokens
 // leave the rows of x out: one token, 32000 of 4096 58.7 -> 51.8, 28000 of 4096 53 -> 46.
 // (Half full, 17000 of 8192, 73 would become 82; 64 tokens, 28000 of 8192, 93 98.)
 static int lp_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&l)[2]) {
   const int n = ce_tiles(m, v, d, l);
-  if (n != 1 || l[0].mt != 1) return n;
-  const int64_t tiles = ceil_to(m, 64) * ceil_to(v, 64), slots = cu_slots();
-  if (tiles <= slots || (m <= 32 && d >= 2048 && 2 * tiles >= 3 * slots && tiles <= 2 * slots))
-    l[0].nt = 1;
+  const int64_t slots = cu_slots();
+  for (int i = 0; i < n; ++i) {
+    if (l[i].mt != 1) continue;
+    const int64_t tiles = ceil_to(m, 64) * ceil_to(l[i].cols, 64);
+    if (tiles <= slots || (m <= 32 && d >= 2048 && 2 * tiles >= 3 * slots && tiles <= 2 * slots))
+      l[i].nt = 1;
+  }
   return n;
 }
 static int64_t lp_slices(const CeLaunch &l) { return 2 * ceil_to(l.cols, 64 * l.nt); }
