@@ -293,6 +293,39 @@ def test_workspaces_that_held_something(m, v, d):
         _check_backward(x, w, t, da, dh, r, dx, dw)
 
 
+@pytest.mark.parametrize("m,v", [(1, 100), (33, 700)])
+@pytest.mark.parametrize("d", [*range(56, 850, 72), 64, 128, 192, 256, 320, 384, 448, 512, 640])
+def test_every_number_of_steps(m, v, d):
+    """Reductions of 1 to 14 steps of 64, whole ones and with a rest, through the stages
+    of the smallest tiles."""
+    x, w, t, da = ce._inputs(m, v, d, seed=d)
+    dh = ce._randn((m,), 9, 0.5, torch.float32)
+    r = loss.linear_log_probs(x, w, t, top_k=4)
+    _check_forward(x, w, t, r)
+    for keep in (False, True):
+        r = loss.linear_log_probs(x, w, t, keep_logits=keep)
+        _check_forward(x, w, t, r)
+        dx, dw = loss.linear_log_probs_bwd(x, w, t, r, da, dh)
+        _check_backward(x, w, t, da, dh, r, dx, dw)
+
+
+@pytest.mark.parametrize("m,v,d", [(512, 33500, 264), (300, 66000, 136), (256, 66500, 72)])
+def test_columns_behind_whole_rounds(m, v, d):
+    """Two launches over the columns, large tiles and the smallest ones."""
+    print(m, v, d, flush=True)
+    x, w, t, da = ce._inputs(m, v, d, seed=m)
+    t[::3] = v - 1 - torch.arange(len(t[::3]), device="cuda") % 700
+    dh = ce._randn((m,), 9, 0.5, torch.float32)
+    r = loss.linear_log_probs(x, w, t, top_k=9)
+    _check_forward(x, w, t, r)
+    r = loss.linear_log_probs(x, w, t, keep_logits=True)
+    s = loss.linear_log_probs(x, w, t, keep_logits=False)
+    _check_forward(x, w, t, r)
+    got, want = (loss.linear_log_probs_bwd(x, w, t, o, da, dh) for o in (r, s))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    _check_backward(x, w, t, da, dh, r, *got)
+
+
 @pytest.mark.parametrize("size", [1e-36, 1e-20, 1e-9])
 def test_entropy_far_above_log_probabilities(size):
     """dlogp next to nothing beside dentropy: G stays within its range."""
