@@ -39,8 +39,9 @@ def frequencies(rot: int, base: float = 10000.0, factor: float = 1.0,
     ``factor`` > 1 stretches them for contexts that many times longer than trained.
     Without ``trained`` every frequency is divided by it.  With the trained length,
     pairs that turn ``fast`` times or more within it keep theirs, those that turn
-    ``slow`` times or less are divided, with a ramp in the index between, and the
-    values grow by ``0.1 ln(factor) + 1``."""
+    ``slow`` times or less are divided, with a ramp in the index between (from a whole
+    index to a whole one, be it outside the head), and the values grow by
+    ``0.1 ln(factor) + 1``."""
     if rot <= 0 or rot % 2 != 0:
         raise ValueError(f"rot must be positive and even, got {rot}")
     if not (base > 0 and factor >= 1):
@@ -56,9 +57,12 @@ def frequencies(rot: int, base: float = 10000.0, factor: float = 1.0,
     def index(turns: float) -> float:  # of the pair that turns so often within `trained`
         return rot * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    low = max(math.floor(index(fast)), 0)
-    high = min(math.ceil(index(slow)), rot // 2 - 1)
-    ramp = [min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0) for i in range(rot // 2)]
+    # The ramp may begin before the first pair or end behind the last: cut off there, it
+    # would divide a last pair that turns often, or keep a first one that hardly does.
+    low, high = math.floor(index(fast)), math.ceil(index(slow))
+    # (One apart at least, but for a fast and a slow that rounding makes equal.)
+    wide = max(high - low, 1)
+    ramp = [min(max((i - low) / wide, 0.0), 1.0) for i in range(rot // 2)]
     return ([v * (1 - r) + v / factor * r for v, r in zip(f, ramp)],
             0.1 * math.log(factor) + 1.0)
 
