@@ -18,6 +18,13 @@
 // has at least code 1, as it is divided by in the steps that follow.  The step
 // itself uses m and v before they are rounded.  sqrt(v) is correctly rounded, so
 // that codes are the format's and not the machine's.
+// To nearest, a change by less than half the distance of two codes is lost, from 1.6
+// to 3.1 % of r and 3.1 to 6.3 % of m, and a step changes r by (1 - b2) / 2 (g^2 / v - 1)
+// of it, m by (1 - b1) (g / m - 1).  At 0.95 normal gradients change r by 2.5 % down to
+// some 10 % up, enough for the codes' mean to stay within 1 % of fp32 moments; at b2 =
+// 0.99 r of a tenth of the gradients stays 2.6 times too large, at 0.999 3.9 times (and
+// follows the block's largest value instead), at b1 = 0.99 m does not follow a mean that
+// falls to a fifth (2.5 times).  So both are 0.95 at most.
 //
 // A lane takes 8 elements, so a block is 16 lanes, whose maxima meet in DPP moves.
 // All tensors of a launch are one range of chunks; a workgroup finds its tensor by
@@ -45,6 +52,7 @@ constexpr int kAdamBlock = 128;
 constexpr int kAdamEach8 = 8, kAdamEach32 = 4;
 constexpr int kAdamChunk = 4096;  // elements of a workgroup
 constexpr uint32_t kAdamOffset = 0x38000000u;  // 2^-15
+constexpr float kAdamMostBeta = 0.95f;  // of 8-bit moments
 
 enum { kBeta1, kRest1, kBeta2, kRest2, kKeep, kSize, kInvRoot, kEps, kHyper };
 
@@ -214,7 +222,10 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const AdamTable<kCo
   float h[kHyper];
 #pragma unroll
   for (int i = 0; i < kHyper; ++i) h[i] = hyper != nullptr ? hyper[i] : t.c.value[i];
-  const float gs = t.c.grad_scale != nullptr ? *t.c.grad_scale : 1.0f;
+  float gs = t.c.grad_scale != nullptr ? *t.c.grad_scale : 1.0f;
+  // Coefficients of the device that 8-bit moments do not take: all is NaN.
+  if (kBits8 && !(h[kBeta1] <= kAdamMostBeta && h[kBeta2] <= kAdamMostBeta))
+    gs = __builtin_nanf("");
 
   // All loads, then all else.
   float pv[kIter][kEach], gv[kIter][kEach], mv[kIter][kEach], vv[kIter][kEach];
@@ -534,6 +545,11 @@ int32_t nf4s_adamw_step(void *const *params, const void *const *grads, uint16_t 
   if (!aligned(m, 16) || !aligned(v, 16) || !aligned(m_scale, 4) || !aligned(v_scale, 4) ||
       !aligned(device_hyper, 4) || !aligned(grad_scale, 4))
     return fail(NF4S_ERR_MISALIGNED, "m and v must be 16-byte aligned, scales and scalars 4-byte");
+  if (m_scale != nullptr && device_hyper == nullptr &&
+      !(hyper[kBeta1] <= kAdamMostBeta && hyper[kBeta2] <= kAdamMostBeta))
+    return fail(NF4S_ERR_INVALID_ARGUMENT,
+                "8-bit moments take beta1 and beta2 up to 0.95, got %g and %g",
+                (double)hyper[kBeta1], (double)hyper[kBeta2]);
   const AdamList l{params, grads, copies, sizes, types, count};
   AdamCommon c{};
   c.m = m;

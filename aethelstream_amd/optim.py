@@ -24,6 +24,7 @@ from . import _lib
 from .nf4 import _ptr, _require_cuda, _run, _stream_ptr
 
 BLOCK = 128  # elements that share a scale, and what every tensor's moments begin at
+MOST_BETA_8 = 0.95  # beta1 and beta2 with 8-bit moments
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
@@ -34,10 +35,17 @@ class AdamWState:
     with one scale for 128 elements (``m`` int8, ``v`` uint8).
 
     In 8 bits a value is within 2^-4 (m) or 2^-5 (sqrt(v)) of itself, and values
-    below 2^-15 of their block's largest within 2^-19 (2^-20) of that.  A change by less
-    than half of such a step is lost, so with beta2 near 1 a block's v follows its
-    gradients up and, while its largest value stays, hardly down.  A NaN or an infinity
-    in a block's moments makes its scale, and so all 128 of them, NaN."""
+    below 2^-15 of their block's largest within 2^-19 (2^-20) of that.  A NaN or an
+    infinity in a block's moments makes its scale, and so all 128 of them, NaN.
+
+    Rounding is to nearest, so a change by less than half the distance of two codes is
+    lost.  Steps therefore take beta1 and beta2 up to 0.95 (:data:`MOST_BETA_8`) with
+    8-bit moments: there gradients that vary from step to step carry m and sqrt(v)
+    along, within 1 % of 32 bits' on average, also after their size changed.  At beta2 =
+    0.999 sqrt(v) of gradients that grew four times stays at half of what it should be,
+    of a tenth at four times it; at beta1 = 0.98 m keeps the sign of a mean that turned.
+    Gradients that hardly vary in size are followed badly at 0.95 too (they grew: sqrt(v)
+    stays at 0.74; they fell to a tenth: it hardly falls): those need 32 bits."""
 
     sizes: List[int]
     m: torch.Tensor
@@ -144,7 +152,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
     clipping factor).  ``copies``: for each parameter None, or the bfloat16 tensor
     that gets the updated fp32 parameter.  ``hyper``: float32 [8] on the device,
     :func:`coefficients` of the step, in place of step, lr, betas, eps and
-    weight_decay; a captured step needs it to take another step at its replay."""
+    weight_decay; a captured step needs it to take another step at its replay.
+
+    8-bit moments need beta1 and beta2 of at most 0.95, so others than the default; in
+    ``hyper``, which is only seen on the device, larger ones leave parameters and moments
+    NaN."""
     count = len(state.sizes)
     if len(params) != count or len(grads) != count or \
             (copies is not None and len(copies) != count):
@@ -178,6 +190,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
                 raise ValueError(f"{name} must be float32 [{n}] on the moments' device")
     host = None
     if hyper is None:
+        if state.bits == 8 and max(betas) > MOST_BETA_8:
+            raise ValueError(f"8-bit moments take beta1 and beta2 up to {MOST_BETA_8}, got {betas}: "
+                             "the codes would not follow the gradients")
         host = (ctypes.c_float * 8)(*coefficients(step, lr, betas, eps, weight_decay))
     lists = [array("Q", map(_data_ptr, params)), array("Q", map(_data_ptr, grads)),
              None if copies is None else array("Q", [0 if c is None else c.data_ptr()

@@ -465,7 +465,9 @@ int32_t nf4s_rotary_bwd_workspace_size(int64_t m, int64_t hq, int64_t hk, int64_
  *   (bits(|x| / scale + 2^-15) - bits(2^-15)) >> s,  to nearest, ties to even,
  * m with s = 20 in a signed byte, sqrt(v) with s = 19, at least 1 unless v is 0.  A
  * block with an infinity or a NaN has a NaN scale.  The step uses m and v before
- * they are rounded.
+ * they are rounded.  8-bit moments need hyper[0] and hyper[2] of at most 0.95: beyond,
+ * a step's change is less than the codes hold.  Larger ones are an invalid argument;
+ * in device_hyper they leave parameters and moments NaN.
  * m and v 16-byte aligned, the tensors to their elements; what is written must not
  * overlap, nor hold a gradient other than as its own parameter.
  * ------------------------------------------------------------------------- */
