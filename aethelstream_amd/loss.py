@@ -136,6 +136,7 @@ class LogProbs:
     top_logp: Optional[torch.Tensor]  # float32 [M, top_k], with top_k > 0
     top_ids: Optional[torch.Tensor]   # int64 [M, top_k]
     logits: Optional[torch.Tensor] = None  # float32, in the kernels' order, if kept
+    shape: Optional[Tuple[int, int, int]] = None  # tokens, V and d of kept logits
 
 
 def log_probs_workspace_bytes(m: int, v: int, d: int, top_k: int = 0,
@@ -202,7 +203,8 @@ def linear_log_probs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, to
          targets.data_ptr(), m, v, d, top_k, ignore_index, logp.data_ptr(), lse.data_ptr(),
          entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids), _ptr(logits), workspace.data_ptr(),
          workspace.numel() * workspace.element_size(), _stream_ptr(x))
-    return LogProbs(logp, entropy, lse, top_logp, top_ids, logits)
+    return LogProbs(logp, entropy, lse, top_logp, top_ids, logits,
+                    None if logits is None else (m, v, d))
 
 
 def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, out: LogProbs,
@@ -216,8 +218,9 @@ def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     given, which the micro-batches of a step may ``accumulate`` into; the gradients of
     the logits enter both products rounded to bf16, as in
     :func:`linear_cross_entropy_bwd`, divided by the largest ``|dlogp|``.  Kept logits
-    are the forward's: of x and W as they were then.  Tokens with both gradients zero
-    count as zeros times their row of x, which has to be finite."""
+    are the forward's: of x and W as they were then, and of these sizes (``out.shape``).
+    Tokens with both gradients zero count as zeros times their row of x, which has to be
+    finite."""
     _check_head(x, w, targets)
     _require_cuda(out.lse, out.entropy, dlogp, dentropy, dw)
     m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
@@ -229,7 +232,8 @@ def linear_log_probs_bwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     logits = out.logits
     if logits is not None:
         _require_cuda(logits)
-        if logits.dtype != torch.float32 or logits.device != x.device \
+        # Their order goes by all three sizes, other ones may have as many.
+        if logits.dtype != torch.float32 or logits.device != x.device or out.shape != (m, v, d) \
                 or logits.numel() * 4 != _logits_bytes(m, v, d, x.get_device()):
             raise ValueError("out's logits are of another head, or of other tokens")
     dw = _check_dw(dw, accumulate, w, x)
