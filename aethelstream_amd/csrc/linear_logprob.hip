@@ -43,7 +43,9 @@ namespace nf4s {
 constexpr int kLpTop = 32;  // alternatives at most
 // Stored logits of a piece: what the Infinity Cache holds between the two kernels.
 constexpr int64_t kLpPieceBytes = (int64_t)256 << 20;
-// Columns of a piece, whose maxima (of 64 at least) a wave holds in LDS: 16 KB.
+// Columns of a piece, whose half tiles' maxima a wave holds in LDS: 16 KB for 64 columns
+// each.  Half tiles of 32 are at most four a CU (lp_tiles), 1024 of them: 4 KB alone, 12
+// behind whole rounds, whose half tiles have 128.
 constexpr int64_t kLpPieceCols = 1 << 18;
 constexpr int64_t kLpSelectLds = 64 << 10;
 
