@@ -34,9 +34,10 @@ class AdamWState:
     each from a multiple of 128 on (what lies between is zero): fp32, or 8-bit codes
     with one scale for 128 elements (``m`` int8, ``v`` uint8).
 
-    In 8 bits a value is within 2^-4 (m) or 2^-5 (sqrt(v)) of itself, and values
-    below 2^-15 of their block's largest within 2^-19 (2^-20) of that.  A NaN or an
-    infinity in a block's moments makes its scale, and so all 128 of them, NaN.
+    In 8 bits m is off by at most 2^-4 of |m| + 2^-15 s, s its block's largest, and
+    sqrt(v) by 2^-5 of sqrt(v) + 2^-15 s (2^-22 s beside for fp32's own roundings); one
+    that is not zero is 2^-19 s at least, which may be up to that much too large.  A NaN
+    or an infinity in a block's moments makes its scale, and so all 128 of them, NaN.
 
     Rounding is to nearest, so a change by less than half the distance of two codes is
     lost.  Steps therefore take beta1 and beta2 up to 0.95 (:data:`MOST_BETA_8`) with
