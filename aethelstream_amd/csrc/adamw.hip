@@ -192,7 +192,7 @@ __device__ __forceinline__ uint32_t adam_bytes(uint32_t a, uint32_t b, uint32_t 
 // The correctly rounded square root of 0 or of a number in [2^-100, 2^120], in six
 // instructions instead of sixteen: v y with y = rsqrt(v), and half y times what its
 // square leaves.  (Every fp32 number of that range was compared with the correctly
-// rounded root.)
+// rounded root; test_adamw_roots_gpu.py compares all of [1, 4) and samples of any size.)
 __device__ __forceinline__ float adam_root(float v) {
   const float y = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-100f));
   const float s = v * y;

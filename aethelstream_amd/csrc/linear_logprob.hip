@@ -10,9 +10,13 @@
 //   G_c = ([c = t] a - exp(l_c) (a + h (l_c + H))) / C,  a = dlogp, h = dH,
 //   dx = C G . w,  dw = C G^T . x
 // C is the largest |a| (of |h| if that is next to nothing), kept out of the bf16 G as in
-// the cross entropy.  Products accumulate in fp32; maxima, sums and results are fp32.  The
-// rounding of G leaves dx 0.0017 to 0.0024 (relative) from the exact gradient and dw
-// up to 0.0027, a bf16 result's own rounding being 0.0017.
+// the cross entropy.  Products accumulate in fp32; maxima, sums and results are fp32.
+// G is rounded to bf16 because both products are bf16 MFMAs: as two bf16 numbers it would
+// take each of them twice, some 6 and 6 ms more of the 19.8 below.  With all else in 64
+// bits, that rounding and the result's own (0.0017, relative) leave dx of 77 tokens, 32000
+// x 4096, 0.00242 from the exact gradient and dw 0.00177, of 4096 tokens, 128000 x 8192,
+// 0.00233 and 0.00228: what the kernels have, to four digits.  (Up to 0.0027 of other
+// shapes; a dw in fp32 has G's part alone, 0.0007 and 0.0016 of these.)
 //
 // Forward: the tiles of the cross entropy, a lane holding one token's columns.  A
 // half tile leaves its maximum, its sum of exponentials and the sum of e y with y =
@@ -728,7 +732,9 @@ __global__ void __launch_bounds__(1024) lp_common_kernel(const float *dlogp, con
 // whole rounds leave of 1000 tokens, 50021 of 5120, 470 -> 456 (with alternatives).  And
 // where two of them fill at least three quarters of the CUs' places, and few tokens
 // leave the rows of x out: one token, 32000 of 4096 58.7 -> 51.8, 28000 of 4096 53 -> 46.
-// (Half full, 17000 of 8192, 73 would become 82; 64 tokens, 28000 of 8192, 93 98.)
+// (Half full, 17000 of 8192, 73 would become 82; 64 tokens, 28000 of 8192, 93 98.)  A
+// call of more tiles than there are places keeps the larger ones, however full its last
+// round of small ones would be; what whole rounds leave is a launch like any other.
 static int lp_tiles(int64_t m, int64_t v, int64_t d, CeLaunch (&l)[2]) {
   const int n = ce_tiles(m, v, d, l);
   const int64_t slots = cu_slots();

@@ -1,4 +1,4 @@
-"""Cross entropy of a linear head without keeping the logits, and its gradients.
+"""Cross entropy and log probabilities of a linear head, and their gradients.
 
 ``linear_cross_entropy``      loss and log-sum-exp of each token of x . W^T
 ``linear_cross_entropy_bwd``  dX and dW for given gradients of the losses
@@ -9,10 +9,13 @@
 They take the place of the reference's two passes over vocabulary tiles
 (doublepass/src/loss.rs, doublepass/kernels/fused_ce.cu:71-207): the logits live
 in the accumulators of a tile, the gradients are computed in pieces of the
-vocabulary.  x is bf16 [M, d] (the final norm's output), W the bf16 head [V, d],
-targets int64 [M]; losses and log-sum-exp are fp32.  The gradient of the logits
-is an operand of bf16 products and is rounded to bf16 (2^-8 of each entry at
-most), as a bf16 model's own backward pass would; the sums over it are fp32.
+vocabulary.  The cross entropy never stores the logits; ``linear_log_probs`` keeps
+them in fp32 for its gradients, by default while they take no more memory than W
+(``keep_logits``: a pass that only scores says False).  x is bf16 [M, d] (the final
+norm's output), W the bf16 head [V, d], targets int64 [M]; losses and log-sum-exp
+are fp32.  The gradient of the logits is an operand of bf16 products and is rounded
+to bf16 (2^-8 of each entry at most), as a bf16 model's own backward pass would; the
+sums over it are fp32.
 """
 from __future__ import annotations
 
@@ -177,8 +180,9 @@ def linear_log_probs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, to
     ``keep_logits``: the result holds the logits in fp32, and the gradients need not
     multiply x . W^T again (a quarter of a training pass' products).  By default
     (None) where no alternatives are asked for and they take no more memory than W,
-    which is up to d / 2 tokens, 16384 at most; a pass that only scores saves 4 M V
-    bytes and up to a seventh of its time with False."""
+    which is up to d / 2 tokens, 16384 at most; they live as long as the result.  A pass
+    that only scores saves 4 M V bytes (2.1 GB at 4096 tokens, 128000 columns) and up to
+    a seventh of its time with False."""
     _check_head(x, w, targets)
     m, d, v = int(x.shape[0]), int(x.shape[1]), int(w.shape[0])
     top_k = int(top_k)

@@ -192,8 +192,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
     host = None
     if hyper is None:
         if state.bits == 8 and max(betas) > MOST_BETA_8:
-            raise ValueError(f"8-bit moments take beta1 and beta2 up to {MOST_BETA_8}, got {betas}: "
-                             "the codes would not follow the gradients")
+            raise ValueError(f"8-bit moments take beta1 and beta2 up to {MOST_BETA_8}, got {betas}:"
+                             " the codes would not follow the gradients")
         host = (ctypes.c_float * 8)(*coefficients(step, lr, betas, eps, weight_decay))
     lists = [array("Q", map(_data_ptr, params)), array("Q", map(_data_ptr, grads)),
              None if copies is None else array("Q", [0 if c is None else c.data_ptr()

@@ -2,10 +2,10 @@
 
 Queries and keys get their heads' norms and the rotation by position between their
 products and attention; the loss is the advantage-weighted log probability of the
-given tokens with an entropy bonus, taken from the hidden states and the head without
-keeping the logits; an AdamW step updates the fp32 masters, the norms' weights and the
-bf16 head, and the masters are quantized again.  (The attention between is plain torch
-in fp32.)
+given tokens with an entropy bonus, taken from the hidden states and the head (which
+keeps the logits for the gradients while they take no more memory than itself); an
+AdamW step updates the fp32 masters, the norms' weights and the bf16 head, and the
+masters are quantized again.  (The attention between is plain torch in fp32.)
 
     python -m examples.policy_step [--tokens 512 --steps 20]
 """
