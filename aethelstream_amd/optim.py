@@ -46,7 +46,9 @@ class AdamWState:
     0.999 sqrt(v) of gradients that grew four times stays at half of what it should be,
     of a tenth at four times it; at beta1 = 0.98 m keeps the sign of a mean that turned.
     Gradients that hardly vary in size are followed badly at 0.95 too (they grew: sqrt(v)
-    stays at 0.74; they fell to a tenth: it hardly falls): those need 32 bits."""
+    stays at 0.74; they fell to a tenth: it hardly falls): those need 32 bits.  With a
+    gradient of zero |m| falls by a code's distance at least, so that a value whose
+    gradients end comes to rest also where others of its block go on."""
 
     sizes: List[int]
     m: torch.Tensor

@@ -463,7 +463,8 @@ int32_t nf4s_rotary_bwd_workspace_size(int64_t m, int64_t hq, int64_t hk, int64_
  * scale for each 128 elements, the largest |m| and sqrt(v) of them (2^-126 at
  * least): x is held as the magnitude
  *   (bits(|x| / scale + 2^-15) - bits(2^-15)) >> s,  to nearest, ties to even,
- * m with s = 20 in a signed byte, sqrt(v) with s = 19, at least 1 unless v is 0.  A
+ * m with s = 20 in a signed byte, sqrt(v) with s = 19, at least 1 unless v is 0; m of
+ * a zero gradient one lower where it would stand for no less than before the step.  A
  * block with an infinity or a NaN has a NaN scale.  The step uses m and v before
  * they are rounded.  8-bit moments need hyper[0] and hyper[2] of at most 0.95: beyond,
  * a step's change is less than the codes hold.  Larger ones are an invalid argument;
