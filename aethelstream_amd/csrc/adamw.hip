@@ -42,7 +42,7 @@
 // Bound by memory: 28 bytes an element in fp32, 30 with a copy (202 M elements: 1068
 // us, 5.7 TB/s), 10 with 8-bit moments, bf16 parameters and gradients (512 M elements:
 // 931 us, 5.5 TB/s).  The latter was bound by vector instructions, 90 an element (1173
-// us), of which the compiler's square root and division were 26; 64 now.  What 8-bit
+// us), of which the compiler's square root and division were 26; 70 now.  What 8-bit
 // moments stand for, 10 bytes an element: 512 M in 955 us (5.4 TB/s; 1308 with 8 values
 // a lane, whose 16-byte stores leave every other 16 bytes to the next).
 #include <algorithm>
