@@ -48,7 +48,8 @@ class AdamWState:
     Gradients that hardly vary in size are followed badly at 0.95 too (they grew: sqrt(v)
     stays at 0.74; they fell to a tenth: it hardly falls): those need 32 bits.  With a
     gradient of zero |m| falls by a code's distance at least, so that a value whose
-    gradients end comes to rest also where others of its block go on."""
+    gradients end comes to rest also where others of its block go on.  (Gradients of less
+    than some 2^-16 of their block's largest, but not zero, are lost in m's codes.)"""
 
     sizes: List[int]
     m: torch.Tensor
